@@ -943,6 +943,71 @@ int kgat_comm_gather_at(kgat_comm *comm, const void *send, void *recv, const int
 int kgat_comm_alltoallv(kgat_comm *comm, const void *send, const int64_t *send_off, void *recv,
                         const int64_t *recv_off, void *stream);
 
+/* ---- dense-head operators: rows of float, bf16 or fp16 elements ----
+ * Rows may start at any multiple of the element size and lie any ld apart (inputs: also closer than their
+ * width, e.g. 0 for one row shown n times; outputs: at least their width).  Outputs overlap no input unless said so.
+ * Every sum, statistic and weight gradient is held in 32 bits; results do not change from call to call. */
+enum { KGAT_F32 = 0, KGAT_BF16 = 1, KGAT_F16 = 2 };
+
+#define KGAT_NORM_MAX_D (1 << 20)
+
+/* Layer norm over the d columns of n rows (multi_head_attention.py:30, 58, trainable):
+ *   y = (x - mean) rstd * weight + bias,  rstd = 1 / sqrt(var + eps), var the mean squared deviation.
+ * weight / bias [d] are nullable (1 and 0) and of w_dtype: KGAT_F32 or the rows' dtype.  mean / rstd [n] (both or
+ * neither) are what the backward reads.  n = 0 is allowed. */
+int kgat_layer_norm_fwd(int32_t dtype, const void *x, int64_t ldx, int32_t w_dtype, const void *weight,
+                        const void *bias, void *y, int64_t ldy, float *mean, float *rstd, int64_t n, int32_t d,
+                        float eps, void *stream);
+/* Its backward.  g = dy weight, xhat = (x - mean) rstd:
+ *   dx = rstd (g - mean(g) - xhat mean(g xhat)),  dweight = sum_rows dy xhat,  dbias = sum_rows dy.
+ * dx, dweight, dbias (of w_dtype) are nullable: not wanted.  workspace (kgat_layer_norm_bwd_workspace floats) only
+ * where dweight or dbias is.  n = 0 writes zero sums. */
+int64_t kgat_layer_norm_bwd_workspace(int64_t n, int32_t d);
+int kgat_layer_norm_bwd(int32_t dtype, const void *dy, int64_t lddy, const void *x, int64_t ldx, const float *mean,
+                        const float *rstd, int32_t w_dtype, const void *weight, void *dx, int64_t lddx, void *dweight,
+                        void *dbias, int64_t n, int32_t d, float *workspace, int64_t workspace_floats, void *stream);
+
+#define KGAT_ACT8_BLOCK 32
+#define KGAT_ACT8_MAX_D (1 << 20)
+
+/* Activations [n, d] kept in 8 bits for the backward, a power-of-two scale for each 32 columns of a row:
+ *   e = floor(log2 max|x|) - 6 (at least -126),  q = clamp(round_half_even(x 2^-e), -127, 127),  value = q 2^e.
+ * q int8 [n][32 ceil(d / 32)] (16-byte aligned; zeros behind column d), e uint8 [n][ceil(d / 32)] holds e + 127, or
+ * 255 for a block with an infinity or a NaN, which stands for NaN. */
+int kgat_act8_pack(int32_t dtype, const void *x, int64_t ldx, int64_t n, int32_t d, int8_t *q, uint8_t *e,
+                   void *stream);
+/* x [n, d] = the values, rounded once where dtype has fewer bits (fp16's subnormals; bf16 and float hold them). */
+int kgat_act8_unpack(int32_t dtype, const int8_t *q, const uint8_t *e, int64_t n, int32_t d, void *x, int64_t ldx,
+                     void *stream);
+/* A linear layer's weight gradient from its checkpointed input: dW [o][d] = dy^T x, db [o] (nullable) = the column
+ * sums of dy [n, o].  The products are exact (bf16 matrix instructions, dy as one to three bf16 terms) and summed in
+ * 32 bits.  A row of dy with an infinity or a NaN gives NaN.  n = 0 writes zeros. */
+int64_t kgat_act8_wgrad_workspace(int64_t n, int32_t o, int32_t d);
+int kgat_act8_wgrad(int32_t dtype, const void *dy, int64_t lddy, const int8_t *q, const uint8_t *e, int64_t n,
+                    int32_t o, int32_t d, float *dW, float *db, float *workspace, int64_t workspace_floats,
+                    void *stream);
+
+#define KGAT_LOGPROB_MAX_ITEMS 1024
+#define KGAT_LOGPROB_MAX_K 128
+
+/* Log probabilities of t given items under each of `rows` score rows of `cols` items (the distribution that
+ * main.py:70-130 ranks): z = scale * scores (scale in [2^-64, 2^64]), logp[r][i] = z[items[r][i]] - logsumexp z.
+ * stats [4][rows]: the row's largest score, log2 sum 2^((s - max) scale log2 e), the entropy, the logsumexp -- what the
+ * backward reads.  k > 0 (at most KGAT_LOGPROB_MAX_K and cols): the k best items, best first, equal scores by
+ * ascending item, and their log probabilities, [rows][k].  A negative item is padding (logp 0); one >= cols gives NaN.
+ * -inf scores have probability 0; a row of them alone gives logp and logsumexp -inf and entropy 0.  A row with a NaN or
+ * a +inf gives NaN and best items -1.  workspace: kgat_log_prob_workspace floats, 8-byte aligned. */
+int64_t kgat_log_prob_workspace(int32_t rows, int32_t cols, int32_t k);
+int kgat_log_prob_fwd(int32_t dtype, const void *scores, int64_t ld, int32_t rows, int32_t cols, float scale,
+                      const int64_t *items, int32_t t, int32_t k, float *logp, float *stats, int64_t *top_item,
+                      float *top_logp, float *workspace, int64_t workspace_floats, void *stream);
+/* dscores = the gradient of sum dlogp logp + sum dentropy entropy (dentropy [rows] nullable): for each column j
+ *   scale (sum_i dlogp_i [items_i = j] - p_j (sum_i dlogp_i + dentropy (logp_j + entropy))),
+ * padding counts nowhere, a row without a distribution gives 0.  dscores may be scores itself (same ld). */
+int kgat_log_prob_bwd(int32_t dtype, const void *scores, int64_t ld, int32_t rows, int32_t cols, float scale,
+                      const int64_t *items, int32_t t, const float *stats, const float *dlogp, const float *dentropy,
+                      void *dscores, int64_t ld_dscores, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

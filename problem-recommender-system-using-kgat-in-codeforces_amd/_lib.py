@@ -38,6 +38,12 @@ class AdamTensor(ctypes.Structure):
 
 
 KGAT_ADAM_MAX_TENSORS = 16
+KGAT_F32, KGAT_BF16, KGAT_F16 = 0, 1, 2
+KGAT_NORM_MAX_D = 1 << 20
+KGAT_ACT8_BLOCK = 32
+KGAT_ACT8_MAX_D = 1 << 20
+KGAT_LOGPROB_MAX_ITEMS = 1024
+KGAT_LOGPROB_MAX_K = 128
 KGAT_COMM_ID_BYTES = 128
 
 
@@ -244,6 +250,21 @@ _SIGNATURES = {
     "kgat_ids_check_multi": (ctypes.c_int, [ctypes.POINTER(Ids), ctypes.POINTER(c_i64), c_vp, c_vp, c_vp, c_vp]),
     "kgat_gemm_f32": (ctypes.c_int, [c_i32, c_i32, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp,
                                      c_i64, c_i64, c_i64, c_i32, c_vp]),
+    "kgat_layer_norm_fwd": (ctypes.c_int, [c_i32, c_vp, c_i64, c_i32, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_i32,
+                                           c_f32, c_vp]),
+    "kgat_layer_norm_bwd_workspace": (c_i64, [c_i64, c_i32]),
+    "kgat_layer_norm_bwd": (ctypes.c_int, [c_i32, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i32, c_vp, c_vp, c_i64, c_vp,
+                                           c_vp, c_i64, c_i32, c_vp, c_i64, c_vp]),
+    "kgat_act8_pack": (ctypes.c_int, [c_i32, c_vp, c_i64, c_i64, c_i32, c_vp, c_vp, c_vp]),
+    "kgat_act8_unpack": (ctypes.c_int, [c_i32, c_vp, c_vp, c_i64, c_i32, c_vp, c_i64, c_vp]),
+    "kgat_act8_wgrad_workspace": (c_i64, [c_i64, c_i32, c_i32]),
+    "kgat_act8_wgrad": (ctypes.c_int, [c_i32, c_vp, c_i64, c_vp, c_vp, c_i64, c_i32, c_i32, c_vp, c_vp, c_vp, c_i64,
+                                       c_vp]),
+    "kgat_log_prob_workspace": (c_i64, [c_i32, c_i32, c_i32]),
+    "kgat_log_prob_fwd": (ctypes.c_int, [c_i32, c_vp, c_i64, c_i32, c_i32, c_f32, c_vp, c_i32, c_i32, c_vp, c_vp, c_vp,
+                                         c_vp, c_vp, c_i64, c_vp]),
+    "kgat_log_prob_bwd": (ctypes.c_int, [c_i32, c_vp, c_i64, c_i32, c_i32, c_f32, c_vp, c_i32, c_vp, c_vp, c_vp, c_vp,
+                                         c_i64, c_vp]),
     "kgat_comm_load": (ctypes.c_int, [ctypes.c_char_p]),
     "kgat_comm_error_string": (ctypes.c_char_p, [ctypes.c_int]),
     "kgat_comm_unique_id": (ctypes.c_int, [c_vp]),

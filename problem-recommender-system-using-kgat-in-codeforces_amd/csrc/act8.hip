@@ -1,0 +1,395 @@
+// Activations kept in 8 bits between the forward and the backward.
+//
+// A row's columns are cut into blocks of 32.  With A the largest |x| of a block,
+//   e = floor(log2 A) - 6  (at least -126),   q = clamp(round_half_even(x 2^-e), -127, 127),   value = q 2^e,
+// so |x - value| <= 2^(e-1) <= 2^-7 A (one step, 2^-6 A, where x 2^-e lies above 127.5).  A block that holds an
+// infinity or a NaN has the exponent code 255 and stands for NaN in all its columns: a diverged step stays visible.
+// Stored: q as int8 [n, 32 ceil(d/32)] (zeros behind column d), the code e + 127 as one byte a block.
+//
+// The power-of-two scale costs up to one bit against max / 127, and buys exactness: q 2^e has 7 bits of mantissa,
+// so it IS a bf16 number, and the weight gradient dW = dy^T x runs on the bf16 matrix instructions without any
+// further rounding of x.  dy goes in as it is (bf16) or as the exact sum of two (fp16) or three (float) bf16 terms.
+#include "dense.hpp"
+
+namespace kgat {
+
+namespace {
+
+constexpr int kBlock = KGAT_ACT8_BLOCK;
+
+__device__ __forceinline__ float scale_of(uint32_t code) { return __uint_as_float(code << 23); }  // 255: inf
+
+struct Pack {
+  const void* x;
+  int64_t ldx;
+  int8_t* q;
+  uint8_t* e;
+  int64_t n;
+  int32_t d;
+};
+
+// A thread packs one 16-byte vector of a row, the 8 (float) or 4 (16-bit) threads of a block share its maximum.
+template <typename T>
+__global__ __launch_bounds__(256) void act8_pack_kernel(Pack a) {
+  constexpr int V = Vec<T>::N, kLanes = kBlock / V;
+  const int32_t nb = (a.d + kBlock - 1) / kBlock;
+  const uint32_t per_row = static_cast<uint32_t>(nb) * kLanes;  // vectors of a padded row
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * 256;
+  const int64_t row0 = first / per_row;  // uniform
+  const uint32_t at = static_cast<uint32_t>(first - row0 * per_row) + threadIdx.x;
+  const int64_t row = row0 + at / per_row;
+  const int32_t vec = static_cast<int32_t>(at % per_row), c = vec * V;
+  const bool live = row < a.n;
+  const Vec<T> t = load_vec(static_cast<const T*>(a.x) + (live ? row : 0) * a.ldx + c, live ? a.d - c : 0);
+  uint32_t top = 0;
+  float f[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    f[j] = static_cast<float>(t.e[j]);
+    const uint32_t b = __float_as_uint(f[j]) & 0x7FFFFFFFu;  // |f| orders as its bits; inf and NaN are the largest
+    top = top > b ? top : b;
+  }
+#pragma unroll
+  for (int o = 1; o < kLanes; o <<= 1) {
+    const uint32_t b = static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o));
+    top = top > b ? top : b;
+  }
+  if (!live) return;
+  const uint32_t ex = top >> 23;  // biased exponent of the maximum
+  const uint32_t code = ex == 255 ? 255u : ex < 7 ? 1u : ex - 6;
+  const float inv = __uint_as_float((254u - code) << 23);  // 2^-e (code 255: unused)
+  uint32_t w[V / 4] = {};
+  if (code != 255) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int v = static_cast<int>(fminf(fmaxf(rintf(f[j] * inv), -127.f), 127.f));
+      w[j / 4] |= (static_cast<uint32_t>(v) & 255u) << (8 * (j % 4));
+    }
+  }
+  uint32_t* q = reinterpret_cast<uint32_t*>(a.q + row * (static_cast<int64_t>(nb) * kBlock) + c);
+#pragma unroll
+  for (int j = 0; j < V / 4; ++j) q[j] = w[j];
+  if (vec % kLanes == 0) a.e[row * nb + vec / kLanes] = static_cast<uint8_t>(code);
+}
+
+struct Unpack {
+  const int8_t* q;
+  const uint8_t* e;
+  void* x;
+  int64_t ldx;
+  int64_t n;
+  int32_t d;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void act8_unpack_kernel(Unpack a) {
+  constexpr int V = Vec<T>::N;
+  const int32_t nb = (a.d + kBlock - 1) / kBlock;
+  const uint32_t per_row = (static_cast<uint32_t>(a.d) + V - 1) / V;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * 256;
+  const int64_t row0 = first / per_row;
+  const uint32_t at = static_cast<uint32_t>(first - row0 * per_row) + threadIdx.x;
+  const int64_t row = row0 + at / per_row;
+  const int32_t c = static_cast<int32_t>(at % per_row) * V;
+  if (row >= a.n) return;
+  const uint32_t* q = reinterpret_cast<const uint32_t*>(a.q + row * (static_cast<int64_t>(nb) * kBlock) + c);
+  const float s = scale_of(a.e[row * nb + c / kBlock]);
+  Vec<T> t;
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    t.e[j] = static_cast<T>(static_cast<float>(static_cast<int8_t>(q[j / 4] >> (8 * (j % 4)))) * s);
+  store_vec(static_cast<T*>(a.x) + row * a.ldx + c, t, a.d - c);
+}
+
+// ---------------------------------------------------------------------------------------------- weight gradient
+// dW[o, i] = sum_n dy[n, o] x[n, i]: a block takes a 128 x 128 tile of dW and a share of the rows (split over
+// blockIdx.z, the shares' tiles summed in order by act8_join_kernel), 4 waves of 64 x 64 each as 4 x 4 tiles of
+// v_mfma_f32_16x16x32_bf16.  The reduction runs over the rows, which both operands store apart: a thread takes 8
+// rows x 4 columns and turns them in its registers, so that LDS holds [column][row] with the 8 rows of a lane's
+// operand together (one ds_read_b128).  Column 4 c + j of the tile lies at LDS row 32 j + c: the 32 threads of a
+// row write 32 neighbouring LDS rows at a pitch of 36 dwords, which spreads 16 of them over all 64 banks.
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kTile = 128, kDepth = 64;                 // rows of dy and x a step
+constexpr int kLdsPitch = kDepth * 2 + 16;              // bytes
+constexpr int kPlane = kTile * kLdsPitch;
+
+struct Wgrad {
+  const void* dy;
+  int64_t lddy;
+  const int8_t* q;
+  const uint8_t* e;
+  float* out;  // [splits][o][d]
+  int64_t n, per;  // rows, rows of a split
+  int32_t o, d, nb;
+};
+
+template <typename T> constexpr int kPlanes = 3;
+template <> constexpr int kPlanes<__bf16> = 1;
+template <> constexpr int kPlanes<_Float16> = 2;
+
+__device__ __forceinline__ uint32_t high_halves(uint32_t lo, uint32_t hi) {  // [hi's upper 16 : lo's upper 16]
+  return __builtin_amdgcn_perm(hi, lo, 0x07060302);
+}
+
+// f's next bf16 term: its upper 16 bits; what is left of f is exact.
+__device__ __forceinline__ uint32_t take_term(float& f) {
+  const uint32_t h = __float_as_uint(f) & 0xFFFF0000u;
+  f -= __uint_as_float(h);
+  return h;
+}
+
+template <typename T>
+struct Quad {  // 4 columns of one row
+  T e[4];
+};
+
+template <typename T>
+__device__ __forceinline__ Quad<T> load_quad(const T* p, int64_t count) {
+  Quad<T> v;
+  if (count >= 4) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<u32x4*>(v.e) = *reinterpret_cast<const u32x4_any*>(p);
+    } else {
+      typedef u32x2 u32x2_any __attribute__((aligned(2)));
+      *reinterpret_cast<u32x2*>(v.e) = *reinterpret_cast<const u32x2_any*>(p);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v.e[j] = j < count ? p[j] : static_cast<T>(0.f);
+  }
+  return v;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void act8_wgrad_kernel(Wgrad a) {
+  constexpr int P = kPlanes<T>;
+  __shared__ __align__(16) char lds[(P + 1) * kPlane];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int cg = tid & 31, kg = tid >> 5;
+  const int32_t o0 = blockIdx.y * kTile, i0 = blockIdx.x * kTile;
+  const int64_t r0 = blockIdx.z * a.per, r1 = r0 + a.per < a.n ? r0 + a.per : a.n;
+  const int64_t ldq = static_cast<int64_t>(a.nb) * kBlock;
+  const int32_t oc = o0 + cg * 4, ic = i0 + cg * 4;
+  const bool in_i = ic < ldq;
+  floatx4 acc[4][4];
+#pragma unroll
+  for (int m = 0; m < 4; ++m)
+#pragma unroll
+    for (int n = 0; n < 4; ++n) acc[m][n] = floatx4{0.f, 0.f, 0.f, 0.f};
+  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+
+  for (int64_t r = r0; r < r1; r += kDepth) {
+    const int64_t k0 = r + kg * 8;
+    Quad<T> y[8];
+    uint32_t x[8];
+    uint32_t code[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const bool in = k0 + k < r1;
+      y[k] = load_quad(static_cast<const T*>(a.dy) + (in ? k0 + k : 0) * a.lddy + oc, in ? a.o - oc : 0);
+      x[k] = in && in_i ? *reinterpret_cast<const uint32_t*>(a.q + (k0 + k) * ldq + ic) : 0u;
+      code[k] = in && in_i ? a.e[(k0 + k) * a.nb + ic / kBlock] : 1u;
+    }
+    __syncthreads();  // the last step's operands are read
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      char* at = lds + (32 * j + cg) * kLdsPitch + kg * 16;
+      if constexpr (P == 1) {
+        u32x4 w;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t lo = reinterpret_cast<const uint32_t*>(y[2 * k].e)[j >> 1];
+          const uint32_t hi = reinterpret_cast<const uint32_t*>(y[2 * k + 1].e)[j >> 1];
+          w[k] = __builtin_amdgcn_perm(hi, lo, (j & 1) != 0 ? 0x07060302 : 0x05040100);
+        }
+        *reinterpret_cast<u32x4*>(at) = w;
+      } else {
+        float f[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] = static_cast<float>(y[k].e[j]);
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          u32x4 w;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t lo = take_term(f[2 * k]), hi = take_term(f[2 * k + 1]);
+            w[k] = high_halves(lo, hi);
+          }
+          *reinterpret_cast<u32x4*>(at + p * kPlane) = w;
+        }
+      }
+      u32x4 w;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float lo = static_cast<float>(static_cast<int8_t>(x[2 * k] >> (8 * j))) * scale_of(code[2 * k]);
+        const float hi = static_cast<float>(static_cast<int8_t>(x[2 * k + 1] >> (8 * j))) * scale_of(code[2 * k + 1]);
+        w[k] = high_halves(__float_as_uint(lo), __float_as_uint(hi));
+      }
+      *reinterpret_cast<u32x4*>(at + P * kPlane) = w;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < kDepth / 32; ++s) {
+      const int off = (lane & 15) * kLdsPitch + s * 64 + (lane >> 4) * 16;
+      bf16x8 b[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        b[n] = *reinterpret_cast<const bf16x8*>(lds + P * kPlane + (wn + n * 16) * kLdsPitch + off);
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const bf16x8 v = *reinterpret_cast<const bf16x8*>(lds + p * kPlane + (wm + m * 16) * kLdsPitch + off);
+#pragma unroll
+          for (int n = 0; n < 4; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, b[n], acc[m][n], 0, 0, 0);
+        }
+    }
+  }
+  float* out = a.out + static_cast<int64_t>(blockIdx.z) * a.o * a.d;
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const int ln = wn + n * 16 + (lane & 15);
+    const int32_t col = i0 + (ln & 31) * 4 + (ln >> 5);
+    if (col >= a.d) continue;
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int lm = wm + m * 16 + (lane >> 4) * 4 + i;
+        const int32_t row = o0 + (lm & 31) * 4 + (lm >> 5);
+        if (row < a.o) out[static_cast<int64_t>(row) * a.d + col] = acc[m][n][i];
+      }
+  }
+}
+
+// The column sums of dy by row shares: 64 columns a block, its 4 waves every fourth row.
+template <typename T>
+__global__ __launch_bounds__(256) void act8_dbias_kernel(const T* dy, int64_t lddy, int64_t n, int32_t o, int64_t per,
+                                                         float* part) {
+  __shared__ float lds[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int32_t c = blockIdx.x * 64 + lane;
+  const int64_t r0 = blockIdx.y * per, r1 = r0 + per < n ? r0 + per : n;
+  float s = 0.f;
+  if (c < o)
+    for (int64_t r = r0 + wave; r < r1; r += 4) s += static_cast<float>(dy[r * lddy + c]);
+  lds[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0 && c < o) part[static_cast<int64_t>(blockIdx.y) * o + c] = (lds[0][lane] + lds[1][lane]) + (lds[2][lane] + lds[3][lane]);
+}
+
+// out[i] = sum over the parts, in their order, of part[p][i].
+__global__ __launch_bounds__(256) void act8_join_kernel(const float* part, int32_t parts, int64_t n, float* out) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= n) return;
+  float s = 0.f;
+  for (int p = 0; p < parts; ++p) s += part[p * n + i];
+  out[i] = s;
+}
+
+struct Splits {
+  int32_t w, b;  // row shares of dW and of db
+};
+
+Splits wgrad_splits(int64_t n, int32_t o, int32_t d) {
+  const int64_t tiles = static_cast<int64_t>((o + kTile - 1) / kTile) * ((d + kTile - 1) / kTile);
+  int64_t w = (2 * kCUs + tiles - 1) / tiles, most = (n + 511) / 512;
+  if (w > most) w = most;
+  const int64_t strips = (o + 63) / 64;
+  int64_t b = (4 * kCUs + strips - 1) / strips;
+  most = (n + 63) / 64;
+  if (b > most) b = most;
+  return {static_cast<int32_t>(w < 1 ? 1 : w), static_cast<int32_t>(b < 1 ? 1 : b)};
+}
+
+bool act8_shape_ok(int64_t n, int32_t d) { return n >= 0 && d >= 1 && d <= KGAT_ACT8_MAX_D; }
+
+// Blocks of 256 threads for n rows of per_row vectors; -1: more than a launch holds.
+int64_t flat_blocks(int64_t n, int64_t per_row) {
+  if (n > (int64_t{1} << 52) / per_row) return -1;
+  const int64_t b = (n * per_row + 255) / 256;
+  return b > 0x7FFFFFFF ? -1 : b;
+}
+
+}  // namespace
+
+}  // namespace kgat
+
+extern "C" int kgat_act8_pack(int32_t dtype, const void* x, int64_t ldx, int64_t n, int32_t d, int8_t* q, uint8_t* e,
+                              void* stream) {
+  using namespace kgat;
+  if (!x || !q || !e || !act8_shape_ok(n, d) || ldx < 0 || (reinterpret_cast<uintptr_t>(q) & 15))
+    return KGAT_ERR_INVALID;
+  const Pack a{x, ldx, q, e, n, d};
+  return with_dtype(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    const int64_t blocks = flat_blocks(n, static_cast<int64_t>((d + kBlock - 1) / kBlock) * (kBlock / Vec<T>::N));
+    if (blocks < 0) return KGAT_ERR_INVALID;
+    if (n == 0) return KGAT_OK;
+    hipLaunchKernelGGL(act8_pack_kernel<T>, dim3(static_cast<uint32_t>(blocks)), dim3(256), 0,
+                       reinterpret_cast<hipStream_t>(stream), a);
+    KGAT_LAUNCH_CHECK();
+    return KGAT_OK;
+  });
+}
+
+extern "C" int kgat_act8_unpack(int32_t dtype, const int8_t* q, const uint8_t* e, int64_t n, int32_t d, void* x,
+                                int64_t ldx, void* stream) {
+  using namespace kgat;
+  if (!x || !q || !e || !act8_shape_ok(n, d) || ldx < d || (reinterpret_cast<uintptr_t>(q) & 15))
+    return KGAT_ERR_INVALID;
+  const Unpack a{q, e, x, ldx, n, d};
+  return with_dtype(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    const int64_t blocks = flat_blocks(n, (d + Vec<T>::N - 1) / Vec<T>::N);
+    if (blocks < 0) return KGAT_ERR_INVALID;
+    if (n == 0) return KGAT_OK;
+    hipLaunchKernelGGL(act8_unpack_kernel<T>, dim3(static_cast<uint32_t>(blocks)), dim3(256), 0,
+                       reinterpret_cast<hipStream_t>(stream), a);
+    KGAT_LAUNCH_CHECK();
+    return KGAT_OK;
+  });
+}
+
+extern "C" int64_t kgat_act8_wgrad_workspace(int64_t n, int32_t o, int32_t d) {
+  if (!kgat::act8_shape_ok(n, d) || o < 1 || o > KGAT_ACT8_MAX_D) return -1;
+  const kgat::Splits s = kgat::wgrad_splits(n, o, d);
+  return static_cast<int64_t>(s.w) * o * d + static_cast<int64_t>(s.b) * o;
+}
+
+extern "C" int kgat_act8_wgrad(int32_t dtype, const void* dy, int64_t lddy, const int8_t* q, const uint8_t* e,
+                               int64_t n, int32_t o, int32_t d, float* dW, float* db, float* workspace,
+                               int64_t workspace_floats, void* stream) {
+  using namespace kgat;
+  if (!dy || !q || !e || !dW || !act8_shape_ok(n, d) || o < 1 || o > KGAT_ACT8_MAX_D || lddy < 0 ||
+      (reinterpret_cast<uintptr_t>(q) & 15))
+    return KGAT_ERR_INVALID;
+  if (!workspace || workspace_floats < kgat_act8_wgrad_workspace(n, o, d)) return KGAT_ERR_WORKSPACE;
+  const Splits s = wgrad_splits(n, o, d);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  float* part_b = workspace + static_cast<int64_t>(s.w) * o * d;
+  return with_dtype(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    Wgrad a{dy, lddy, q, e, s.w == 1 ? dW : workspace, n, (n + s.w - 1) / s.w, o, d, (d + kBlock - 1) / kBlock};
+    a.per = (a.per + kDepth - 1) / kDepth * kDepth;
+    hipLaunchKernelGGL(act8_wgrad_kernel<T>, dim3((d + kTile - 1) / kTile, (o + kTile - 1) / kTile, s.w), dim3(256), 0,
+                       st, a);
+    KGAT_LAUNCH_CHECK();
+    if (s.w > 1) {
+      const int64_t size = static_cast<int64_t>(o) * d;
+      hipLaunchKernelGGL(act8_join_kernel, dim3(static_cast<uint32_t>((size + 255) / 256)), dim3(256), 0, st, workspace,
+                         s.w, size, dW);
+      KGAT_LAUNCH_CHECK();
+    }
+    if (db != nullptr) {
+      hipLaunchKernelGGL(act8_dbias_kernel<T>, dim3((o + 63) / 64, s.b), dim3(256), 0, st, static_cast<const T*>(dy),
+                         lddy, n, o, (n + s.b - 1) / s.b, part_b);
+      KGAT_LAUNCH_CHECK();
+      hipLaunchKernelGGL(act8_join_kernel, dim3((o + 255) / 256), dim3(256), 0, st, part_b, s.b,
+                         static_cast<int64_t>(o), db);
+      KGAT_LAUNCH_CHECK();
+    }
+    return KGAT_OK;
+  });
+}

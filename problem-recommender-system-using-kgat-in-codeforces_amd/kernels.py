@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+from typing import NamedTuple
 
 import torch
 
@@ -1408,3 +1409,259 @@ def fill(t: torch.Tensor, value: float) -> torch.Tensor:
 
 def zeros(shape, device) -> torch.Tensor:
     return fill(torch.empty(shape, dtype=torch.float32, device=device), 0.0)
+
+
+# ---------------------------------------------------------------- dense-head operators
+# Layer norm, 8-bit activation checkpoints and log probabilities over rows of float32, bfloat16 or float16.  Their
+# inputs may be any 2-D view with unit stride in the last dimension; statistics, sums and weight gradients are float32.
+ROW_DTYPES = {torch.float32: _lib.KGAT_F32, torch.bfloat16: _lib.KGAT_BF16, torch.float16: _lib.KGAT_F16}
+
+
+def _req_rows(t: torch.Tensor, name: str) -> int:
+    """The KGAT_* code of a 2-D row tensor's type (checked as _req does)."""
+    if isinstance(t, torch.Tensor) and t.dtype not in ROW_DTYPES:
+        raise ValueError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
+    _req(t, name, dtype=getattr(t, "dtype", None), dim=2)
+    return ROW_DTYPES[t.dtype]
+
+
+def _req_like(t: torch.Tensor, name: str, like: torch.Tensor, shape, dtype) -> None:
+    """A contiguous tensor of this shape and type on ``like``'s device."""
+    _req(t, name, dtype=dtype, dim=len(shape))
+    if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{name}: contiguous {list(shape)} expected, got {list(t.shape)}")
+    if t.device != like.device:
+        raise ValueError(f"{name}: on {t.device}, the rows are on {like.device}")
+
+
+def _row_call(like: torch.Tensor, name: str, *args) -> None:
+    """One library call on the current stream of ``like``'s device, which need not be the current device."""
+    if like.device.index == torch.cuda.current_device():
+        _lib.call(name, *args, stream_ptr(like.device))
+    else:
+        with torch.cuda.device(like.device):
+            _lib.call(name, *args, stream_ptr(like.device))
+
+
+def _ptr(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+def _norm_weight(t: torch.Tensor | None, name: str, x: torch.Tensor) -> None:
+    if t is None:
+        return
+    if isinstance(t, torch.Tensor) and t.dtype not in (torch.float32, x.dtype):
+        raise ValueError(f"{name}: expected torch.float32 or the rows' {x.dtype}, got {t.dtype}")
+    _req_like(t, name, x, (x.shape[1],), getattr(t, "dtype", None))
+
+
+def layer_norm_fwd(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                   eps: float = 1e-5, stats: bool = False):
+    """y = (x - mean) * rstd * weight + bias over the columns of x [n, d], in x's type (kgat_layer_norm_fwd).
+    weight / bias [d]: float32 or x's type, both of one.  With ``stats``: (y, mean, rstd), float32 [n], what
+    layer_norm_bwd reads."""
+    code = _req_rows(x, "x")
+    n, d = x.shape
+    if not 1 <= d <= _lib.KGAT_NORM_MAX_D:
+        raise ValueError(f"x: width must be in [1, {_lib.KGAT_NORM_MAX_D}], got {d}")
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"eps must be finite and not negative, got {eps}")
+    _norm_weight(weight, "weight", x)
+    _norm_weight(bias, "bias", x)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError("weight and bias must have one type")
+    w_code = ROW_DTYPES[next((t.dtype for t in (weight, bias) if t is not None), torch.float32)]
+    y = torch.empty(n, d, dtype=x.dtype, device=x.device)
+    mr = torch.empty(2, n, dtype=torch.float32, device=x.device) if stats else None
+    mean, rstd = mr.unbind(0) if stats else (None, None)
+    if n:
+        _row_call(x, "kgat_layer_norm_fwd", code, x.data_ptr(), x.stride(0), w_code, _ptr(weight), _ptr(bias),
+                  y.data_ptr(), d, _ptr(mean), _ptr(rstd), n, d, float(eps))
+    return (y, mean, rstd) if stats else y
+
+
+def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                   weight: torch.Tensor | None = None, need_dx: bool = True, need_dweight: bool = True,
+                   need_dbias: bool = True):
+    """(dx, dweight, dbias) of layer_norm_fwd (kgat_layer_norm_bwd), None for what is not needed.  dy has x's shape and
+    type; dweight / dbias have weight's type (float32 without a weight)."""
+    code = _req_rows(x, "x")
+    _req_rows(dy, "dy")
+    n, d = x.shape
+    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
+        raise ValueError("dy must have x's shape, type and device")
+    if not 1 <= d <= _lib.KGAT_NORM_MAX_D:
+        raise ValueError(f"x: width must be in [1, {_lib.KGAT_NORM_MAX_D}], got {d}")
+    _req_like(mean, "mean", x, (n,), torch.float32)
+    _req_like(rstd, "rstd", x, (n,), torch.float32)
+    _norm_weight(weight, "weight", x)
+    w_dtype = torch.float32 if weight is None else weight.dtype
+    dx = torch.empty(n, d, dtype=x.dtype, device=x.device) if need_dx else None
+    dw = torch.empty(d, dtype=w_dtype, device=x.device) if need_dweight else None
+    db = torch.empty(d, dtype=w_dtype, device=x.device) if need_dbias else None
+    ws = None
+    if need_dweight or need_dbias:
+        if n == 0:
+            return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
+        ws = torch.empty(max(1, int(_lib.lib().kgat_layer_norm_bwd_workspace(n, d))), dtype=torch.float32,
+                         device=x.device)
+    if n and (need_dx or ws is not None):
+        _row_call(x, "kgat_layer_norm_bwd", code, dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0),
+                  mean.data_ptr(), rstd.data_ptr(), ROW_DTYPES[w_dtype], _ptr(weight), _ptr(dx), d, _ptr(dw), _ptr(db),
+                  n, d, _ptr(ws), 0 if ws is None else ws.numel())
+    return dx, dw, db
+
+
+class Act8:
+    """Activations [n, d] kept in 8 bits (act8_pack): ``q`` int8 [n, 32 * ceil(d / 32)] and ``e`` uint8
+    [n, ceil(d / 32)], the power-of-two scale of each 32 columns of a row (value = q * 2^(e - 127); e = 255: NaN).
+    ``dtype`` is the packed tensor's type.  1.03 bytes an element against 4 or 2."""
+    __slots__ = ("q", "e", "shape", "dtype")
+
+    def __init__(self, q: torch.Tensor, e: torch.Tensor, shape: tuple[int, int], dtype: torch.dtype):
+        self.q, self.e, self.shape, self.dtype = q, e, shape, dtype
+
+    @property
+    def device(self) -> torch.device:
+        return self.q.device
+
+    def nbytes(self) -> int:
+        return self.q.numel() + self.e.numel()
+
+
+def _req_act8(a) -> tuple[int, int]:
+    if not isinstance(a, Act8):
+        raise ValueError("expected an act8_pack result")
+    n, d = a.shape
+    nb = (d + _lib.KGAT_ACT8_BLOCK - 1) // _lib.KGAT_ACT8_BLOCK
+    _req_like(a.q, "q", a.q, (n, nb * _lib.KGAT_ACT8_BLOCK), torch.int8)
+    _req_like(a.e, "e", a.q, (n, nb), torch.uint8)
+    if a.q.data_ptr() % 16:
+        raise ValueError("q must be 16-byte aligned")
+    return n, d
+
+
+def act8_pack(x: torch.Tensor) -> Act8:
+    """x [n, d] in 8 bits with a power-of-two scale for each 32 columns of a row (kgat_act8_pack): within 2^-7 of each
+    block's largest absolute value (2^-6 in its topmost 1/255).  A block with an infinity or a NaN becomes NaN."""
+    code = _req_rows(x, "x")
+    n, d = x.shape
+    if not 1 <= d <= _lib.KGAT_ACT8_MAX_D:
+        raise ValueError(f"x: width must be in [1, {_lib.KGAT_ACT8_MAX_D}], got {d}")
+    nb = (d + _lib.KGAT_ACT8_BLOCK - 1) // _lib.KGAT_ACT8_BLOCK
+    q = torch.empty(n, nb * _lib.KGAT_ACT8_BLOCK, dtype=torch.int8, device=x.device)
+    e = torch.empty(n, nb, dtype=torch.uint8, device=x.device)
+    if n:
+        _row_call(x, "kgat_act8_pack", code, x.data_ptr(), x.stride(0), n, d, q.data_ptr(), e.data_ptr())
+    return Act8(q, e, (n, d), x.dtype)
+
+
+def act8_unpack(a: Act8, dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The values of a checkpoint as [n, d] in ``dtype`` (default: the packed tensor's), or into ``out`` (any 2-D view
+    with unit stride in the last dimension)."""
+    n, d = _req_act8(a)
+    if out is None:
+        out = torch.empty(n, d, dtype=dtype or a.dtype, device=a.device)
+    elif dtype is not None and out.dtype != dtype:
+        raise ValueError(f"out has {out.dtype}, not {dtype}")
+    code = _req_rows(out, "out")
+    if tuple(out.shape) != (n, d) or out.device != a.device or (n > 1 and out.stride(0) < d):
+        raise ValueError(f"out: [{n}, {d}] rows that do not overlap expected, on {a.device}")
+    if n:
+        _row_call(out, "kgat_act8_unpack", code, a.q.data_ptr(), a.e.data_ptr(), n, d, out.data_ptr(),
+                  max(out.stride(0), d))
+    return out
+
+
+def act8_wgrad(dy: torch.Tensor, a: Act8, bias: bool = True):
+    """(dW, db) of a linear layer y = x W^T + b from its checkpointed input: dW = dy^T x float32 [o, d] and db = the
+    column sums of dy float32 [o] (None without ``bias``).  Exact products, summed in 32 bits (kgat_act8_wgrad)."""
+    n, d = _req_act8(a)
+    code = _req_rows(dy, "dy")
+    o = dy.shape[1]
+    if dy.shape[0] != n or dy.device != a.device:
+        raise ValueError(f"dy: {n} rows on {a.device} expected, got {list(dy.shape)} on {dy.device}")
+    if not 1 <= o <= _lib.KGAT_ACT8_MAX_D:
+        raise ValueError(f"dy: width must be in [1, {_lib.KGAT_ACT8_MAX_D}], got {o}")
+    dW = torch.empty(o, d, dtype=torch.float32, device=dy.device)
+    db = torch.empty(o, dtype=torch.float32, device=dy.device) if bias else None
+    if n == 0:
+        return dW.zero_(), None if db is None else db.zero_()
+    ws = torch.empty(max(1, int(_lib.lib().kgat_act8_wgrad_workspace(n, o, d))), dtype=torch.float32, device=dy.device)
+    _row_call(dy, "kgat_act8_wgrad", code, dy.data_ptr(), dy.stride(0), a.q.data_ptr(), a.e.data_ptr(), n, o, d,
+              dW.data_ptr(), _ptr(db), ws.data_ptr(), ws.numel())
+    return dW, db
+
+
+class LogProbs(NamedTuple):
+    """log_prob_fwd's results: ``logp`` [n, t], ``entropy`` and ``lse`` [n], ``top_items`` int64 and ``top_logp`` [n, k]
+    (None for k = 0), ``stats`` [4, n] (what log_prob_bwd reads; entropy and lse are two of its rows)."""
+    logp: torch.Tensor
+    entropy: torch.Tensor
+    lse: torch.Tensor
+    top_items: torch.Tensor | None
+    top_logp: torch.Tensor | None
+    stats: torch.Tensor
+
+
+def _req_scores(scores: torch.Tensor, items: torch.Tensor, scale: float) -> int:
+    code = _req_rows(scores, "scores")
+    n, c = scores.shape
+    if not 1 <= c < 2 ** 31 or n >= 2 ** 31:
+        raise ValueError(f"scores: 1 to 2^31 - 1 columns and fewer than 2^31 rows expected, got {list(scores.shape)}")
+    _req(items, "items", dtype=torch.int64, dim=2)
+    if items.shape[0] != n or not items.is_contiguous() or items.device != scores.device:
+        raise ValueError(f"items: contiguous [{n}, t] on {scores.device} expected")
+    if items.shape[1] > _lib.KGAT_LOGPROB_MAX_ITEMS:
+        raise ValueError(f"items: at most {_lib.KGAT_LOGPROB_MAX_ITEMS} a row, got {items.shape[1]}")
+    if not 2.0 ** -64 <= scale <= 2.0 ** 64:
+        raise ValueError(f"scale must be in [2^-64, 2^64], got {scale}")
+    return code
+
+
+def log_prob_fwd(scores: torch.Tensor, items: torch.Tensor, k: int = 0, scale: float = 1.0) -> LogProbs:
+    """Log probabilities of the given items (int64 [n, t]) under softmax(scale * scores) of each row of scores [n, c],
+    the row's entropy and logsumexp, and its ``k`` best items (best first, equal scores by ascending item) with theirs,
+    from one pass over the scores (kgat_log_prob_fwd).  A negative item is padding: logp 0; one >= c gives NaN.  -inf
+    scores have probability 0; a row of them alone gives -inf and entropy 0, one with a NaN or a +inf NaN and best
+    items -1."""
+    code = _req_scores(scores, items, scale)
+    (n, c), t = scores.shape, items.shape[1]
+    if not 0 <= k <= min(c, _lib.KGAT_LOGPROB_MAX_K):
+        raise ValueError(f"k must be in [0, min(columns, {_lib.KGAT_LOGPROB_MAX_K})], got {k}")
+    dev = scores.device
+    logp = torch.empty(n, t, dtype=torch.float32, device=dev)
+    stats = torch.empty(4, n, dtype=torch.float32, device=dev)
+    top = torch.empty(n, k, dtype=torch.int64, device=dev) if k else None
+    top_logp = torch.empty(n, k, dtype=torch.float32, device=dev) if k else None
+    if n:
+        need = int(_lib.lib().kgat_log_prob_workspace(n, c, k))
+        ws = torch.empty(need, dtype=torch.float32, device=dev) if need else None
+        _row_call(scores, "kgat_log_prob_fwd", code, scores.data_ptr(), scores.stride(0), n, c, float(scale),
+                  _ptr(items), t, k, _ptr(logp), stats.data_ptr(), _ptr(top), _ptr(top_logp), _ptr(ws), need)
+    return LogProbs(logp, stats[2], stats[3], top, top_logp, stats)
+
+
+def log_prob_bwd(scores: torch.Tensor, items: torch.Tensor, stats: torch.Tensor, dlogp: torch.Tensor,
+                 dentropy: torch.Tensor | None = None, scale: float = 1.0,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+    """The gradient of sum(dlogp * logp) + sum(dentropy * entropy) into the scores, in their type, from log_prob_fwd's
+    ``stats`` (kgat_log_prob_bwd).  ``out`` may be ``scores`` itself: the gradient takes its place."""
+    code = _req_scores(scores, items, scale)
+    n, c = scores.shape
+    _req_like(stats, "stats", scores, (4, n), torch.float32)
+    _req_like(dlogp, "dlogp", scores, tuple(items.shape), torch.float32)
+    if dentropy is not None:
+        _req_like(dentropy, "dentropy", scores, (n,), torch.float32)
+    if out is None:
+        out = torch.empty(n, c, dtype=scores.dtype, device=scores.device)
+    else:
+        _req_rows(out, "out")
+        if out.shape != scores.shape or out.dtype != scores.dtype or out.device != scores.device or \
+                (n > 1 and out.stride(0) < c):
+            raise ValueError("out must have the scores' shape, type and device, and rows that do not overlap")
+    if n:
+        _row_call(scores, "kgat_log_prob_bwd", code, scores.data_ptr(), scores.stride(0), n, c, float(scale),
+                  _ptr(items), items.shape[1], stats.data_ptr(), _ptr(dlogp), _ptr(dentropy), out.data_ptr(),
+                  max(out.stride(0), c))
+    return out
