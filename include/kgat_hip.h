@@ -962,7 +962,7 @@ int kgat_layer_norm_fwd(int32_t dtype, const void *x, int64_t ldx, int32_t w_dty
  *   dx = rstd (g - mean(g) - xhat mean(g xhat)),  dweight = sum_rows dy xhat,  dbias = sum_rows dy.
  * dx, dweight, dbias (of w_dtype) are nullable: not wanted.  workspace (kgat_layer_norm_bwd_workspace floats) only
  * where dweight or dbias is.  n = 0 writes zero sums. */
-int64_t kgat_layer_norm_bwd_workspace(int64_t n, int32_t d);
+int64_t kgat_layer_norm_bwd_workspace(int32_t dtype, int64_t n, int32_t d);
 int kgat_layer_norm_bwd(int32_t dtype, const void *dy, int64_t lddy, const void *x, int64_t ldx, const float *mean,
                         const float *rstd, int32_t w_dtype, const void *weight, void *dx, int64_t lddx, void *dweight,
                         void *dbias, int64_t n, int32_t d, float *workspace, int64_t workspace_floats, void *stream);

@@ -252,7 +252,7 @@ _SIGNATURES = {
                                      c_i64, c_i64, c_i64, c_i32, c_vp]),
     "kgat_layer_norm_fwd": (ctypes.c_int, [c_i32, c_vp, c_i64, c_i32, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_i32,
                                            c_f32, c_vp]),
-    "kgat_layer_norm_bwd_workspace": (c_i64, [c_i64, c_i32]),
+    "kgat_layer_norm_bwd_workspace": (c_i64, [c_i32, c_i64, c_i32]),
     "kgat_layer_norm_bwd": (ctypes.c_int, [c_i32, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i32, c_vp, c_vp, c_i64, c_vp,
                                            c_vp, c_i64, c_i32, c_vp, c_i64, c_vp]),
     "kgat_act8_pack": (ctypes.c_int, [c_i32, c_vp, c_i64, c_i64, c_i32, c_vp, c_vp, c_vp]),

@@ -4,48 +4,82 @@
 //   y  = xhat w + b
 //   g  = dy w,  dx = rstd (g - mean(g) - xhat mean(g xhat))
 //   dw = sum over rows of dy xhat,  db = sum over rows of dy
+#include <type_traits>
+
 #include "dense.hpp"
 
 namespace kgat {
 
 namespace {
 
-// A weight vector of the rows' type or of float, element by element (read once a block).
+// A weight vector, of float or of the rows' type T.
 struct NormVec {
-  const void* p;
+  void* p;
   int32_t dtype;
+  template <typename T>
   __device__ __forceinline__ float at(int64_t j) const {
-    if (dtype == KGAT_F32) return static_cast<const float*>(p)[j];
-    if (dtype == KGAT_BF16) return static_cast<float>(static_cast<const __bf16*>(p)[j]);
-    return static_cast<float>(static_cast<const _Float16*>(p)[j]);
+    return dtype == KGAT_F32 ? static_cast<const float*>(p)[j] : static_cast<float>(static_cast<const T*>(p)[j]);
   }
   __device__ __forceinline__ void put(int64_t j, float v) const {
-    void* q = const_cast<void*>(p);
-    if (dtype == KGAT_F32) static_cast<float*>(q)[j] = v;
-    else if (dtype == KGAT_BF16) static_cast<__bf16*>(q)[j] = static_cast<__bf16>(v);
-    else static_cast<_Float16*>(q)[j] = static_cast<_Float16>(v);
+    if (dtype == KGAT_F32) static_cast<float*>(p)[j] = v;
+    else if (dtype == KGAT_BF16) static_cast<__bf16*>(p)[j] = static_cast<__bf16>(v);
+    else static_cast<_Float16*>(p)[j] = static_cast<_Float16>(v);
   }
 };
 
-// Sums of K values over the G threads of a row (G a power of two; G > 64: the whole block, through LDS).
-template <int G, int K>
-__device__ __forceinline__ void group_sum(float (&v)[K], float* lds) {
+// A thread's columns of a weight vector; `none` behind the last one and where there is no vector.  The branches are
+// uniform and the index is clamped, so no lane takes a path of its own: with a per-element choice of type under the
+// lane's own bound, hipcc 7.2 lost a live address register on the fp16 path.
+template <typename W, int V, int NV>
+__device__ __forceinline__ void load_columns_of(const W* p, int lane, int G, int32_t d, float none, float (&out)[NV][V]) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int c = (i * G + lane) * V + j;
+      const float v = static_cast<float>(p[c < d ? c : d - 1]);
+      out[i][j] = c < d ? v : none;
+    }
+}
+
+template <typename T, int V, int NV>
+__device__ __forceinline__ void load_columns(const NormVec& w, int lane, int G, int32_t d, float none,
+                                             float (&out)[NV][V]) {
+  if (w.p == nullptr) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) out[i][j] = none;
+  } else if (sizeof(T) == 4 || w.dtype == KGAT_F32) {
+    load_columns_of(static_cast<const float*>(w.p), lane, G, d, none, out);
+  } else {
+    load_columns_of(static_cast<const T*>(w.p), lane, G, d, none, out);
+  }
+}
+
+// Sums of K values over the G threads of a row (G a power of two; G > 64: whole waves, through LDS).  Every thread of
+// the block calls it.  `turn` alternates between two LDS halves, so one barrier a sum is enough: who writes a half
+// again has passed the barrier of the sum between, and with it every reader of the half.
+template <int G, int THREADS, int K>
+__device__ __forceinline__ void group_sum(float (&v)[K], float* lds, int& turn) {
 #pragma unroll
   for (int o = (G < 64 ? G : 64) / 2; o > 0; o >>= 1)
 #pragma unroll
     for (int i = 0; i < K; ++i) v[i] += __shfl_xor(v[i], o);
   if constexpr (G > 64) {
-    constexpr int kWaves = G / 64;
+    constexpr int kWaves = THREADS / 64;
     const int wave = threadIdx.x >> 6;
-    __syncthreads();  // the last sum's readers are done with lds
+    float* at = lds + turn * K * kWaves;
+    turn ^= 1;
     if ((threadIdx.x & 63) == 0)
 #pragma unroll
-      for (int i = 0; i < K; ++i) lds[i * kWaves + wave] = v[i];
+      for (int i = 0; i < K; ++i) at[i * kWaves + wave] = v[i];
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < K; ++i) {
       float s = 0.f;
-      for (int w = 0; w < kWaves; ++w) s += lds[i * kWaves + w];
+#pragma unroll
+      for (int w = 0; w < G / 64; ++w) s += at[i * kWaves + wave / (G / 64) * (G / 64) + w];
       v[i] = s;
     }
   }
@@ -64,33 +98,45 @@ struct NormFwd {
   float eps;
 };
 
-// G threads hold a row as NV vectors each.
+// G threads hold a row as NV vectors each, and the weights of their columns over all the rows they take (a row's
+// weights are 8 bytes a column: read again for every row they would be up to four times its own bytes, from the
+// cache).  The next row is on its way while one is normalised.
 template <typename T, int G, int NV, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_fwd_kernel(NormFwd a) {
   constexpr int V = Vec<T>::N;
   __shared__ float lds[2 * (THREADS / 64)];
+  int turn = 0;
   const int lane = threadIdx.x % G;
   const int64_t step = static_cast<int64_t>(gridDim.x) * (THREADS / G);
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (THREADS / G);
   const float d = static_cast<float>(a.d);
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * (THREADS / G) + threadIdx.x / G; row - threadIdx.x / G < a.n;
-       row += step) {
-    const bool live = row < a.n;
-    const T* x = static_cast<const T*>(a.x) + (live ? row : 0) * a.ldx;
-    float v[NV][V];
-    float s[1] = {0.f};
+  float w[NV][V], b[NV][V];
+  load_columns<T>(a.w, lane, G, a.d, 1.f, w);
+  load_columns<T>(a.b, lane, G, a.d, 0.f, b);
+  Vec<T> next[NV];
+  auto fetch = [&](int64_t row) {
+    const T* x = static_cast<const T*>(a.x) + (row < a.n ? row : 0) * a.ldx;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * G + lane) * V;
-      const Vec<T> t = load_vec(x + c, live ? a.d - c : 0);
+      next[i] = load_vec(x + c, row < a.n ? a.d - c : 0);
+    }
+  };
+  fetch(first + threadIdx.x / G);
+  for (int64_t base = first; base < a.n; base += step) {
+    const int64_t row = base + threadIdx.x / G;
+    float v[NV][V];
+    float s[1] = {0.f}, q[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        v[i][j] = static_cast<float>(t.e[j]);
+        v[i][j] = static_cast<float>(next[i].e[j]);
         s[0] += v[i][j];
       }
-    }
-    group_sum<G>(s, lds);
+    if (base + step < a.n) fetch(row + step);
+    group_sum<G, THREADS>(s, lds, turn);
     const float mean = s[0] / d;
-    float q[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -98,28 +144,22 @@ __global__ __launch_bounds__(THREADS) void norm_fwd_kernel(NormFwd a) {
         v[i][j] -= mean;
         if ((i * G + lane) * V + j < a.d) q[0] += v[i][j] * v[i][j];
       }
-    group_sum<G>(q, lds);
+    group_sum<G, THREADS>(q, lds, turn);
     const float rstd = 1.f / sqrtf(q[0] / d + a.eps);
-    if (!live) continue;
-    T* y = static_cast<T*>(a.y) + row * a.ldy;
+    if (row < a.n) {
+      T* y = static_cast<T*>(a.y) + row * a.ldy;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * G + lane) * V;
-      Vec<T> t;
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * G + lane) * V;
+        Vec<T> t;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float r = v[i][j] * rstd;
-        if (c + j < a.d) {
-          if (a.w.p != nullptr) r *= a.w.at(c + j);
-          if (a.b.p != nullptr) r += a.b.at(c + j);
-        }
-        t.e[j] = static_cast<T>(r);
+        for (int j = 0; j < V; ++j) t.e[j] = static_cast<T>(v[i][j] * rstd * w[i][j] + b[i][j]);
+        store_vec(y + c, t, a.d - c);
       }
-      store_vec(y + c, t, a.d - c);
-    }
-    if (lane == 0 && a.mean != nullptr) {
-      a.mean[row] = mean;
-      a.rstd[row] = rstd;
+      if (lane == 0 && a.mean != nullptr) {
+        a.mean[row] = mean;
+        a.rstd[row] = rstd;
+      }
     }
   }
 }
@@ -129,6 +169,7 @@ template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_fwd_wide_kernel(NormFwd a) {
   constexpr int V = Vec<T>::N;
   __shared__ float lds[2 * (THREADS / 64)];
+  int turn = 0;
   const float d = static_cast<float>(a.d);
   for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
@@ -139,7 +180,7 @@ __global__ __launch_bounds__(THREADS) void norm_fwd_wide_kernel(NormFwd a) {
 #pragma unroll
       for (int j = 0; j < V; ++j) s[0] += static_cast<float>(t.e[j]);
     }
-    group_sum<THREADS>(s, lds);
+    group_sum<THREADS, THREADS>(s, lds, turn);
     const float mean = s[0] / d;
     for (int64_t c = threadIdx.x * V; c < a.d; c += THREADS * V) {
       const Vec<T> t = load_vec(x + c, a.d - c);
@@ -149,7 +190,7 @@ __global__ __launch_bounds__(THREADS) void norm_fwd_wide_kernel(NormFwd a) {
         if (c + j < a.d) q[0] += e * e;
       }
     }
-    group_sum<THREADS>(q, lds);
+    group_sum<THREADS, THREADS>(q, lds, turn);
     const float rstd = 1.f / sqrtf(q[0] / d + a.eps);
     for (int64_t c = threadIdx.x * V; c < a.d; c += THREADS * V) {
       Vec<T> t = load_vec(x + c, a.d - c);
@@ -157,8 +198,8 @@ __global__ __launch_bounds__(THREADS) void norm_fwd_wide_kernel(NormFwd a) {
       for (int j = 0; j < V; ++j)
         if (c + j < a.d) {
           float r = (static_cast<float>(t.e[j]) - mean) * rstd;
-          if (a.w.p != nullptr) r *= a.w.at(c + j);
-          if (a.b.p != nullptr) r += a.b.at(c + j);
+          if (a.w.p != nullptr) r *= a.w.template at<T>(c + j);
+          if (a.b.p != nullptr) r += a.b.template at<T>(c + j);
           t.e[j] = static_cast<T>(r);
         }
       store_vec(y + c, t, a.d - c);
@@ -186,11 +227,119 @@ struct NormBwd {
   int32_t parts;
 };
 
+// The backward in one pass over x and dy: G threads hold a row as NV vectors, keep the weights of their columns and
+// the columns' sums of dy xhat and dy over all the rows they take, and write dx.  At the end the block joins its row
+// groups' sums in their order (by lane exchange within a wave, then through LDS) into its part.
+template <typename T, int G, int NV, int THREADS>
+__global__ __launch_bounds__(THREADS) void norm_bwd_kernel(NormBwd a) {
+  constexpr int V = Vec<T>::N, kGroups = THREADS / (G < 64 ? 64 : G);
+  __shared__ float lds[4 * (THREADS / 64)];
+  __shared__ float cols[kGroups > 1 ? G * NV * V : 1];
+  int turn = 0;
+  const int lane = threadIdx.x % G;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (THREADS / G);
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (THREADS / G);
+  const float d = static_cast<float>(a.d);
+  float w[NV][V], dw[NV][V], db[NV][V];
+  load_columns<T>(a.w, lane, G, a.d, 1.f, w);
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) dw[i][j] = db[i][j] = 0.f;
+  Vec<T> nx[NV], ng[NV];
+  float nmean = 0.f, nrstd = 0.f;
+  auto fetch = [&](int64_t row) {
+    const bool live = row < a.n;
+    const T* x = static_cast<const T*>(a.x) + (live ? row : 0) * a.ldx;
+    const T* dy = static_cast<const T*>(a.dy) + (live ? row : 0) * a.lddy;
+    nmean = live ? a.mean[row] : 0.f;
+    nrstd = live ? a.rstd[row] : 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * G + lane) * V;
+      nx[i] = load_vec(x + c, live ? a.d - c : 0);
+      ng[i] = load_vec(dy + c, live ? a.d - c : 0);
+    }
+  };
+  fetch(first + threadIdx.x / G);
+  for (int64_t base = first; base < a.n; base += step) {
+    const int64_t row = base + threadIdx.x / G;
+    const float mean = nmean, rstd = nrstd;
+    float xh[NV][V], g[NV][V];
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        xh[i][j] = (static_cast<float>(nx[i].e[j]) - mean) * rstd;
+        g[i][j] = static_cast<float>(ng[i].e[j]);
+        db[i][j] += g[i][j];
+        dw[i][j] += g[i][j] * xh[i][j];
+        g[i][j] *= w[i][j];
+        s[0] += g[i][j];
+        s[1] += g[i][j] * xh[i][j];
+      }
+    if (base + step < a.n) fetch(row + step);
+    if (a.dx == nullptr) continue;
+    group_sum<G, THREADS>(s, lds, turn);
+    const float mg = s[0] / d, mgx = s[1] / d;
+    if (row < a.n) {
+      T* dx = static_cast<T*>(a.dx) + row * a.lddx;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * G + lane) * V;
+        Vec<T> t;
+#pragma unroll
+        for (int j = 0; j < V; ++j) t.e[j] = static_cast<T>(rstd * (g[i][j] - mg - xh[i][j] * mgx));
+        store_vec(dx + c, t, a.d - c);
+      }
+    }
+  }
+  if (a.part == nullptr) return;
+  auto join = [&](float (&v)[NV][V], int which) {
+    if constexpr (G < 64)
+#pragma unroll
+      for (int o = G; o < 64; o <<= 1)
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int j = 0; j < V; ++j) v[i][j] += __shfl_xor(v[i][j], o);
+    const int group = threadIdx.x / (G < 64 ? 64 : G);
+    if constexpr (kGroups > 1) {
+      __syncthreads();
+      for (int k = 1; k < kGroups; ++k) {  // one group after the other: the sums' order is fixed
+        if (group == k && (threadIdx.x & 63) < G)
+#pragma unroll
+          for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              float* at = cols + (i * V + j) * G + lane;
+              *at = k == 1 ? v[i][j] : *at + v[i][j];
+            }
+        __syncthreads();
+      }
+    }
+    if (group == 0 && (threadIdx.x & 63) < G) {
+      float* to = a.part + (static_cast<int64_t>(blockIdx.x) * 2 + which) * a.d;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const int c = (i * G + lane) * V + j;
+          if (c < a.d) to[c] = kGroups > 1 ? v[i][j] + cols[(i * V + j) * G + lane] : v[i][j];
+        }
+    }
+  };
+  join(dw, 0);
+  join(db, 1);
+}
+
 // dx, a block per row (rows of any width).
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_dx_kernel(NormBwd a) {
   constexpr int V = Vec<T>::N;
-  __shared__ float lds[2 * (THREADS / 64)];
+  __shared__ float lds[4 * (THREADS / 64)];
+  int turn = 0;
   const float d = static_cast<float>(a.d);
   for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
@@ -204,12 +353,12 @@ __global__ __launch_bounds__(THREADS) void norm_dx_kernel(NormBwd a) {
       for (int j = 0; j < V; ++j)
         if (c + j < a.d) {
           float g = static_cast<float>(tg.e[j]);
-          if (a.w.p != nullptr) g *= a.w.at(c + j);
+          if (a.w.p != nullptr) g *= a.w.template at<T>(c + j);
           s[0] += g;
           s[1] += g * ((static_cast<float>(tx.e[j]) - mean) * rstd);
         }
     }
-    group_sum<THREADS>(s, lds);
+    group_sum<THREADS, THREADS>(s, lds, turn);
     const float mg = s[0] / d, mgx = s[1] / d;
     for (int64_t c = threadIdx.x * V; c < a.d; c += THREADS * V) {
       const Vec<T> tx = load_vec(x + c, a.d - c), tg = load_vec(dy + c, a.d - c);
@@ -217,7 +366,7 @@ __global__ __launch_bounds__(THREADS) void norm_dx_kernel(NormBwd a) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         float g = static_cast<float>(tg.e[j]);
-        if (a.w.p != nullptr && c + j < a.d) g *= a.w.at(c + j);
+        if (a.w.p != nullptr && c + j < a.d) g *= a.w.template at<T>(c + j);
         t.e[j] = static_cast<T>(rstd * (g - mg - (static_cast<float>(tx.e[j]) - mean) * rstd * mgx));
       }
       store_vec(dx + c, t, a.d - c);
@@ -267,43 +416,78 @@ __global__ __launch_bounds__(1024) void norm_cols_join_kernel(NormBwd a) {
   if (to.p != nullptr) to.put(c < a.d ? c : c - a.d, s);
 }
 
-template <typename T, int G, int NV, int THREADS>
-int launch_fwd(const NormFwd& a, hipStream_t st) {
-  const int rows = THREADS / G;
-  const int grid = blocks_for(a.n, rows, 1 << 20);
-  hipLaunchKernelGGL((norm_fwd_kernel<T, G, NV, THREADS>), dim3(grid), dim3(THREADS), 0, st, a);
-  KGAT_LAUNCH_CHECK();
-  return KGAT_OK;
+// The rows' shape: G threads a row, NV vectors a thread, E elements of a thread at most; a narrow row shares its wave
+// with others.  f(G, NV) as integral constants; false: wider than 1024 E columns.
+template <typename T, int E, typename F>
+bool with_shape(int32_t d, F&& f) {
+  constexpr int NV = E / Vec<T>::N;
+  const auto use = [&](auto g, auto nv) {
+    f(g, nv);
+    return true;
+  };
+  const std::integral_constant<int, 1> one{};
+  const std::integral_constant<int, NV> all{};
+  const int nvec = (d + Vec<T>::N - 1) / Vec<T>::N;
+  if (nvec <= 8) return use(std::integral_constant<int, 8>{}, one);
+  if (nvec <= 16) return use(std::integral_constant<int, 16>{}, one);
+  if (nvec <= 32) return use(std::integral_constant<int, 32>{}, one);
+  if (nvec <= 64) return use(std::integral_constant<int, 64>{}, one);
+  if (nvec <= 64 * NV) return use(std::integral_constant<int, 64>{}, all);
+  if (nvec <= 128 * NV) return use(std::integral_constant<int, 128>{}, all);
+  if (nvec <= 256 * NV) return use(std::integral_constant<int, 256>{}, all);
+  if (nvec <= 512 * NV) return use(std::integral_constant<int, 512>{}, all);
+  if (nvec <= 1024 * NV) return use(std::integral_constant<int, 1024>{}, all);
+  return false;
 }
+
+// Elements of a thread: the forward keeps two weights beside each, the backward also two sums, which leaves 8 in the
+// 128 registers of a 1024-thread block (16 spilled 34 to 63 of them).
+constexpr int kFwdElems = 16, kBwdElems = 8;
+constexpr int kBwdThreads = 1024;
 
 template <typename T>
 int norm_fwd(const NormFwd& a, hipStream_t st) {
-  const int nvec = (a.d + Vec<T>::N - 1) / Vec<T>::N;
-  if (nvec <= 16) return launch_fwd<T, 16, 1, 256>(a, st);
-  if (nvec <= 64) return launch_fwd<T, 64, 1, 256>(a, st);
-  if (nvec <= 256) return launch_fwd<T, 64, 4, 256>(a, st);
-  if (nvec <= 1024) return launch_fwd<T, 256, 4, 256>(a, st);
-  hipLaunchKernelGGL((norm_fwd_wide_kernel<T, 1024>), dim3(blocks_for(a.n, 1, 1 << 20)), dim3(1024), 0, st, a);
+  const bool done = with_shape<T, kFwdElems>(a.d, [&](auto g, auto nv) {
+    constexpr int G = decltype(g)::value, NV = decltype(nv)::value, kThreads = G > 256 ? G : 256;
+    const int grid = blocks_for(a.n, kThreads / G, kCUs * (2048 / kThreads));  // every thread the chip holds, at most
+    hipLaunchKernelGGL((norm_fwd_kernel<T, G, NV, kThreads>), dim3(grid), dim3(kThreads), 0, st, a);
+  });
+  if (!done)
+    hipLaunchKernelGGL((norm_fwd_wide_kernel<T, 1024>), dim3(blocks_for(a.n, 1, 1 << 20)), dim3(1024), 0, st, a);
   KGAT_LAUNCH_CHECK();
   return KGAT_OK;
 }
 
+// The row shares whose column sums are kept apart.
+template <typename T>
 int norm_parts(int64_t n, int32_t d) {
+  int parts = 0;
+  if (with_shape<T, kBwdElems>(d, [&](auto g, auto) { parts = blocks_for(n, kBwdThreads / decltype(g)::value, kCUs); })) return parts;
   const int64_t cols = (static_cast<int64_t>(d) + 63) / 64;
-  int64_t p = (1024 + cols - 1) / cols;  // about 1024 blocks in all, 16 rows at least in each
+  int64_t p = (1024 + cols - 1) / cols;  // wide rows: about 1024 blocks in all, 16 rows at least in each
   if (p > (n + 15) / 16) p = (n + 15) / 16;
   return p < 1 ? 1 : static_cast<int>(p);
 }
 
 template <typename T>
-int norm_bwd(const NormBwd& a, hipStream_t st) {
-  if (a.dx != nullptr && a.n > 0) {
+int norm_bwd(NormBwd a, hipStream_t st) {
+  const bool cols = a.dw.p != nullptr || a.db.p != nullptr;
+  a.parts = norm_parts<T>(a.n, a.d);
+  if (!cols) a.part = nullptr;
+  const bool done = with_shape<T, kBwdElems>(a.d, [&](auto g, auto nv) {
+    constexpr int G = decltype(g)::value, NV = decltype(nv)::value;
+    hipLaunchKernelGGL((norm_bwd_kernel<T, G, NV, kBwdThreads>), dim3(a.parts), dim3(kBwdThreads), 0, st, a);
+  });
+  KGAT_LAUNCH_CHECK();
+  if (!done && a.dx != nullptr && a.n > 0) {
     hipLaunchKernelGGL((norm_dx_kernel<T, 256>), dim3(blocks_for(a.n, 1, 1 << 20)), dim3(256), 0, st, a);
     KGAT_LAUNCH_CHECK();
   }
-  if (a.dw.p == nullptr && a.db.p == nullptr) return KGAT_OK;
-  hipLaunchKernelGGL(norm_cols_kernel<T>, dim3((a.d + 63) / 64, a.parts), dim3(256), 0, st, a);
-  KGAT_LAUNCH_CHECK();
+  if (!cols) return KGAT_OK;
+  if (!done) {
+    hipLaunchKernelGGL(norm_cols_kernel<T>, dim3((a.d + 63) / 64, a.parts), dim3(256), 0, st, a);
+    KGAT_LAUNCH_CHECK();
+  }
   hipLaunchKernelGGL(norm_cols_join_kernel, dim3((2 * a.d + 63) / 64), dim3(1024), 0, st, a);
   KGAT_LAUNCH_CHECK();
   return KGAT_OK;
@@ -322,15 +506,17 @@ extern "C" int kgat_layer_norm_fwd(int32_t dtype, const void* x, int64_t ldx, in
   if (!x || !y || n < 0 || d < 1 || d > KGAT_NORM_MAX_D || ldx < 0 || ldy < d || !(eps >= 0.f) ||
       (mean == nullptr) != (rstd == nullptr) || !norm_vec_ok(w_dtype, dtype))
     return KGAT_ERR_INVALID;
-  NormFwd a{x, ldx, y, ldy, {weight, w_dtype}, {bias, w_dtype}, mean, rstd, n, d, eps};
+  NormFwd a{x, ldx, y, ldy, {const_cast<void*>(weight), w_dtype}, {const_cast<void*>(bias), w_dtype}, mean, rstd, n, d, eps};
   return with_dtype(dtype, [&](auto t) {
     return n == 0 ? static_cast<int>(KGAT_OK) : norm_fwd<decltype(t)>(a, reinterpret_cast<hipStream_t>(stream));
   });
 }
 
-extern "C" int64_t kgat_layer_norm_bwd_workspace(int64_t n, int32_t d) {
+extern "C" int64_t kgat_layer_norm_bwd_workspace(int32_t dtype, int64_t n, int32_t d) {
+  using namespace kgat;
   if (n < 0 || d < 1 || d > KGAT_NORM_MAX_D) return -1;
-  return static_cast<int64_t>(kgat::norm_parts(n, d)) * 2 * d;
+  if (dtype != KGAT_F32 && dtype != KGAT_BF16 && dtype != KGAT_F16) return -1;
+  return static_cast<int64_t>(dtype == KGAT_F32 ? norm_parts<float>(n, d) : norm_parts<__bf16>(n, d)) * 2 * d;
 }
 
 extern "C" int kgat_layer_norm_bwd(int32_t dtype, const void* dy, int64_t lddy, const void* x, int64_t ldx,
@@ -339,11 +525,11 @@ extern "C" int kgat_layer_norm_bwd(int32_t dtype, const void* dy, int64_t lddy, 
                                    int64_t workspace_floats, void* stream) {
   using namespace kgat;
   if (!dy || !x || !mean || !rstd || n < 0 || d < 1 || d > KGAT_NORM_MAX_D || lddy < 0 || ldx < 0 ||
-      (dx != nullptr && lddx < d) || !norm_vec_ok(w_dtype, dtype))
+      (dx != nullptr && lddx < d) || !norm_vec_ok(w_dtype, dtype) || dtype < KGAT_F32 || dtype > KGAT_F16)
     return KGAT_ERR_INVALID;
   const bool cols = dweight != nullptr || dbias != nullptr;
-  if (cols && (!workspace || workspace_floats < kgat_layer_norm_bwd_workspace(n, d))) return KGAT_ERR_WORKSPACE;
-  NormBwd a{dy, lddy, x, ldx, mean, rstd, {weight, w_dtype}, {dweight, w_dtype}, {dbias, w_dtype}, dx, lddx, n, d,
-            workspace, norm_parts(n, d)};
+  if (cols && (!workspace || workspace_floats < kgat_layer_norm_bwd_workspace(dtype, n, d))) return KGAT_ERR_WORKSPACE;
+  NormBwd a{dy, lddy, x, ldx, mean, rstd, {const_cast<void*>(weight), w_dtype}, {dweight, w_dtype}, {dbias, w_dtype}, dx, lddx, n, d,
+            workspace, 0};
   return with_dtype(dtype, [&](auto t) { return norm_bwd<decltype(t)>(a, reinterpret_cast<hipStream_t>(stream)); });
 }

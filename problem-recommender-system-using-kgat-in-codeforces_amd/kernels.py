@@ -1503,7 +1503,7 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: 
     if need_dweight or need_dbias:
         if n == 0:
             return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
-        ws = torch.empty(max(1, int(_lib.lib().kgat_layer_norm_bwd_workspace(n, d))), dtype=torch.float32,
+        ws = torch.empty(max(1, int(_lib.lib().kgat_layer_norm_bwd_workspace(code, n, d))), dtype=torch.float32,
                          device=x.device)
     if n and (need_dx or ws is not None):
         _row_call(x, "kgat_layer_norm_bwd", code, dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0),

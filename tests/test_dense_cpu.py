@@ -33,9 +33,10 @@ def test_layer_norm_entries_refuse():
         ({"ldy": 7}, INVALID), ({"eps": -1.0}, INVALID), ({"eps": float("nan")}, INVALID), ({"mean": P}, INVALID),
         ({"rstd": P}, INVALID), ({"wt": 1}, INVALID), ({"wt": 9}, INVALID), ({"n": 0}, 0), ({"n": 0, "dtype": 5}, INVALID)])
     lib = L.lib()
-    need = lib.kgat_layer_norm_bwd_workspace(100, 64)
+    need = lib.kgat_layer_norm_bwd_workspace(1, 100, 64)
     assert need >= 128
-    assert lib.kgat_layer_norm_bwd_workspace(-1, 64) == -1 and lib.kgat_layer_norm_bwd_workspace(1, 0) == -1
+    assert lib.kgat_layer_norm_bwd_workspace(0, -1, 64) == -1 and lib.kgat_layer_norm_bwd_workspace(0, 1, 0) == -1
+    assert lib.kgat_layer_norm_bwd_workspace(3, 1, 64) == -1
     bwd = dict(dtype=1, dy=P, lddy=64, x=P, ldx=64, mean=P, rstd=P, wt=0, w=None, dx=P, lddx=64, dw=P, db=P, n=100, d=64,
                ws=P, wsn=need, st=None)
     refused("kgat_layer_norm_bwd", bwd, [
