@@ -102,26 +102,28 @@ __global__ __launch_bounds__(256) void act8_unpack_kernel(Unpack a) {
 }
 
 // ---------------------------------------------------------------------------------------------- weight gradient
-// dW[o, i] = sum_n dy[n, o] x[n, i]: a block takes a 128 x 128 tile of dW and a share of the rows (split over
-// blockIdx.z, the shares' tiles summed in order by act8_join_kernel), 4 waves of 64 x 64 each as 4 x 4 tiles of
-// v_mfma_f32_16x16x32_bf16.  The reduction runs over the rows, which both operands store apart: a thread takes 8
-// rows x 4 columns and turns them in its registers, so that LDS holds [column][row] with the 8 rows of a lane's
-// operand together (one ds_read_b128).  Column 4 c + j of the tile lies at LDS row 32 j + c: the 32 threads of a
-// row write 32 neighbouring LDS rows at a pitch of 36 dwords, which spreads 16 of them over all 64 banks.
+// dW[o, i] = sum_n dy[n, o] x[n, i]: a block of 2 B threads takes a B x B tile of dW and a share of the rows (split
+// over the grid, the shares' tiles summed in order by act8_join_kernel), 64 rows a step.  The reduction runs over the
+// rows, which both operands store apart: a thread takes 8 rows x 4 columns and turns them in its registers (v_perm
+// pairs the halves of two rows; x is decoded on the way: v_cvt_f32_ubyte, one fma with the scale, the upper halves), so
+// that LDS holds [column][row] with the 8 rows of a lane's operand together, one ds_read_b128 for a
+// v_mfma_f32_32x32x16_bf16.  Column 4 c + j of the tile lies at LDS row (B / 4) j + c: the threads of a row write
+// neighbouring LDS rows at a pitch of 36 dwords, which spreads 16 of them over all 64 banks.
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
 
-constexpr int kTile = 128, kDepth = 64;                 // rows of dy and x a step
-constexpr int kLdsPitch = kDepth * 2 + 16;              // bytes
-constexpr int kPlane = kTile * kLdsPitch;
+constexpr int kDepth = 64;                  // rows a step
+constexpr int kLdsPitch = kDepth * 2 + 16;  // bytes
 
 struct Wgrad {
   const void* dy;
   int64_t lddy;
   const int8_t* q;
   const uint8_t* e;
-  float* out;  // [splits][o][d]
-  int64_t n, per;  // rows, rows of a split
+  float* out;      // [splits][o][d]
+  int64_t n, per;  // rows, rows of a split (a multiple of kDepth; every split has one at least)
   int32_t o, d, nb;
+  int32_t tiles_o, tiles_d, splits;
 };
 
 template <typename T> constexpr int kPlanes = 3;
@@ -145,120 +147,208 @@ struct Quad {  // 4 columns of one row
 };
 
 template <typename T>
-__device__ __forceinline__ Quad<T> load_quad(const T* p, int64_t count) {
+__device__ __forceinline__ Quad<T> load_quad(const T* p) {
   Quad<T> v;
-  if (count >= 4) {
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<u32x4*>(v.e) = *reinterpret_cast<const u32x4_any*>(p);
-    } else {
-      typedef u32x2 u32x2_any __attribute__((aligned(2)));
-      *reinterpret_cast<u32x2*>(v.e) = *reinterpret_cast<const u32x2_any*>(p);
-    }
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<u32x4*>(v.e) = *reinterpret_cast<const u32x4_any*>(p);
   } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v.e[j] = j < count ? p[j] : static_cast<T>(0.f);
+    typedef u32x2 u32x2_any __attribute__((aligned(2)));
+    *reinterpret_cast<u32x2*>(v.e) = *reinterpret_cast<const u32x2_any*>(p);
   }
   return v;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void act8_wgrad_kernel(Wgrad a) {
-  constexpr int P = kPlanes<T>;
-  __shared__ __align__(16) char lds[(P + 1) * kPlane];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int cg = tid & 31, kg = tid >> 5;
-  const int32_t o0 = blockIdx.y * kTile, i0 = blockIdx.x * kTile;
-  const int64_t r0 = blockIdx.z * a.per, r1 = r0 + a.per < a.n ? r0 + a.per : a.n;
-  const int64_t ldq = static_cast<int64_t>(a.nb) * kBlock;
-  const int32_t oc = o0 + cg * 4, ic = i0 + cg * 4;
-  const bool in_i = ic < ldq;
-  floatx4 acc[4][4];
-#pragma unroll
-  for (int m = 0; m < 4; ++m)
-#pragma unroll
-    for (int n = 0; n < 4; ++n) acc[m][n] = floatx4{0.f, 0.f, 0.f, 0.f};
-  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+// LDS buffers: two (the next step is written while one is multiplied) where the operands fit twice beside a second
+// block, one and two barriers a step for dy's two and three terms.
+template <typename T> constexpr int kStages = kPlanes<T> == 1 ? 2 : 1;
 
-  for (int64_t r = r0; r < r1; r += kDepth) {
-    const int64_t k0 = r + kg * 8;
-    Quad<T> y[8];
-    uint32_t x[8];
-    uint32_t code[8];
+// NARROW: dy has fewer than 4 columns.
+template <typename T, int B, bool NARROW>
+__global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
+  constexpr int P = kPlanes<T>, kPlane = B * kLdsPitch, kBuffer = (P + 1) * kPlane;
+  // Waves along d; 32 x 32 tiles of a wave along o and d.
+  constexpr int kWavesN = B == 64 ? 2 : B / 64, FM = B == 64 ? 2 : B / 64, FN = B == 64 ? 1 : 2;
+  static_assert(kWavesN * FN * 32 == B && (2 * B / 64) / kWavesN * FM * 32 == B, "the waves cover the tile");
+  __shared__ __align__(16) char lds[kStages<T> * kBuffer];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int cg = tid % (B / 4), kg = tid / (B / 4);
+  // Blocks b, b + 8, ... run on one XCD: give it neighbouring tiles (4 along o at a time), whose operands its L2 shares.
+  const int total = a.tiles_o * a.tiles_d * a.splits;
+  int id = blockIdx.x;
+  if (total % 8 == 0) id = id % 8 * (total / 8) + id / 8;
+  const int split = id / (a.tiles_o * a.tiles_d);
+  id -= split * (a.tiles_o * a.tiles_d);
+  const int strip = id / (4 * a.tiles_d), rows_here = a.tiles_o - strip * 4 < 4 ? a.tiles_o - strip * 4 : 4;
+  id -= strip * 4 * a.tiles_d;
+  const int32_t o0 = (strip * 4 + id % rows_here) * B, i0 = id / rows_here * B;
+
+  const int64_t r0 = split * a.per, r1 = r0 + a.per < a.n ? r0 + a.per : a.n;
+  const int32_t ldq = a.nb * kBlock;
+  // A quad that would pass the last column starts earlier: its columns are computed twice, and written twice with the
+  // same value.
+  auto first_of = [](int32_t c, int32_t width) { return c < width - 4 ? c : width > 4 ? width - 4 : 0; };
+  const T* dy = static_cast<const T*>(a.dy) + (r0 + kg * 8) * a.lddy + first_of(o0 + cg * 4, a.o);
+  const int32_t ic = first_of(i0 + cg * 4, ldq);
+  const int8_t* qp = a.q + (r0 + kg * 8) * ldq + ic;
+  const uint8_t* ep = a.e + (r0 + kg * 8) * a.nb + ic / kBlock;
+
+  floatx16 acc[FM][FN];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const bool in = k0 + k < r1;
-      y[k] = load_quad(static_cast<const T*>(a.dy) + (in ? k0 + k : 0) * a.lddy + oc, in ? a.o - oc : 0);
-      x[k] = in && in_i ? *reinterpret_cast<const uint32_t*>(a.q + (k0 + k) * ldq + ic) : 0u;
-      code[k] = in && in_i ? a.e[(k0 + k) * a.nb + ic / kBlock] : 1u;
+  for (int m = 0; m < FM; ++m)
+#pragma unroll
+    for (int n = 0; n < FN; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[m][n][i] = 0.f;
+  const int wm = (wave / kWavesN) * FM * 32, wn = (wave % kWavesN) * FN * 32;
+
+  Quad<T> y[8];
+  uint32_t x[8], code[8];
+  auto row_of = [&](const T* p) {
+    if constexpr (NARROW) {
+      Quad<T> v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v.e[j] = p[j < a.o ? j : a.o - 1];
+      return v;
+    } else {
+      return load_quad(p);
     }
-    __syncthreads();  // the last step's operands are read
+  };
+  // The next kDepth rows' operands, `left` of them in the share: behind the last one x repeats it and dy is 0.
+  auto fetch = [&](int64_t left) {
+    if (left >= kDepth) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      char* at = lds + (32 * j + cg) * kLdsPitch + kg * 16;
-      if constexpr (P == 1) {
-        u32x4 w;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t lo = reinterpret_cast<const uint32_t*>(y[2 * k].e)[j >> 1];
-          const uint32_t hi = reinterpret_cast<const uint32_t*>(y[2 * k + 1].e)[j >> 1];
-          w[k] = __builtin_amdgcn_perm(hi, lo, (j & 1) != 0 ? 0x07060302 : 0x05040100);
-        }
-        *reinterpret_cast<u32x4*>(at) = w;
-      } else {
-        float f[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) f[k] = static_cast<float>(y[k].e[j]);
-#pragma unroll
-        for (int p = 0; p < P; ++p) {
-          u32x4 w;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t lo = take_term(f[2 * k]), hi = take_term(f[2 * k + 1]);
-            w[k] = high_halves(lo, hi);
-          }
-          *reinterpret_cast<u32x4*>(at + p * kPlane) = w;
-        }
+      for (int k = 0; k < 8; ++k) {
+        y[k] = row_of(dy + k * a.lddy);
+        x[k] = *reinterpret_cast<const uint32_t*>(qp + k * static_cast<int64_t>(ldq));
+        code[k] = ep[k * static_cast<int64_t>(a.nb)];
       }
+    } else {
+      const int32_t last = static_cast<int32_t>(left) - 1 - kg * 8;  // from this thread's first row
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int64_t at = k < last ? k : last;
+        y[k] = row_of(dy + at * a.lddy);
+        x[k] = *reinterpret_cast<const uint32_t*>(qp + at * ldq);
+        code[k] = ep[at * a.nb];
+        if (k > last)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y[k].e[j] = static_cast<T>(0.f);
+      }
+    }
+    dy += kDepth * a.lddy;
+    qp += kDepth * static_cast<int64_t>(ldq);
+    ep += kDepth * static_cast<int64_t>(a.nb);
+  };
+  // Column j of the thread's quads into a buffer.
+  auto store = [&](char* buffer, int j) {
+    char* at = buffer + ((B / 4) * j + cg) * kLdsPitch + kg * 16;
+    if constexpr (P == 1) {
       u32x4 w;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float lo = static_cast<float>(static_cast<int8_t>(x[2 * k] >> (8 * j))) * scale_of(code[2 * k]);
-        const float hi = static_cast<float>(static_cast<int8_t>(x[2 * k + 1] >> (8 * j))) * scale_of(code[2 * k + 1]);
-        w[k] = high_halves(__float_as_uint(lo), __float_as_uint(hi));
+        const uint32_t lo = reinterpret_cast<const uint32_t*>(y[2 * k].e)[j >> 1];
+        const uint32_t hi = reinterpret_cast<const uint32_t*>(y[2 * k + 1].e)[j >> 1];
+        w[k] = __builtin_amdgcn_perm(hi, lo, (j & 1) != 0 ? 0x07060302 : 0x05040100);
       }
-      *reinterpret_cast<u32x4*>(at + P * kPlane) = w;
-    }
-    __syncthreads();
+      *reinterpret_cast<u32x4*>(at) = w;
+    } else {
+      float f[8];
 #pragma unroll
-    for (int s = 0; s < kDepth / 32; ++s) {
-      const int off = (lane & 15) * kLdsPitch + s * 64 + (lane >> 4) * 16;
-      bf16x8 b[4];
+      for (int k = 0; k < 8; ++k) f[k] = static_cast<float>(y[k].e[j]);
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
-        b[n] = *reinterpret_cast<const bf16x8*>(lds + P * kPlane + (wn + n * 16) * kLdsPitch + off);
+      for (int p = 0; p < P; ++p) {
+        u32x4 w;
 #pragma unroll
-      for (int p = 0; p < P; ++p)
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          const bf16x8 v = *reinterpret_cast<const bf16x8*>(lds + p * kPlane + (wm + m * 16) * kLdsPitch + off);
-#pragma unroll
-          for (int n = 0; n < 4; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, b[n], acc[m][n], 0, 0, 0);
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t lo = take_term(f[2 * k]), hi = take_term(f[2 * k + 1]);
+          w[k] = high_halves(lo, hi);
         }
+        *reinterpret_cast<u32x4*>(at + p * kPlane) = w;
+      }
     }
-  }
-  float* out = a.out + static_cast<int64_t>(blockIdx.z) * a.o * a.d;
+    u32x4 w;
 #pragma unroll
-  for (int n = 0; n < 4; ++n) {
-    const int ln = wn + n * 16 + (lane & 15);
-    const int32_t col = i0 + (ln & 31) * 4 + (ln >> 5);
+    for (int k = 0; k < 4; ++k) {
+      float f[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float s = scale_of(code[2 * k + h]);
+        const uint32_t u = ((x[2 * k + h] ^ 0x80808080u) >> (8 * j)) & 255u;  // q + 128
+        f[h] = __builtin_fmaf(static_cast<float>(u), s, -128.f * s);          // exact; NaN where s is inf
+      }
+      w[k] = high_halves(__float_as_uint(f[0]), __float_as_uint(f[1]));
+    }
+    *reinterpret_cast<u32x4*>(at + P * kPlane) = w;
+  };
+  auto multiply = [&](const char* buffer, int s) {
+    const int off = (lane & 31) * kLdsPitch + s * 32 + (lane >> 5) * 16;
+    bf16x8 b[FN];
+#pragma unroll
+    for (int n = 0; n < FN; ++n)
+      b[n] = *reinterpret_cast<const bf16x8*>(buffer + P * kPlane + (wn + n * 32) * kLdsPitch + off);
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int m = 0; m < FM; ++m) {
+        const bf16x8 v = *reinterpret_cast<const bf16x8*>(buffer + p * kPlane + (wm + m * 32) * kLdsPitch + off);
+#pragma unroll
+        for (int n = 0; n < FN; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, b[n], acc[m][n], 0, 0, 0);
+      }
+  };
+
+  fetch(r1 - r0);
+  if constexpr (kStages<T> == 2) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) store(lds, j);
+    if (r0 + kDepth < r1) fetch(r1 - r0 - kDepth);
+    __syncthreads();
+    int turn = 0;
+    int64_t r = r0;
+    do {
+      const char* now = lds + turn * kBuffer;
+      turn ^= 1;
+      multiply(now, 0);
+      multiply(now, 1);
+      if (r + kDepth < r1) {
+        store(lds + turn * kBuffer, 0);
+        store(lds + turn * kBuffer, 1);
+      }
+      multiply(now, 2);
+      if (r + kDepth < r1) {
+        store(lds + turn * kBuffer, 2);
+        store(lds + turn * kBuffer, 3);
+        if (r + 2 * kDepth < r1) fetch(r1 - r - 2 * kDepth);
+      }
+      multiply(now, 3);
+      __syncthreads();
+      r += kDepth;
+    } while (r < r1);
+  } else {
+    int64_t r = r0;
+    do {
+      __syncthreads();  // the last step's operands are read
+#pragma unroll
+      for (int j = 0; j < 4; ++j) store(lds, j);
+      if (r + kDepth < r1) fetch(r1 - r - kDepth);
+      __syncthreads();
+#pragma unroll
+      for (int s = 0; s < kDepth / 16; ++s) multiply(lds, s);
+      r += kDepth;
+    } while (r < r1);
+  }
+  float* out = a.out + static_cast<int64_t>(split) * a.o * a.d;
+#pragma unroll
+  for (int n = 0; n < FN; ++n) {
+    const int ln = wn + n * 32 + (lane & 31);
+    const int32_t col = first_of(i0 + ln % (B / 4) * 4, ldq) + ln / (B / 4);
     if (col >= a.d) continue;
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
+    for (int m = 0; m < FM; ++m)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int lm = wm + m * 16 + (lane >> 4) * 4 + i;
-        const int32_t row = o0 + (lm & 31) * 4 + (lm >> 5);
-        if (row < a.o) out[static_cast<int64_t>(row) * a.d + col] = acc[m][n][i];
+      for (int i = 0; i < 16; ++i) {
+        const int lm = wm + m * 32 + (i >> 2) * 8 + (lane >> 5) * 4 + (i & 3);
+        const int32_t row = first_of(o0 + lm % (B / 4) * 4, a.o) + lm / (B / 4);
+        if (!NARROW || row < a.o) out[static_cast<int64_t>(row) * a.d + col] = acc[m][n][i];
       }
   }
 }
@@ -289,18 +379,26 @@ __global__ __launch_bounds__(256) void act8_join_kernel(const float* part, int32
 }
 
 struct Splits {
+  int32_t tile;  // B
   int32_t w, b;  // row shares of dW and of db
+  int64_t per;   // rows of a share of dW
 };
 
+template <typename T>
 Splits wgrad_splits(int64_t n, int32_t o, int32_t d) {
-  const int64_t tiles = static_cast<int64_t>((o + kTile - 1) / kTile) * ((d + kTile - 1) / kTile);
-  int64_t w = (2 * kCUs + tiles - 1) / tiles, most = (n + 511) / 512;
+  const int64_t least = o < d ? o : d;
+  const int32_t tile = kPlanes<T> == 1 && least > 128 ? 256 : least > 64 ? 128 : 64;
+  const int64_t tiles = static_cast<int64_t>((o + tile - 1) / tile) * ((d + tile - 1) / tile);
+  const int64_t fill = tile == 256 ? kCUs : tile == 128 ? 2 * kCUs : 4 * kCUs;  // blocks the chip holds
+  int64_t w = fill / tiles, most = (n + 511) / 512;
   if (w > most) w = most;
+  if (w < 1) w = 1;
+  const int64_t per = n < 1 ? kDepth : ((n + w - 1) / w + kDepth - 1) / kDepth * kDepth;
   const int64_t strips = (o + 63) / 64;
   int64_t b = (4 * kCUs + strips - 1) / strips;
   most = (n + 63) / 64;
   if (b > most) b = most;
-  return {static_cast<int32_t>(w < 1 ? 1 : w), static_cast<int32_t>(b < 1 ? 1 : b)};
+  return {tile, static_cast<int32_t>(n < 1 ? 1 : (n + per - 1) / per), static_cast<int32_t>(b < 1 ? 1 : b), per};
 }
 
 bool act8_shape_ok(int64_t n, int32_t d) { return n >= 0 && d >= 1 && d <= KGAT_ACT8_MAX_D; }
@@ -352,9 +450,10 @@ extern "C" int kgat_act8_unpack(int32_t dtype, const int8_t* q, const uint8_t* e
   });
 }
 
-extern "C" int64_t kgat_act8_wgrad_workspace(int64_t n, int32_t o, int32_t d) {
-  if (!kgat::act8_shape_ok(n, d) || o < 1 || o > KGAT_ACT8_MAX_D) return -1;
-  const kgat::Splits s = kgat::wgrad_splits(n, o, d);
+extern "C" int64_t kgat_act8_wgrad_workspace(int32_t dtype, int64_t n, int32_t o, int32_t d) {
+  using namespace kgat;
+  if (!act8_shape_ok(n, d) || o < 1 || o > KGAT_ACT8_MAX_D || dtype < KGAT_F32 || dtype > KGAT_F16) return -1;
+  const Splits s = dtype == KGAT_BF16 ? wgrad_splits<__bf16>(n, o, d) : wgrad_splits<float>(n, o, d);
   return static_cast<int64_t>(s.w) * o * d + static_cast<int64_t>(s.b) * o;
 }
 
@@ -363,21 +462,35 @@ extern "C" int kgat_act8_wgrad(int32_t dtype, const void* dy, int64_t lddy, cons
                                int64_t workspace_floats, void* stream) {
   using namespace kgat;
   if (!dy || !q || !e || !dW || !act8_shape_ok(n, d) || o < 1 || o > KGAT_ACT8_MAX_D || lddy < 0 ||
-      (reinterpret_cast<uintptr_t>(q) & 15))
+      (reinterpret_cast<uintptr_t>(q) & 15) || dtype < KGAT_F32 || dtype > KGAT_F16)
     return KGAT_ERR_INVALID;
-  if (!workspace || workspace_floats < kgat_act8_wgrad_workspace(n, o, d)) return KGAT_ERR_WORKSPACE;
-  const Splits s = wgrad_splits(n, o, d);
+  if (!workspace || workspace_floats < kgat_act8_wgrad_workspace(dtype, n, o, d)) return KGAT_ERR_WORKSPACE;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  float* part_b = workspace + static_cast<int64_t>(s.w) * o * d;
   return with_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    Wgrad a{dy, lddy, q, e, s.w == 1 ? dW : workspace, n, (n + s.w - 1) / s.w, o, d, (d + kBlock - 1) / kBlock};
-    a.per = (a.per + kDepth - 1) / kDepth * kDepth;
-    hipLaunchKernelGGL(act8_wgrad_kernel<T>, dim3((d + kTile - 1) / kTile, (o + kTile - 1) / kTile, s.w), dim3(256), 0,
-                       st, a);
+    const Splits s = wgrad_splits<T>(n, o, d);
+    float* part_b = workspace + static_cast<int64_t>(s.w) * o * d;
+    const int64_t size = static_cast<int64_t>(o) * d;
+    if (n == 0) {  // sums of nothing
+      hipLaunchKernelGGL(act8_join_kernel, dim3(static_cast<uint32_t>((size + 255) / 256)), dim3(256), 0, st, workspace,
+                         0, size, dW);
+      KGAT_LAUNCH_CHECK();
+      if (db != nullptr)
+        hipLaunchKernelGGL(act8_join_kernel, dim3((o + 255) / 256), dim3(256), 0, st, part_b, 0, static_cast<int64_t>(o), db);
+      KGAT_LAUNCH_CHECK();
+      return KGAT_OK;
+    }
+    const Wgrad a{dy, lddy, q, e, s.w == 1 ? dW : workspace, n, s.per, o, d, (d + kBlock - 1) / kBlock,
+                  (o + s.tile - 1) / s.tile, (d + s.tile - 1) / s.tile, s.w};
+    const int64_t blocks = static_cast<int64_t>(a.tiles_o) * a.tiles_d * s.w;
+    if (blocks > 0x7FFFFFFF) return KGAT_ERR_INVALID;
+    const dim3 grid(static_cast<uint32_t>(blocks));
+    if (o < 4) hipLaunchKernelGGL((act8_wgrad_kernel<T, 64, true>), grid, dim3(128), 0, st, a);
+    else if (s.tile == 64) hipLaunchKernelGGL((act8_wgrad_kernel<T, 64, false>), grid, dim3(128), 0, st, a);
+    else if (s.tile == 128) hipLaunchKernelGGL((act8_wgrad_kernel<T, 128, false>), grid, dim3(256), 0, st, a);
+    else if constexpr (kPlanes<T> == 1) hipLaunchKernelGGL((act8_wgrad_kernel<T, 256, false>), grid, dim3(512), 0, st, a);
     KGAT_LAUNCH_CHECK();
     if (s.w > 1) {
-      const int64_t size = static_cast<int64_t>(o) * d;
       hipLaunchKernelGGL(act8_join_kernel, dim3(static_cast<uint32_t>((size + 255) / 256)), dim3(256), 0, st, workspace,
                          s.w, size, dW);
       KGAT_LAUNCH_CHECK();

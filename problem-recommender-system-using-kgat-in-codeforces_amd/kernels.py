@@ -1587,7 +1587,7 @@ def act8_wgrad(dy: torch.Tensor, a: Act8, bias: bool = True):
     db = torch.empty(o, dtype=torch.float32, device=dy.device) if bias else None
     if n == 0:
         return dW.zero_(), None if db is None else db.zero_()
-    ws = torch.empty(max(1, int(_lib.lib().kgat_act8_wgrad_workspace(n, o, d))), dtype=torch.float32, device=dy.device)
+    ws = torch.empty(max(1, int(_lib.lib().kgat_act8_wgrad_workspace(code, n, o, d))), dtype=torch.float32, device=dy.device)
     _row_call(dy, "kgat_act8_wgrad", code, dy.data_ptr(), dy.stride(0), a.q.data_ptr(), a.e.data_ptr(), n, o, d,
               dW.data_ptr(), _ptr(db), ws.data_ptr(), ws.numel())
     return dW, db
