@@ -40,7 +40,7 @@ __global__ __launch_bounds__(256) void act8_pack_kernel(Pack a) {
   const int64_t row = row0 + at / per_row;
   const int32_t vec = static_cast<int32_t>(at % per_row), c = vec * V;
   const bool live = row < a.n;
-  const Vec<T> t = load_vec(static_cast<const T*>(a.x) + (live ? row : 0) * a.ldx + c, live ? a.d - c : 0);
+  const Vec<T> t = load_row(static_cast<const T*>(a.x) + (live ? row : a.n - 1) * a.ldx, c, a.d);
   uint32_t top = 0;
   float f[V];
 #pragma unroll
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256) void act8_unpack_kernel(Unpack a) {
 #pragma unroll
   for (int j = 0; j < V; ++j)
     t.e[j] = static_cast<T>(static_cast<float>(static_cast<int8_t>(q[j / 4] >> (8 * (j % 4)))) * s);
-  store_vec(static_cast<T*>(a.x) + row * a.ldx + c, t, a.d - c);
+  store_row(static_cast<T*>(a.x) + row * a.ldx, c, a.d, t);
 }
 
 // ---------------------------------------------------------------------------------------------- weight gradient

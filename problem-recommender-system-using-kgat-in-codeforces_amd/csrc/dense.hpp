@@ -22,27 +22,54 @@ struct Vec {
   };
 };
 
-// The first `count` elements of a vector at p (count >= N: all of them); the others are `fill`.
+// Elements [c, c + N) of a row of d; those behind its end are 0.  The row's last vector, where it is cut, is read as the
+// row's last N elements and moved down: two shifts in one lane instead of N - 1 loads by all.
 template <typename T>
-__device__ __forceinline__ Vec<T> load_vec(const T* p, int64_t count, float fill = 0.f) {
+__device__ __forceinline__ Vec<T> load_row(const T* row, int64_t c, int64_t d) {
+  constexpr int N = Vec<T>::N;
   Vec<T> v;
-  if (count >= Vec<T>::N) {
-    v.raw = *reinterpret_cast<const u32x4_any*>(p);
+  if (c + N <= d) {
+    v.raw = *reinterpret_cast<const u32x4_any*>(row + c);
+  } else if (c >= d) {
+    v.raw = u32x4{0, 0, 0, 0};
+  } else if (d >= N) {
+    v.raw = *reinterpret_cast<const u32x4_any*>(row + d - N);
+    uint64_t lo = static_cast<uint64_t>(v.raw[1]) << 32 | v.raw[0], hi = static_cast<uint64_t>(v.raw[3]) << 32 | v.raw[2];
+    const int bits = static_cast<int>(c + N - d) * 8 * static_cast<int>(sizeof(T));  // 16 to 112
+    lo = bits >= 64 ? hi >> (bits - 64) : lo >> bits | hi << (64 - bits);
+    hi = bits >= 64 ? 0 : hi >> bits;
+    v.raw = u32x4{static_cast<uint32_t>(lo), static_cast<uint32_t>(lo >> 32), static_cast<uint32_t>(hi),
+                  static_cast<uint32_t>(hi >> 32)};
   } else {
 #pragma unroll
-    for (int j = 0; j < Vec<T>::N; ++j) v.e[j] = j < count ? p[j] : static_cast<T>(fill);
+    for (int j = 0; j < N; ++j) v.e[j] = c + j < d ? row[c + j] : static_cast<T>(0.f);
   }
   return v;
 }
 
+// The other way: elements behind the row's end are left alone.
 template <typename T>
-__device__ __forceinline__ void store_vec(T* p, const Vec<T>& v, int64_t count) {
-  if (count >= Vec<T>::N) {
+__device__ __forceinline__ void store_row(T* row, int64_t c, int64_t d, Vec<T> v) {
+  T* p = row + c;
+  if (c + Vec<T>::N <= d) {
     *reinterpret_cast<u32x4_any*>(p) = v.raw;
-  } else {
-#pragma unroll
-    for (int j = 0; j < Vec<T>::N; ++j)
-      if (j < count) p[j] = v.e[j];
+  } else if (c < d) {
+    const int count = static_cast<int>(d - c) * static_cast<int>(sizeof(T)) / 2;  // 2-byte units: 1 to 7
+    typedef u32x2 u32x2_any __attribute__((aligned(2)));
+    typedef uint32_t u32_any __attribute__((aligned(2)));
+    char* at = reinterpret_cast<char*>(p);
+    if ((count & 4) != 0) {
+      *reinterpret_cast<u32x2_any*>(at) = u32x2{v.raw[0], v.raw[1]};
+      v.raw[0] = v.raw[2];
+      v.raw[1] = v.raw[3];
+      at += 8;
+    }
+    if ((count & 2) != 0) {
+      *reinterpret_cast<u32_any*>(at) = v.raw[0];
+      v.raw[0] = v.raw[1];
+      at += 4;
+    }
+    if (sizeof(T) == 2 && (count & 1) != 0) *reinterpret_cast<uint16_t*>(at) = static_cast<uint16_t>(v.raw[0]);
   }
 }
 

@@ -27,18 +27,18 @@ struct NormVec {
   }
 };
 
-// A thread's columns of a weight vector; `none` behind the last one and where there is no vector.  The branches are
-// uniform and the index is clamped, so no lane takes a path of its own: with a per-element choice of type under the
-// lane's own bound, hipcc 7.2 lost a live address register on the fp16 path.
+// A thread's columns of a weight vector; `none` where there is no vector.  The choices are uniform: with a choice of
+// type for every element under the lane's own bound, hipcc 7.2 lost a live address register on the fp16 path.
 template <typename W, int V, int NV>
-__device__ __forceinline__ void load_columns_of(const W* p, int lane, int G, int32_t d, float none, float (&out)[NV][V]) {
+__device__ __forceinline__ void load_columns_of(const W* p, int lane, int G, int32_t d, float (&out)[NV][V]) {
+  constexpr int N = Vec<W>::N < V ? Vec<W>::N : V;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = (i * G + lane) * V + j;
-      const float v = static_cast<float>(p[c < d ? c : d - 1]);
-      out[i][j] = c < d ? v : none;
+    for (int j = 0; j < V; j += N) {
+      const Vec<W> v = load_row(p, (i * G + lane) * V + j, d);
+#pragma unroll
+      for (int k = 0; k < N; ++k) out[i][j + k] = static_cast<float>(v.e[k]);
     }
 }
 
@@ -51,9 +51,9 @@ __device__ __forceinline__ void load_columns(const NormVec& w, int lane, int G, 
 #pragma unroll
       for (int j = 0; j < V; ++j) out[i][j] = none;
   } else if (sizeof(T) == 4 || w.dtype == KGAT_F32) {
-    load_columns_of(static_cast<const float*>(w.p), lane, G, d, none, out);
+    load_columns_of(static_cast<const float*>(w.p), lane, G, d, out);
   } else {
-    load_columns_of(static_cast<const T*>(w.p), lane, G, d, none, out);
+    load_columns_of(static_cast<const T*>(w.p), lane, G, d, out);
   }
 }
 
@@ -115,12 +115,9 @@ __global__ __launch_bounds__(THREADS) void norm_fwd_kernel(NormFwd a) {
   load_columns<T>(a.b, lane, G, a.d, 0.f, b);
   Vec<T> next[NV];
   auto fetch = [&](int64_t row) {
-    const T* x = static_cast<const T*>(a.x) + (row < a.n ? row : 0) * a.ldx;
+    const T* x = static_cast<const T*>(a.x) + (row < a.n ? row : a.n - 1) * a.ldx;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * G + lane) * V;
-      next[i] = load_vec(x + c, row < a.n ? a.d - c : 0);
-    }
+    for (int i = 0; i < NV; ++i) next[i] = load_row(x, (i * G + lane) * V, a.d);
   };
   fetch(first + threadIdx.x / G);
   for (int64_t base = first; base < a.n; base += step) {
@@ -154,7 +151,7 @@ __global__ __launch_bounds__(THREADS) void norm_fwd_kernel(NormFwd a) {
         Vec<T> t;
 #pragma unroll
         for (int j = 0; j < V; ++j) t.e[j] = static_cast<T>(v[i][j] * rstd * w[i][j] + b[i][j]);
-        store_vec(y + c, t, a.d - c);
+        store_row(y, c, a.d, t);
       }
       if (lane == 0 && a.mean != nullptr) {
         a.mean[row] = mean;
@@ -176,14 +173,14 @@ __global__ __launch_bounds__(THREADS) void norm_fwd_wide_kernel(NormFwd a) {
     T* y = static_cast<T*>(a.y) + row * a.ldy;
     float s[1] = {0.f}, q[1] = {0.f};
     for (int64_t c = threadIdx.x * V; c < a.d; c += THREADS * V) {
-      const Vec<T> t = load_vec(x + c, a.d - c);
+      const Vec<T> t = load_row(x, c, a.d);
 #pragma unroll
       for (int j = 0; j < V; ++j) s[0] += static_cast<float>(t.e[j]);
     }
     group_sum<THREADS, THREADS>(s, lds, turn);
     const float mean = s[0] / d;
     for (int64_t c = threadIdx.x * V; c < a.d; c += THREADS * V) {
-      const Vec<T> t = load_vec(x + c, a.d - c);
+      const Vec<T> t = load_row(x, c, a.d);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float e = static_cast<float>(t.e[j]) - mean;
@@ -193,7 +190,7 @@ __global__ __launch_bounds__(THREADS) void norm_fwd_wide_kernel(NormFwd a) {
     group_sum<THREADS, THREADS>(q, lds, turn);
     const float rstd = 1.f / sqrtf(q[0] / d + a.eps);
     for (int64_t c = threadIdx.x * V; c < a.d; c += THREADS * V) {
-      Vec<T> t = load_vec(x + c, a.d - c);
+      Vec<T> t = load_row(x, c, a.d);
 #pragma unroll
       for (int j = 0; j < V; ++j)
         if (c + j < a.d) {
@@ -202,7 +199,7 @@ __global__ __launch_bounds__(THREADS) void norm_fwd_wide_kernel(NormFwd a) {
           if (a.b.p != nullptr) r += a.b.template at<T>(c + j);
           t.e[j] = static_cast<T>(r);
         }
-      store_vec(y + c, t, a.d - c);
+      store_row(y, c, a.d, t);
     }
     if (threadIdx.x == 0 && a.mean != nullptr) {
       a.mean[row] = mean;
@@ -249,16 +246,17 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(NormBwd a) {
   Vec<T> nx[NV], ng[NV];
   float nmean = 0.f, nrstd = 0.f;
   auto fetch = [&](int64_t row) {
-    const bool live = row < a.n;
-    const T* x = static_cast<const T*>(a.x) + (live ? row : 0) * a.ldx;
-    const T* dy = static_cast<const T*>(a.dy) + (live ? row : 0) * a.lddy;
-    nmean = live ? a.mean[row] : 0.f;
-    nrstd = live ? a.rstd[row] : 0.f;
+    const bool live = row < a.n;  // behind the last row: no column is read, dy is 0
+    const int64_t at = live ? row : a.n - 1;
+    const T* x = static_cast<const T*>(a.x) + at * a.ldx;
+    const T* dy = static_cast<const T*>(a.dy) + at * a.lddy;
+    nmean = live ? a.mean[at] : 0.f;
+    nrstd = live ? a.rstd[at] : 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * G + lane) * V;
-      nx[i] = load_vec(x + c, live ? a.d - c : 0);
-      ng[i] = load_vec(dy + c, live ? a.d - c : 0);
+      const int c = live ? (i * G + lane) * V : a.d;
+      nx[i] = load_row(x, c, a.d);
+      ng[i] = load_row(dy, c, a.d);
     }
   };
   fetch(first + threadIdx.x / G);
@@ -291,7 +289,7 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(NormBwd a) {
         Vec<T> t;
 #pragma unroll
         for (int j = 0; j < V; ++j) t.e[j] = static_cast<T>(rstd * (g[i][j] - mg - xh[i][j] * mgx));
-        store_vec(dx + c, t, a.d - c);
+        store_row(dx, c, a.d, t);
       }
     }
   }
@@ -348,7 +346,7 @@ __global__ __launch_bounds__(THREADS) void norm_dx_kernel(NormBwd a) {
     const float mean = a.mean[row], rstd = a.rstd[row];
     float s[2] = {0.f, 0.f};
     for (int64_t c = threadIdx.x * V; c < a.d; c += THREADS * V) {
-      const Vec<T> tx = load_vec(x + c, a.d - c), tg = load_vec(dy + c, a.d - c);
+      const Vec<T> tx = load_row(x, c, a.d), tg = load_row(dy, c, a.d);
 #pragma unroll
       for (int j = 0; j < V; ++j)
         if (c + j < a.d) {
@@ -361,7 +359,7 @@ __global__ __launch_bounds__(THREADS) void norm_dx_kernel(NormBwd a) {
     group_sum<THREADS, THREADS>(s, lds, turn);
     const float mg = s[0] / d, mgx = s[1] / d;
     for (int64_t c = threadIdx.x * V; c < a.d; c += THREADS * V) {
-      const Vec<T> tx = load_vec(x + c, a.d - c), tg = load_vec(dy + c, a.d - c);
+      const Vec<T> tx = load_row(x, c, a.d), tg = load_row(dy, c, a.d);
       Vec<T> t;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
@@ -369,7 +367,7 @@ __global__ __launch_bounds__(THREADS) void norm_dx_kernel(NormBwd a) {
         if (a.w.p != nullptr && c + j < a.d) g *= a.w.template at<T>(c + j);
         t.e[j] = static_cast<T>(rstd * (g - mg - (static_cast<float>(tx.e[j]) - mean) * rstd * mgx));
       }
-      store_vec(dx + c, t, a.d - c);
+      store_row(dx, c, a.d, t);
     }
   }
 }
@@ -449,7 +447,7 @@ template <typename T>
 int norm_fwd(const NormFwd& a, hipStream_t st) {
   const bool done = with_shape<T, kFwdElems>(a.d, [&](auto g, auto nv) {
     constexpr int G = decltype(g)::value, NV = decltype(nv)::value, kThreads = G > 256 ? G : 256;
-    const int grid = blocks_for(a.n, kThreads / G, kCUs * (2048 / kThreads));  // every thread the chip holds, at most
+    const int grid = blocks_for(a.n, kThreads / G, kCUs * (kThreads > 512 ? 1 : 1024 / kThreads));  // 16 waves a CU
     hipLaunchKernelGGL((norm_fwd_kernel<T, G, NV, kThreads>), dim3(grid), dim3(kThreads), 0, st, a);
   });
   if (!done)

@@ -4,10 +4,11 @@
 //   S = sum e^(z - scale m),  W = sum (z - scale m) e^(z - scale m)
 //   lse = scale m + log S,  logp_j = z_j - lse,  H = -sum p log p = log S - W / S   (both terms >= 0: no cancellation)
 //   ds_j = scale (sum_t g_t [item_t = j] - p_j (sum_t g_t + g_H (logp_j + H)))
-// m, S and W come from one pass: a thread that meets a larger score rescales what it has,
+// m, S and W come from one pass: who meets a larger score rescales what it has,
 //   S <- S f,  W <- f (W + delta S),  delta = (old m - new m) scale,  f = e^delta.
-// Everything is kept in base 2 (t = (s - m) scale log2 e, one v_exp_f32 an element).  The difference is taken before
-// the product, so that rows of one single value, were it the type's lowest, come out uniform.
+// Exponents are kept in base 2, x = s c - rho with c = scale log2 e and rho = m c rounded: one fma and one v_exp_f32 an
+// element, and rho's rounding is the same in every x and in lse.  Where m c leaves the floats' middle range (rows of
+// the type's lowest or largest value) x = (s - m) c instead, so that equal scores stay equal.
 //
 // Masked scores (-inf) have p = 0 and count nowhere.  A row of nothing else has no distribution: logp and lse -inf,
 // H 0, gradient 0.  A row with a NaN or a +inf: everything NaN, best items -1, gradient NaN.
@@ -22,24 +23,93 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLow = -1e30f;  // a base-2 exponent whose power is 0, and whose products with 0 are 0
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }  // NaN wins
+
+// A maximum m and the reference rho that stands for it in base 2.
+struct Ref {
+  float m, rho;
+  bool far;  // m c is no ordinary float
+  __device__ __forceinline__ Ref(float m_, float c) : m(m_), rho(m_ * c), far(!(fabsf(m_ * c) < 1e37f)) {}
+  __device__ __forceinline__ float operator()(float s, float c) const {
+    return far ? (s - m) * c : __builtin_fmaf(s, c, -rho);
+  }
+};
 
 // A part of a row: its maximum, and S and W relative to it.
 struct Stat {
   float m, s, w;
 };
 
-// The factor that brings sums relative to `from` to `to` >= from (-inf: nothing was summed).
+// Brings sums relative to a.m to `to` >= a.m (-inf: nothing was summed).
 __device__ __forceinline__ Stat rebase(Stat a, float to, float c) {
-  const float delta = fmaxf((a.m - to) * c, kLow);  // from -inf (or NaN from two of them): kLow
+#pragma clang fp contract(off)
+  const Ref from(a.m, c), ref(to, c);
+  float delta = from.far || ref.far ? (a.m - to) * c : from.rho - ref.rho;
+  delta = fmaxf(delta, kLow);  // from -inf, or NaN from two of them
   const float f = exp2_fast(delta);
   return {to, a.s * f, f * (a.w + delta * a.s)};
 }
 
-__device__ __forceinline__ Stat combine(Stat a, Stat b, float c) {
-  const float m = fmaxf(a.m, b.m);
+// Joins the parts of N lanes (a power of two): the largest maximum first, one rescaling each, then plain sums.
+template <int N>
+__device__ __forceinline__ Stat join_lanes(Stat a, float c) {
+  float m = a.m;
+#pragma unroll
+  for (int o = 1; o < N; o <<= 1) m = max_nan(m, __shfl_xor(m, o));
   a = rebase(a, m, c);
-  b = rebase(b, m, c);
-  return {m, a.s + b.s, a.w + b.w};
+#pragma unroll
+  for (int o = 1; o < N; o <<= 1) {
+    a.s += __shfl_xor(a.s, o);
+    a.w += __shfl_xor(a.w, o);
+  }
+  return a;
+}
+
+struct LogProb {
+  const void* s;
+  int64_t ld;
+  int32_t rows, cols;
+  float scale;
+  const int64_t* items;  // [rows][t]
+  int32_t t, k;
+  float* logp;           // [rows][t]
+  float* stats;          // [4][rows]: m, log2 S, H, lse
+  int64_t* top_item;     // [rows][k]
+  float* top_logp;       // [rows][k]
+  int32_t splits;        // blocks of a row
+  int32_t per;           // columns of a split
+  float* part;           // [rows][splits][4]: m, S, W
+  uint64_t* lists;       // [rows][splits][k], best first, 0 behind the last
+};
+
+// What a whole row's sums say.
+struct Row {
+  bool none, bad;
+  Ref ref;
+  float l2;
+  __device__ __forceinline__ Row(Stat r, float c)
+      : none(r.m == -INFINITY), bad(!(r.m < INFINITY)), ref(r.m, c), l2(none ? 0.f : log2f(r.s)) {}
+  __device__ __forceinline__ float logp(float s, float c, float scale) const {
+    const float x = ref(s, c);
+    if (bad || none) return bad ? NAN : -INFINITY;
+    return x > -1e37f ? (x - l2) * kLn2 : (s - ref.m) * scale;  // a mask of the lowest value: s c may pass the floats' range
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void finish_row(const LogProb& a, int row, Stat r, const Row& w, float c) {
+  const T* s = static_cast<const T*>(a.s) + static_cast<int64_t>(row) * a.ld;
+  const int64_t rows = a.rows;
+  if (threadIdx.x == 0) {
+    a.stats[row] = w.bad ? NAN : r.m;
+    a.stats[rows + row] = w.l2;
+    a.stats[2 * rows + row] = w.bad ? NAN : w.none ? 0.f : (w.l2 - r.w / r.s) * kLn2;
+    a.stats[3 * rows + row] = w.bad ? NAN : w.none ? -INFINITY : w.ref.far ? r.m * a.scale + w.l2 * kLn2 : (w.ref.rho + w.l2) * kLn2;
+  }
+  for (int i = threadIdx.x; i < a.t; i += blockDim.x) {
+    const int64_t at = static_cast<int64_t>(row) * a.t + i, j = a.items[at];
+    a.logp[at] = j < 0 ? 0.f : j >= a.cols ? NAN : w.logp(static_cast<float>(s[j]), c, a.scale);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------- best items
@@ -58,300 +128,303 @@ __device__ __forceinline__ int32_t key_item(uint64_t k) {
   return static_cast<int32_t>(0xFFFFFFFFu - static_cast<uint32_t>(k));
 }
 
-// A wave's list of its 64 E largest keys, descending: element 64 i + lane in k[i].
-template <int E>
-struct Best {
-  uint64_t k[E];
+// A block's candidates.  Scores at or above a floor enter; when the pool fills up, the k best stay and the k-th
+// becomes the floor.  Every key is one of a kind, so an element's place is the number of larger keys: ranks are counted,
+// not sorted, and do not depend on the order in which the candidates came.
+template <int NT>
+struct Pool {
+  static constexpr int kSize = NT + 256;  // what is kept (at most 128) and one key of every thread always fit
+  uint64_t key[2][kSize];
+  float group[256];
+  float group_floor[4];
+  int count, first_lost, now;
+  uint64_t floor_key;  // the k-th key, once k were kept (0: none)
+  float floor;         // no smaller score enters
 };
 
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int o) {
-  const uint32_t lo = static_cast<uint32_t>(__shfl_xor(static_cast<int>(static_cast<uint32_t>(v)), o));
-  const uint32_t hi = static_cast<uint32_t>(__shfl_xor(static_cast<int>(static_cast<uint32_t>(v >> 32)), o));
-  return (static_cast<uint64_t>(hi) << 32) | lo;
-}
-
-// Orders a wave's LDS writes before its later LDS reads by other lanes (LDS works in order within a wave: this holds
-// the compiler, and costs no instruction).
-__device__ __forceinline__ void wave_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
-
-// Sorts a bitonic list of 64 E descending.
-template <int E>
-__device__ __forceinline__ void merge_down(Best<E>& b, int lane) {
-#pragma unroll
-  for (int i = E / 2; i > 0; i >>= 1)
-#pragma unroll
-    for (int j = 0; j < E; ++j)
-      if ((j & i) == 0) {
-        const uint64_t x = b.k[j], y = b.k[j + i];
-        b.k[j] = x > y ? x : y;
-        b.k[j + i] = x > y ? y : x;
-      }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1)
-#pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const uint64_t x = b.k[j], y = shfl_xor64(x, o);
-      b.k[j] = ((lane & o) == 0) == (x > y) ? x : y;
-    }
-}
-
-// 64 keys, one a lane, sorted descending.
-__device__ __forceinline__ uint64_t sort64(uint64_t v, int lane) {
-#pragma unroll
-  for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll
-    for (int o = size >> 1; o > 0; o >>= 1) {
-      const uint64_t y = shfl_xor64(v, o);
-      const bool down = (lane & size) == 0, low = (lane & o) == 0;
-      v = (down == low) == (v > y) ? v : y;
-    }
-  return v;
-}
-
-// The 64 E largest of the list and of another sorted one: the larger of element i of one and of the last but i of
-// the other are those, and bitonic.
-template <int E>
-__device__ __forceinline__ void merge(Best<E>& a, const Best<E>& b, int lane) {
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const uint64_t y = shfl_xor64(b.k[E - 1 - i], 63);
-    a.k[i] = a.k[i] > y ? a.k[i] : y;
-  }
-  merge_down(a, lane);
-}
-
-template <int E>
-__device__ __forceinline__ uint64_t key_at(const Best<E>& b, int i) {  // i uniform
-  uint64_t v = b.k[0];
-  if (E > 1 && i >= 64) v = b.k[E - 1];
-  const uint32_t lo = static_cast<uint32_t>(__shfl(static_cast<int>(static_cast<uint32_t>(v)), i & 63));
-  const uint32_t hi = static_cast<uint32_t>(__shfl(static_cast<int>(static_cast<uint32_t>(v >> 32)), i & 63));
-  return (static_cast<uint64_t>(hi) << 32) | lo;
-}
-
-struct LogProb {
-  const void* s;
-  int64_t ld;
-  int32_t rows, cols;
-  float scale;
-  const int64_t* items;  // [rows][t]
-  int32_t t, k;
-  float* logp;           // [rows][t]
-  float* stats;          // [4][rows]: m, log2 S, H, lse
-  int64_t* top_item;     // [rows][k]
-  float* top_logp;       // [rows][k]
-  int32_t splits;        // blocks of a row
-  int32_t per;           // columns of a split
-  float* part;           // [rows][splits][4]: m, S, W
-  uint64_t* lists;       // [rows][splits][k]
-};
-
-// What a whole row's sums say: written by one block.
-template <typename T>
-__device__ __forceinline__ void finish_row(const LogProb& a, int row, Stat r) {
-  const T* s = static_cast<const T*>(a.s) + static_cast<int64_t>(row) * a.ld;
-  const bool none = r.s == 0.f;  // nothing but -inf
-  const float l2 = none ? 0.f : log2f(r.s);
-  const float ls = l2 * kLn2;
+template <int NT>
+__device__ __forceinline__ void pool_start(Pool<NT>& p) {
   if (threadIdx.x == 0) {
-    a.stats[row] = none ? -INFINITY : r.s != r.s ? r.s : r.m;
-    a.stats[a.rows + row] = l2;
-    a.stats[2 * static_cast<int64_t>(a.rows) + row] = none ? 0.f : ls - r.w / r.s * kLn2;
-    a.stats[3 * static_cast<int64_t>(a.rows) + row] = none ? -INFINITY : r.m * a.scale + ls;
-  }
-  for (int i = threadIdx.x; i < a.t; i += blockDim.x) {
-    const int64_t at = static_cast<int64_t>(row) * a.t + i, j = a.items[at];
-    float v = 0.f;
-    if (j >= a.cols) v = NAN;
-    else if (j >= 0) v = none ? -INFINITY : (static_cast<float>(s[j]) - r.m) * a.scale - ls;
-    a.logp[at] = v;
+    p.count = p.now = 0;
+    p.first_lost = 0x7FFFFFFF;
+    p.floor_key = 0;
+    p.floor = -INFINITY;
   }
 }
 
-template <int E>
-__device__ __forceinline__ void write_best(const LogProb& a, int row, Stat r, const Best<E>& b, int lane) {
-  const bool none = r.s == 0.f, bad = r.s != r.s;
-  const float ls = none ? 0.f : log2f(r.s) * kLn2;
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const int at = i * 64 + lane;
-    if (at < a.k) {
-      const int64_t o = static_cast<int64_t>(row) * a.k + at;
-      a.top_item[o] = bad ? -1 : key_item(b.k[i]);
-      a.top_logp[o] = bad ? NAN : none ? -INFINITY : (key_score(b.k[i]) - r.m) * a.scale - ls;
+// Ranks the first n keys: f(rank, key) for those among the k best.
+template <int NT, typename F>
+__device__ __forceinline__ void pool_rank(const Pool<NT>& p, int n, int k, F&& f) {
+  const uint64_t* key = p.key[p.now];
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const uint64_t mine = key[i];
+    int rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) rank += key[j] > mine ? 1 : 0;
+    if (rank < k) f(rank, mine);
+  }
+}
+
+// Keeps the k best of the first n keys.  The whole block calls it, between barriers of its own.
+template <int NT>
+__device__ __forceinline__ void pool_keep(Pool<NT>& p, int n, int k) {
+  uint64_t* to = p.key[1 - p.now];
+  pool_rank(p, n, k, [&](int rank, uint64_t key) { to[rank] = key; });
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    p.now = 1 - p.now;
+    p.count = n < k ? n : k;
+    p.first_lost = 0x7FFFFFFF;
+    if (n >= k) {
+      p.floor_key = to[k - 1];
+      p.floor = key_score(to[k - 1]);
     }
   }
+  __syncthreads();
 }
 
-// One block per row (splits = 1) or per share of a row.  E: 64-key registers of the lists (0: no best items).
-template <typename T, int E, int THREADS>
-__global__ __launch_bounds__(THREADS) void log_prob_kernel(LogProb a) {
-  constexpr int V = Vec<T>::N, kWaves = THREADS / 64, kList = E > 0 ? 64 * E : 1;
+// One key of every thread that has one, with room for all made before.  The whole block calls it.
+template <int NT>
+__device__ __forceinline__ void pool_step(Pool<NT>& p, bool in, uint64_t key, int k) {
+  __syncthreads();
+  const int n = p.count;
+  __syncthreads();  // everyone has read the count
+  if (n > Pool<NT>::kSize - NT) pool_keep(p, n, k);
+  in = in && key > p.floor_key;
+  const uint64_t who = __ballot(in);
+  if (who != 0) {
+    int base = 0;
+    if ((threadIdx.x & 63) == 0) base = atomicAdd(&p.count, __popcll(who));
+    base = __shfl(base, 0);
+    if (in) p.key[p.now][base + __popcll(who & ((1ull << (threadIdx.x & 63)) - 1))] = key;
+  }
+}
+
+// The floor from the threads' own maxima: with the k-th largest of G (64 or 256 > k) groups' maxima as the floor, k
+// scores at least reach it, and of unordered scores hardly more: -G log(1 - k / G) on average.
+template <int NT>
+__device__ __forceinline__ void pool_floor(Pool<NT>& p, float top, int k) {
+  const int groups = k <= 48 ? 64 : 256, lanes = NT / groups;
+  for (int o = 1; o < lanes; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+  if (threadIdx.x % lanes == 0) p.group[threadIdx.x / lanes] = top;
+  if (threadIdx.x < 4) p.group_floor[threadIdx.x] = -INFINITY;
+  __syncthreads();
+  if (threadIdx.x < groups) {
+    const float mine = p.group[threadIdx.x];
+    int reach = 0;
+#pragma unroll 8
+    for (int j = 0; j < groups; ++j) reach += p.group[j] >= mine ? 1 : 0;
+    float v = reach >= k ? mine : -INFINITY;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) v = fmaxf(v, __shfl_xor(v, o));
+    if ((threadIdx.x & 63) == 0) p.group_floor[threadIdx.x >> 6] = v;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0)
+    p.floor = fmaxf(fmaxf(p.group_floor[0], p.group_floor[1]), fmaxf(p.group_floor[2], p.group_floor[3]));
+  __syncthreads();
+}
+
+// A block takes a row (splits = 1) or a share of one, NT M columns at a time, all in registers: maximum, sums, and with
+// TOP the scores that reach the pool's floor.
+template <typename T, bool TOP, int NT, int M>
+__global__ __launch_bounds__(NT, 4) void log_prob_kernel(LogProb a) {
+  constexpr int V = Vec<T>::N, U = M / V, kWaves = NT / 64;
   __shared__ Stat part[kWaves];
-  __shared__ uint64_t queue[E > 0 ? kWaves * 128 : 1];
-  __shared__ uint64_t lists[E > 0 ? kWaves * kList : 1];
+  __shared__ Pool<TOP ? NT : 0> pool;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int row = blockIdx.x, split = blockIdx.y;
   const T* s = static_cast<const T*>(a.s) + static_cast<int64_t>(row) * a.ld;
   const int64_t c0 = static_cast<int64_t>(split) * a.per;
   const int64_t c1 = c0 + a.per < a.cols ? c0 + a.per : a.cols;
   const float c = a.scale * kLog2e;
+  if constexpr (TOP) pool_start(pool);
 
   Stat r{-INFINITY, 0.f, 0.f};
-  Best<E < 1 ? 1 : E> best;
-  uint64_t* mine = queue + (E > 0 ? wave * 128 : 0);
-  int queued = 0, held = 0;    // keys in the queue; keys that reached the list
-  float floor = -INFINITY;     // the list's k-th score once it holds k,
-  uint64_t floor_key = 0;      // and its key
-  bool full = false;
-  if constexpr (E > 0) {
+  for (int64_t base = c0; base < c1; base += NT * M) {
+    float f[M];
+    Vec<T> t[U];
 #pragma unroll
-    for (int i = 0; i < E; ++i) best.k[i] = 0;
-  }
-  // Takes the queue's first 64 keys (fewer at the end) into the list.
-  auto drain = [&]() {
-    if constexpr (E > 0) {
-      const int take = queued < 64 ? queued : 64;
-      Best<E> b;
+    for (int u = 0; u < U; ++u) t[u] = load_row(s, base + (u * NT + threadIdx.x) * V, c1);
+    const bool whole = base + NT * M <= c1;  // uniform
+    float top = -INFINITY;
 #pragma unroll
-      for (int i = 1; i < E; ++i) b.k[i] = 0;
-      b.k[0] = sort64(lane < take ? mine[lane] : 0, lane);
-      const uint64_t rest = 64 + lane < queued ? mine[64 + lane] : 0;
-      wave_fence();
-      mine[lane] = rest;
-      wave_fence();
-      merge<E>(best, b, lane);
-      queued -= take;
-      held += take;
-      if (held >= a.k) {
-        full = true;
-        floor_key = key_at<E>(best, a.k - 1);
-        floor = key_score(floor_key);
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        float x = static_cast<float>(t[u].e[j]);
+        if (!whole && base + (u * NT + threadIdx.x) * V + j >= c1) x = -INFINITY;
+        f[u * V + j] = x;
+        top = max_nan(top, x);
+      }
+    r = rebase(r, max_nan(r.m, top), c);
+    const Ref ref(r.m, c);
+    if (!__any(ref.far && r.m != -INFINITY)) {
+#pragma unroll
+      for (int i = 0; i < M; ++i) {
+        const float x = fmaxf(__builtin_fmaf(f[i], c, -ref.rho), kLow);  // -inf (and NaN, which r.m holds): kLow
+        const float e = exp2_fast(x);
+        r.s += e;
+        r.w += e * x;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < M; ++i) {
+        const float x = fmaxf(ref(f[i], c), kLow);
+        const float e = exp2_fast(x);
+        r.s += e;
+        r.w += e * x;
       }
     }
-  };
-  for (int64_t base = c0 + static_cast<int64_t>(wave) * 64 * V; base < c1; base += static_cast<int64_t>(THREADS) * V) {
-    const int64_t col = base + lane * V;
-    const Vec<T> t = load_vec(s + col, c1 - col, -INFINITY);
-    float f[V], top = -INFINITY;
+    if constexpr (TOP) {
+      if (base == c0) pool_floor(pool, top, a.k);
+      // Candidates: a wave reserves room for all of its own at once.
+      const float floor = pool.floor;
+      const uint64_t floor_key = pool.floor_key;
+      auto item = [&](int i) { return static_cast<uint32_t>(base) + (i / V * NT + threadIdx.x) * V + i % V; };
+      bool lost = false;
+      if (__any(top >= floor)) {
+        uint32_t enters = 0;
+        int mine = 0;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      f[j] = static_cast<float>(t.e[j]);
-      top = fmaxf(top, f[j]);
-    }
-    const float m = fmaxf(r.m, top);
-    r = rebase(r, m, c);
-    const float ms = fmaxf(m, -3.402823466e38f);  // no score yet: -inf - ms stays -inf
+        for (int i = 0; i < M; ++i) {
+          bool in = f[i] >= floor;
+          if (!whole) in = in && item(i) < static_cast<uint32_t>(c1);
+          if (floor_key != 0) in = in && item_key(f[i], item(i)) > floor_key;
+          enters |= in ? 1u << i : 0u;
+          mine += __popcll(__ballot(in));
+        }
+        int at = 0;
+        if (lane == 0 && mine > 0) at = atomicAdd(&pool.count, mine);
+        at = __shfl(at, 0);
+        lost = mine > 0 && at + mine > Pool<NT>::kSize;
+        if (lost) {
+          if (lane == 0) atomicMin(&pool.first_lost, at);
+        } else if (mine > 0) {
+          uint64_t* key = pool.key[pool.now];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float x = (f[j] - ms) * c, e = exp2_fast(x);
-      r.s += e;
-      r.w += e * fmaxf(x, kLow);
-    }
-    if constexpr (E > 0) {
-      // Columns rise from vector to vector of a wave, so a score equal to the list's k-th ranks behind it: once the
-      // list holds k, only a larger one opens the vector (within it, the keys decide).
-      if (__any(top > floor || !full)) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const uint64_t key = item_key(f[j], static_cast<uint32_t>(col + j));
-          const bool in = (key > floor_key || !full) && col + j < c1;
-          const uint64_t who = __ballot(in);
-          if (who != 0) {
-            if (in) mine[queued + __popcll(who & ((1ull << lane) - 1))] = key;
-            queued += __popcll(who);
-            wave_fence();
-            if (queued >= 64) drain();
+          for (int i = 0; i < M; ++i) {
+            const bool in = (enters >> i & 1u) != 0;
+            const uint64_t who = __ballot(in);
+            if (in) key[at + __popcll(who & ((1ull << lane) - 1))] = item_key(f[i], item(i));
+            at += __popcll(who);
           }
         }
       }
+      __syncthreads();
+      const int n = pool.count, held = pool.first_lost < n ? pool.first_lost : n;
+      __syncthreads();
+      if (n > Pool<NT>::kSize) {
+        // More candidates than room (many equal scores, or rising ones): what is held is cut to the k best, and the waves
+        // that found no room go on one element at a time.
+        pool_keep(pool, held, a.k);
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+          const bool in = lost && item(i) < static_cast<uint32_t>(c1) && f[i] == f[i];
+          pool_step(pool, in, item_key(f[i], item(i)), a.k);
+        }
+        __syncthreads();
+      } else if (n > Pool<NT>::kSize / 2 && base + NT * M < c1) {
+        pool_keep(pool, n, a.k);
+      }
     }
   }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const Stat b{__shfl_xor(r.m, o), __shfl_xor(r.s, o), __shfl_xor(r.w, o)};
-    r = combine(r, b, c);
-  }
+  r = join_lanes<64>(r, c);
   if (lane == 0) part[wave] = r;
-  if constexpr (E > 0) {
-    if (queued > 0) drain();
-#pragma unroll
-    for (int i = 0; i < E; ++i) lists[wave * kList + i * 64 + lane] = best.k[i];
-  }
   __syncthreads();
-  r = part[0];
-  for (int w = 1; w < kWaves; ++w) r = combine(r, part[w], c);
-  if constexpr (E > 0) {
-    if (wave == 0) {
-      for (int w = 1; w < kWaves; ++w) {
-        Best<E> b;
-#pragma unroll
-        for (int i = 0; i < E; ++i) b.k[i] = lists[w * kList + i * 64 + lane];
-        merge<E>(best, b, lane);
-      }
-      if (a.splits == 1) {
-        write_best<E>(a, row, r, best, lane);
+  r = join_lanes<kWaves>(part[lane % kWaves], c);
+  if (a.splits == 1) {
+    const Row w(r, c);
+    finish_row<T>(a, row, r, w, c);
+    if constexpr (TOP) {
+      const int64_t o = static_cast<int64_t>(row) * a.k;
+      if (w.bad) {
+        for (int i = threadIdx.x; i < a.k; i += NT) {
+          a.top_item[o + i] = -1;
+          a.top_logp[o + i] = NAN;
+        }
       } else {
-        uint64_t* to = a.lists + (static_cast<int64_t>(row) * a.splits + split) * a.k;
-#pragma unroll
-        for (int i = 0; i < E; ++i)
-          if (i * 64 + lane < a.k) to[i * 64 + lane] = best.k[i];
+        pool_rank(pool, pool.count, a.k, [&](int rank, uint64_t key) {
+          a.top_item[o + rank] = key_item(key);
+          a.top_logp[o + rank] = w.logp(key_score(key), c, a.scale);
+        });
       }
     }
-  }
-  if (a.splits == 1) {
-    finish_row<T>(a, row, r);
-  } else if (threadIdx.x == 0) {
-    float* to = a.part + (static_cast<int64_t>(row) * a.splits + split) * 4;
-    to[0] = r.m;
-    to[1] = r.s;
-    to[2] = r.w;
+  } else {
+    const int64_t at = static_cast<int64_t>(row) * a.splits + split;
+    if (threadIdx.x == 0) {
+      a.part[at * 4] = r.m;
+      a.part[at * 4 + 1] = r.s;
+      a.part[at * 4 + 2] = r.w;
+    }
+    if constexpr (TOP) {
+      uint64_t* to = a.lists + at * a.k;
+      const int n = pool.count;
+      for (int i = n + threadIdx.x; i < a.k; i += NT) to[i] = 0;
+      pool_rank(pool, n, a.k, [&](int rank, uint64_t key) { to[rank] = key; });
+    }
   }
 }
 
 // Joins a row's shares in their order.
-template <typename T, int E>
-__global__ __launch_bounds__(256) void log_prob_join_kernel(LogProb a) {
-  constexpr int kList = E > 0 ? 64 * E : 1;
-  __shared__ uint64_t lists[E > 0 ? 4 * kList : 1];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.x;
+template <typename T, bool TOP>
+__global__ __launch_bounds__(1024) void log_prob_join_kernel(LogProb a) {
+  constexpr int NT = 1024;
+  __shared__ Pool<TOP ? NT : 0> pool;
+  const int lane = threadIdx.x & 63, row = blockIdx.x;
   const float c = a.scale * kLog2e;
   const float* part = a.part + static_cast<int64_t>(row) * a.splits * 4;
   Stat r{-INFINITY, 0.f, 0.f};
-  for (int p = lane; p < a.splits; p += 64) r = combine(r, {part[4 * p], part[4 * p + 1], part[4 * p + 2]}, c);
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const Stat b{__shfl_xor(r.m, o), __shfl_xor(r.s, o), __shfl_xor(r.w, o)};
-    r = combine(r, b, c);
+  for (int p = lane; p < a.splits; p += 64) {
+    const Stat b{part[4 * p], part[4 * p + 1], part[4 * p + 2]};
+    const float m = max_nan(r.m, b.m);
+    const Stat x = rebase(r, m, c), y = rebase(b, m, c);
+    r = {m, x.s + y.s, x.w + y.w};
   }
-  if constexpr (E > 0) {
-    Best<E> best;
-#pragma unroll
-    for (int i = 0; i < E; ++i) best.k[i] = 0;
-    for (int p = wave; p < a.splits; p += 4) {
-      const uint64_t* from = a.lists + (static_cast<int64_t>(row) * a.splits + p) * a.k;
-      Best<E> b;
-#pragma unroll
-      for (int i = 0; i < E; ++i) b.k[i] = i * 64 + lane < a.k ? from[i * 64 + lane] : 0;
-      merge<E>(best, b, lane);
-    }
-#pragma unroll
-    for (int i = 0; i < E; ++i) lists[wave * kList + i * 64 + lane] = best.k[i];
-    __syncthreads();
-    if (wave == 0) {
-      for (int w = 1; w < 4; ++w) {
-        Best<E> b;
-#pragma unroll
-        for (int i = 0; i < E; ++i) b.k[i] = lists[w * kList + i * 64 + lane];
-        merge<E>(best, b, lane);
+  r = join_lanes<64>(r, c);
+  const Row w(r, c);
+  finish_row<T>(a, row, r, w, c);
+  if constexpr (TOP) {
+    const int64_t o = static_cast<int64_t>(row) * a.k;
+    if (w.bad) {  // uniform
+      for (int i = threadIdx.x; i < a.k; i += NT) {
+        a.top_item[o + i] = -1;
+        a.top_logp[o + i] = NAN;
       }
-      write_best<E>(a, row, r, best, lane);
+      return;
     }
+    pool_start(pool);
+    __syncthreads();
+    const uint64_t* lists = a.lists + static_cast<int64_t>(row) * a.splits * a.k;
+    auto score_at = [&](int64_t i) { return lists[i] != 0 ? key_score(lists[i]) : -INFINITY; };
+    if (a.splits >= a.k) {  // the lists' best scores, dealt to the groups in turn
+      const int groups = a.k <= 48 ? 64 : 256, lanes = NT / groups;
+      float top = -INFINITY;
+      for (int p = threadIdx.x / lanes + groups * (threadIdx.x % lanes); p < a.splits; p += NT)
+        top = fmaxf(top, score_at(static_cast<int64_t>(p) * a.k));
+      pool_floor(pool, top, a.k);
+    } else {  // each list's score at place k / splits, rounded up: k scores at least reach the smallest of them
+      const int place = (a.k + a.splits - 1) / a.splits - 1;
+      if (threadIdx.x < 64) {
+        float low = INFINITY;
+        for (int p = threadIdx.x; p < a.splits; p += 64) low = fminf(low, score_at(static_cast<int64_t>(p) * a.k + place));
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) low = fminf(low, __shfl_xor(low, o));
+        if (lane == 0) pool.floor = low;
+      }
+      __syncthreads();
+    }
+    const int64_t n = static_cast<int64_t>(a.splits) * a.k;
+    for (int64_t base = 0; base < n; base += NT) {
+      const uint64_t key = base + threadIdx.x < n ? lists[base + threadIdx.x] : 0;
+      pool_step(pool, key != 0 && key_score(key) >= pool.floor, key, a.k);
+    }
+    __syncthreads();
+    pool_rank(pool, pool.count, a.k, [&](int rank, uint64_t key) {
+      a.top_item[o + rank] = key_item(key);
+      a.top_logp[o + rank] = w.logp(key_score(key), c, a.scale);
+    });
   }
-  finish_row<T>(a, row, r);
 }
 
 struct LogProbBwd {
@@ -386,6 +459,7 @@ __global__ __launch_bounds__(256) void log_prob_bwd_kernel(LogProbBwd a) {
   const float gh = a.dentropy != nullptr ? a.dentropy[row] : 0.f;
   const float c = a.scale * kLog2e;
   const bool none = m == -INFINITY;
+  const Ref ref(m, c);
   float g = 0.f;
   for (int i = threadIdx.x; i < a.t; i += 256) {
     const int64_t at = static_cast<int64_t>(row) * a.t + i, j = a.items[at];
@@ -400,7 +474,7 @@ __global__ __launch_bounds__(256) void log_prob_bwd_kernel(LogProbBwd a) {
   g = (sums[0] + sums[1]) + (sums[2] + sums[3]);
 
   auto slope = [&](float x, float own) {
-    const float b = (x - m) * c - l2, p = exp2_fast(b);
+    const float b = ref(x, c) - l2, p = exp2_fast(b);
     return none ? 0.f : a.scale * (own - p * (g + gh * (fmaxf(b, kLow) * kLn2 + h)));
   };
   float mine[kMine];
@@ -426,10 +500,10 @@ __global__ __launch_bounds__(256) void log_prob_bwd_kernel(LogProbBwd a) {
   }
   __syncthreads();
   for (int64_t col = c0 + threadIdx.x * V; col < c1; col += 256 * V) {
-    Vec<T> t = load_vec(s + col, c1 - col);
+    Vec<T> t = load_row(s, col, c1);
 #pragma unroll
     for (int j = 0; j < V; ++j) t.e[j] = static_cast<T>(slope(static_cast<float>(t.e[j]), 0.f));
-    store_vec(ds + col, t, c1 - col);
+    store_row(ds, col, c1, t);
   }
   __syncthreads();
 #pragma unroll
@@ -441,15 +515,18 @@ struct Plan {
   int32_t splits, per;
 };
 
-// Shares of a row: enough blocks for the chip where there are few rows, and no share under 8192 columns.
+constexpr int32_t kTileCols = 8192;   // a 256-thread block's, 32 a thread
+constexpr int32_t kWideCols = 16384;  // a 1024-thread block's, 16 a thread
+
+// One block a row where a row fits a block's registers, or there are rows enough; else shares of whole tiles, about 4
+// blocks a CU in all.
 Plan plan_rows(int32_t rows, int32_t cols) {
-  if (rows < 1) return {1, cols};
+  if (rows < 1 || cols <= kWideCols || rows >= 4 * kCUs) return {1, cols};
+  const int64_t tiles = (static_cast<int64_t>(cols) + kTileCols - 1) / kTileCols;
   int64_t splits = (4 * kCUs + rows - 1) / rows;
-  const int64_t most = (static_cast<int64_t>(cols) + 8191) / 8192;
-  if (splits > most) splits = most;
-  if (cols <= 16384) splits = 1;
-  const int64_t per = ((cols + splits - 1) / splits + 2047) / 2048 * 2048;
-  if (splits == 1 || per >= cols) return {1, cols};
+  if (splits > tiles) splits = tiles;
+  const int64_t per = (tiles + splits - 1) / splits * kTileCols;
+  if (per >= cols) return {1, cols};
   return {static_cast<int32_t>((cols + per - 1) / per), static_cast<int32_t>(per)};
 }
 
@@ -458,16 +535,18 @@ int64_t work_floats(int32_t rows, int32_t cols, int32_t k) {
   return p.splits == 1 ? 0 : static_cast<int64_t>(rows) * p.splits * (4 + 2 * static_cast<int64_t>(k));
 }
 
-template <typename T, int E>
+template <typename T, bool TOP>
 int log_prob(const LogProb& a, hipStream_t st) {
   const dim3 grid(a.rows, a.splits);
-  if (a.splits == 1 && a.cols > 4096 && a.rows <= 2 * kCUs)
-    hipLaunchKernelGGL((log_prob_kernel<T, E, 1024>), grid, dim3(1024), 0, st, a);
+  if (a.cols <= 2048)
+    hipLaunchKernelGGL((log_prob_kernel<T, TOP, 256, 8>), grid, dim3(256), 0, st, a);
+  else if (a.cols <= kWideCols && a.rows <= 2 * kCUs)  // few rows: each in one step of a whole CU's threads
+    hipLaunchKernelGGL((log_prob_kernel<T, TOP, 1024, 16>), grid, dim3(1024), 0, st, a);
   else
-    hipLaunchKernelGGL((log_prob_kernel<T, E, 256>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((log_prob_kernel<T, TOP, 256, 32>), grid, dim3(256), 0, st, a);
   KGAT_LAUNCH_CHECK();
   if (a.splits > 1) {
-    hipLaunchKernelGGL((log_prob_join_kernel<T, E>), dim3(a.rows), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((log_prob_join_kernel<T, TOP>), dim3(a.rows), dim3(1024), 0, st, a);
     KGAT_LAUNCH_CHECK();
   }
   return KGAT_OK;
@@ -505,7 +584,7 @@ extern "C" int kgat_log_prob_fwd(int32_t dtype, const void* scores, int64_t ld, 
     using T = decltype(e);
     if (rows == 0) return KGAT_OK;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    return k == 0 ? log_prob<T, 0>(a, st) : k <= 64 ? log_prob<T, 1>(a, st) : log_prob<T, 2>(a, st);
+    return k == 0 ? log_prob<T, false>(a, st) : log_prob<T, true>(a, st);
   });
 }
 
