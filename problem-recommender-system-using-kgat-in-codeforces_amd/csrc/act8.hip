@@ -121,6 +121,7 @@ struct Wgrad {
   const int8_t* q;
   const uint8_t* e;
   float* out;      // [splits][o][d]
+  float* bias;     // [splits][tiles_d][o] (nullable): the column sums of the rows that a block counts
   int64_t n, per;  // rows, rows of a split (a multiple of kDepth; every split has one at least)
   int32_t o, d, nb;
   int32_t tiles_o, tiles_d, splits;
@@ -203,6 +204,19 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
 
   Quad<T> y[8];
   uint32_t x[8], code[8];
+  // The column sums of dy: the tiles of a split share its steps out among them.
+  float bias[4] = {0.f, 0.f, 0.f, 0.f};
+  int turns = i0 / B;  // steps until this block's next one
+  auto add_bias = [&]() {
+    if (turns == 0) {
+      turns = a.tiles_d;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bias[j] += static_cast<float>(y[k].e[j]);
+    }
+    --turns;
+  };
   auto row_of = [&](const T* p) {
     if constexpr (NARROW) {
       Quad<T> v;
@@ -298,6 +312,7 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
 
   fetch(r1 - r0);
   if constexpr (kStages<T> == 2) {
+    if (a.bias != nullptr) add_bias();
 #pragma unroll
     for (int j = 0; j < 4; ++j) store(lds, j);
     if (r0 + kDepth < r1) fetch(r1 - r0 - kDepth);
@@ -310,6 +325,7 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
       multiply(now, 0);
       multiply(now, 1);
       if (r + kDepth < r1) {
+        if (a.bias != nullptr) add_bias();
         store(lds + turn * kBuffer, 0);
         store(lds + turn * kBuffer, 1);
       }
@@ -326,6 +342,7 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
   } else {
     int64_t r = r0;
     do {
+      if (a.bias != nullptr) add_bias();
       __syncthreads();  // the last step's operands are read
 #pragma unroll
       for (int j = 0; j < 4; ++j) store(lds, j);
@@ -335,6 +352,20 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
       for (int s = 0; s < kDepth / 16; ++s) multiply(lds, s);
       r += kDepth;
     } while (r < r1);
+  }
+  if (a.bias != nullptr) {  // the 8 row groups' sums, in their order
+    float* sums = reinterpret_cast<float*>(lds);
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sums[kg * B + (B / 4) * j + cg] = bias[j];
+    __syncthreads();
+    if (tid < B) {
+      const int32_t row = first_of(o0 + tid % (B / 4) * 4, a.o) + tid / (B / 4);
+      float v = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v += sums[k * B + tid];
+      if (!NARROW || row < a.o) a.bias[(static_cast<int64_t>(split) * a.tiles_d + i0 / B) * a.o + row] = v;
+    }
   }
   float* out = a.out + static_cast<int64_t>(split) * a.o * a.d;
 #pragma unroll
@@ -353,52 +384,53 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
   }
 }
 
-// The column sums of dy by row shares: 64 columns a block, its 4 waves every fourth row.
-template <typename T>
-__global__ __launch_bounds__(256) void act8_dbias_kernel(const T* dy, int64_t lddy, int64_t n, int32_t o, int64_t per,
-                                                         float* part) {
+// Sums of parts, in their order: the first blocks take dW's elements, the others db's.  64 elements a block, its 4
+// waves every fourth part.
+struct Join {
+  const float* part[2];
+  float* out[2];
+  int64_t size[2];
+  int32_t parts[2];
+  uint32_t blocks;  // of the first
+};
+
+__global__ __launch_bounds__(256) void act8_join_kernel(Join a) {
   __shared__ float lds[4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int32_t c = blockIdx.x * 64 + lane;
-  const int64_t r0 = blockIdx.y * per, r1 = r0 + per < n ? r0 + per : n;
+  const int which = blockIdx.x < a.blocks ? 0 : 1;
+  const int64_t i = static_cast<int64_t>(blockIdx.x - (which != 0 ? a.blocks : 0)) * 64 + lane, size = a.size[which];
+  const float* part = a.part[which];
+  const int parts = a.parts[which];
   float s = 0.f;
-  if (c < o)
-    for (int64_t r = r0 + wave; r < r1; r += 4) s += static_cast<float>(dy[r * lddy + c]);
+  if (i < size)
+#pragma unroll 8
+    for (int p = wave; p < parts; p += 4) s += part[p * size + i];
   lds[wave][lane] = s;
   __syncthreads();
-  if (wave == 0 && c < o) part[static_cast<int64_t>(blockIdx.y) * o + c] = (lds[0][lane] + lds[1][lane]) + (lds[2][lane] + lds[3][lane]);
-}
-
-// out[i] = sum over the parts, in their order, of part[p][i].
-__global__ __launch_bounds__(256) void act8_join_kernel(const float* part, int32_t parts, int64_t n, float* out) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= n) return;
-  float s = 0.f;
-  for (int p = 0; p < parts; ++p) s += part[p * n + i];
-  out[i] = s;
+  if (wave == 0 && i < size) a.out[which][i] = (lds[0][lane] + lds[1][lane]) + (lds[2][lane] + lds[3][lane]);
 }
 
 struct Splits {
   int32_t tile;  // B
-  int32_t w, b;  // row shares of dW and of db
-  int64_t per;   // rows of a share of dW
+  int32_t tiles_o, tiles_d;
+  int32_t w;     // row shares
+  int64_t per;   // rows of a share
+  int64_t floats(int32_t o, int32_t d) const {  // workspace: the shares' tiles, and their column sums
+    return static_cast<int64_t>(w) * o * d + static_cast<int64_t>(w) * tiles_d * o;
+  }
 };
 
 template <typename T>
 Splits wgrad_splits(int64_t n, int32_t o, int32_t d) {
   const int64_t least = o < d ? o : d;
   const int32_t tile = kPlanes<T> == 1 && least > 128 ? 256 : least > 64 ? 128 : 64;
-  const int64_t tiles = static_cast<int64_t>((o + tile - 1) / tile) * ((d + tile - 1) / tile);
+  const int32_t tiles_o = (o + tile - 1) / tile, tiles_d = (d + tile - 1) / tile;
   const int64_t fill = tile == 256 ? kCUs : tile == 128 ? 2 * kCUs : 4 * kCUs;  // blocks the chip holds
-  int64_t w = fill / tiles, most = (n + 511) / 512;
+  int64_t w = fill / (static_cast<int64_t>(tiles_o) * tiles_d), most = (n + 511) / 512;
   if (w > most) w = most;
   if (w < 1) w = 1;
   const int64_t per = n < 1 ? kDepth : ((n + w - 1) / w + kDepth - 1) / kDepth * kDepth;
-  const int64_t strips = (o + 63) / 64;
-  int64_t b = (4 * kCUs + strips - 1) / strips;
-  most = (n + 63) / 64;
-  if (b > most) b = most;
-  return {tile, static_cast<int32_t>(n < 1 ? 1 : (n + per - 1) / per), static_cast<int32_t>(b < 1 ? 1 : b), per};
+  return {tile, tiles_o, tiles_d, static_cast<int32_t>(n < 1 ? 1 : (n + per - 1) / per), per};
 }
 
 bool act8_shape_ok(int64_t n, int32_t d) { return n >= 0 && d >= 1 && d <= KGAT_ACT8_MAX_D; }
@@ -453,8 +485,7 @@ extern "C" int kgat_act8_unpack(int32_t dtype, const int8_t* q, const uint8_t* e
 extern "C" int64_t kgat_act8_wgrad_workspace(int32_t dtype, int64_t n, int32_t o, int32_t d) {
   using namespace kgat;
   if (!act8_shape_ok(n, d) || o < 1 || o > KGAT_ACT8_MAX_D || dtype < KGAT_F32 || dtype > KGAT_F16) return -1;
-  const Splits s = dtype == KGAT_BF16 ? wgrad_splits<__bf16>(n, o, d) : wgrad_splits<float>(n, o, d);
-  return static_cast<int64_t>(s.w) * o * d + static_cast<int64_t>(s.b) * o;
+  return (dtype == KGAT_BF16 ? wgrad_splits<__bf16>(n, o, d) : wgrad_splits<float>(n, o, d)).floats(o, d);
 }
 
 extern "C" int kgat_act8_wgrad(int32_t dtype, const void* dy, int64_t lddy, const int8_t* q, const uint8_t* e,
@@ -469,38 +500,29 @@ extern "C" int kgat_act8_wgrad(int32_t dtype, const void* dy, int64_t lddy, cons
   return with_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
     const Splits s = wgrad_splits<T>(n, o, d);
-    float* part_b = workspace + static_cast<int64_t>(s.w) * o * d;
     const int64_t size = static_cast<int64_t>(o) * d;
+    float* part_b = workspace + s.w * size;
+    Join j{{workspace, part_b}, {dW, db}, {size, o}, {s.w, s.w * s.tiles_d}, 0};
     if (n == 0) {  // sums of nothing
-      hipLaunchKernelGGL(act8_join_kernel, dim3(static_cast<uint32_t>((size + 255) / 256)), dim3(256), 0, st, workspace,
-                         0, size, dW);
-      KGAT_LAUNCH_CHECK();
-      if (db != nullptr)
-        hipLaunchKernelGGL(act8_join_kernel, dim3((o + 255) / 256), dim3(256), 0, st, part_b, 0, static_cast<int64_t>(o), db);
-      KGAT_LAUNCH_CHECK();
-      return KGAT_OK;
-    }
-    const Wgrad a{dy, lddy, q, e, s.w == 1 ? dW : workspace, n, s.per, o, d, (d + kBlock - 1) / kBlock,
-                  (o + s.tile - 1) / s.tile, (d + s.tile - 1) / s.tile, s.w};
-    const int64_t blocks = static_cast<int64_t>(a.tiles_o) * a.tiles_d * s.w;
-    if (blocks > 0x7FFFFFFF) return KGAT_ERR_INVALID;
-    const dim3 grid(static_cast<uint32_t>(blocks));
-    if (o < 4) hipLaunchKernelGGL((act8_wgrad_kernel<T, 64, true>), grid, dim3(128), 0, st, a);
-    else if (s.tile == 64) hipLaunchKernelGGL((act8_wgrad_kernel<T, 64, false>), grid, dim3(128), 0, st, a);
-    else if (s.tile == 128) hipLaunchKernelGGL((act8_wgrad_kernel<T, 128, false>), grid, dim3(256), 0, st, a);
-    else if constexpr (kPlanes<T> == 1) hipLaunchKernelGGL((act8_wgrad_kernel<T, 256, false>), grid, dim3(512), 0, st, a);
-    KGAT_LAUNCH_CHECK();
-    if (s.w > 1) {
-      hipLaunchKernelGGL(act8_join_kernel, dim3(static_cast<uint32_t>((size + 255) / 256)), dim3(256), 0, st, workspace,
-                         s.w, size, dW);
+      j.parts[0] = j.parts[1] = 0;
+    } else {
+      const Wgrad a{dy, lddy, q, e, s.w == 1 ? dW : workspace, db == nullptr ? nullptr : j.parts[1] == 1 ? db : part_b,
+                    n, s.per, o, d, (d + kBlock - 1) / kBlock, s.tiles_o, s.tiles_d, s.w};
+      const int64_t blocks = static_cast<int64_t>(s.tiles_o) * s.tiles_d * s.w;
+      if (blocks > 0x7FFFFFFF) return KGAT_ERR_INVALID;
+      const dim3 grid(static_cast<uint32_t>(blocks));
+      if (o < 4) hipLaunchKernelGGL((act8_wgrad_kernel<T, 64, true>), grid, dim3(128), 0, st, a);
+      else if (s.tile == 64) hipLaunchKernelGGL((act8_wgrad_kernel<T, 64, false>), grid, dim3(128), 0, st, a);
+      else if (s.tile == 128) hipLaunchKernelGGL((act8_wgrad_kernel<T, 128, false>), grid, dim3(256), 0, st, a);
+      else if constexpr (kPlanes<T> == 1) hipLaunchKernelGGL((act8_wgrad_kernel<T, 256, false>), grid, dim3(512), 0, st, a);
       KGAT_LAUNCH_CHECK();
     }
-    if (db != nullptr) {
-      hipLaunchKernelGGL(act8_dbias_kernel<T>, dim3((o + 63) / 64, s.b), dim3(256), 0, st, static_cast<const T*>(dy),
-                         lddy, n, o, (n + s.b - 1) / s.b, part_b);
-      KGAT_LAUNCH_CHECK();
-      hipLaunchKernelGGL(act8_join_kernel, dim3((o + 255) / 256), dim3(256), 0, st, part_b, s.b,
-                         static_cast<int64_t>(o), db);
+    const int64_t blocks_w = j.parts[0] == 1 ? 0 : (size + 63) / 64;
+    const int64_t blocks_b = db == nullptr || j.parts[1] == 1 ? 0 : (o + 63) / 64;
+    if (blocks_w + blocks_b > 0x7FFFFFFF) return KGAT_ERR_INVALID;
+    if (blocks_w + blocks_b > 0) {
+      j.blocks = static_cast<uint32_t>(blocks_w);
+      hipLaunchKernelGGL(act8_join_kernel, dim3(static_cast<uint32_t>(blocks_w + blocks_b)), dim3(256), 0, st, j);
       KGAT_LAUNCH_CHECK();
     }
     return KGAT_OK;

@@ -241,11 +241,15 @@ __global__ __launch_bounds__(NT, 4) void log_prob_kernel(LogProb a) {
   if constexpr (TOP) pool_start(pool);
 
   Stat r{-INFINITY, 0.f, 0.f};
-  for (int64_t base = c0; base < c1; base += NT * M) {
-    float f[M];
-    Vec<T> t[U];
+  Vec<T> t[U];
+  auto fetch = [&](int64_t base) {
 #pragma unroll
     for (int u = 0; u < U; ++u) t[u] = load_row(s, base + (u * NT + threadIdx.x) * V, c1);
+  };
+  if constexpr (!TOP) fetch(c0);
+  for (int64_t base = c0; base < c1; base += NT * M) {
+    if constexpr (TOP) fetch(base);
+    float f[M];
     const bool whole = base + NT * M <= c1;  // uniform
     float top = -INFINITY;
 #pragma unroll
@@ -257,23 +261,31 @@ __global__ __launch_bounds__(NT, 4) void log_prob_kernel(LogProb a) {
         f[u * V + j] = x;
         top = max_nan(top, x);
       }
+    if constexpr (!TOP) {  // the next columns are on their way meanwhile (with the candidates' registers: other blocks)
+      if (base + NT * M < c1) fetch(base + NT * M);
+    }
     r = rebase(r, max_nan(r.m, top), c);
     const Ref ref(r.m, c);
-    if (!__any(ref.far && r.m != -INFINITY)) {
+    const bool far = __any(ref.far && r.m != -INFINITY);
 #pragma unroll
-      for (int i = 0; i < M; ++i) {
-        const float x = fmaxf(__builtin_fmaf(f[i], c, -ref.rho), kLow);  // -inf (and NaN, which r.m holds): kLow
-        const float e = exp2_fast(x);
-        r.s += e;
-        r.w += e * x;
-      }
-    } else {
+    for (int u = 0; u < U; ++u) {
+      if (base + u * NT * V >= c1) break;  // uniform: a row's last columns seldom fill a step
+      if (!far) {
 #pragma unroll
-      for (int i = 0; i < M; ++i) {
-        const float x = fmaxf(ref(f[i], c), kLow);
-        const float e = exp2_fast(x);
-        r.s += e;
-        r.w += e * x;
+        for (int j = 0; j < V; ++j) {
+          const float x = fmaxf(__builtin_fmaf(f[u * V + j], c, -ref.rho), kLow);  // -inf (and NaN, which r.m holds): kLow
+          const float e = exp2_fast(x);
+          r.s += e;
+          r.w += e * x;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float x = fmaxf(ref(f[u * V + j], c), kLow);
+          const float e = exp2_fast(x);
+          r.s += e;
+          r.w += e * x;
+        }
       }
     }
     if constexpr (TOP) {
