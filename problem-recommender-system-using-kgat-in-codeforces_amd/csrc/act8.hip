@@ -49,11 +49,11 @@ __global__ __launch_bounds__(256) void act8_pack_kernel(Pack a) {
     const uint32_t b = __float_as_uint(f[j]) & 0x7FFFFFFFu;  // |f| orders as its bits; inf and NaN are the largest
     top = top > b ? top : b;
   }
-#pragma unroll
-  for (int o = 1; o < kLanes; o <<= 1) {
-    const uint32_t b = static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o));
-    top = top > b ? top : b;
-  }
+  // Bits of values >= 0 order as integers: the maximum over the block's lanes.
+  top = __float_as_uint(lanes_all<kLanes>(__uint_as_float(top), [](float x, float y) {
+    const uint32_t p = __float_as_uint(x), q = __float_as_uint(y);
+    return __uint_as_float(p > q ? p : q);
+  }));
   if (!live) return;
   const uint32_t ex = top >> 23;  // biased exponent of the maximum
   const uint32_t code = ex == 255 ? 255u : ex < 7 ? 1u : ex - 6;

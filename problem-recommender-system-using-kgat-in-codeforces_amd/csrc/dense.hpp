@@ -73,6 +73,36 @@ __device__ __forceinline__ void store_row(T* row, int64_t c, int64_t d, Vec<T> v
   }
 }
 
+template <int CTRL>
+__device__ __forceinline__ float lane_row(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, false));
+}
+
+// op over the N lanes that share lane / N (N = 2 ... 64), the result in all of them: within a row of 16 by DPP (see
+// sum16), then rows and halves against each other (v_permlane16_swap and v_permlane32_swap of a register with itself
+// leave the even rows' values in one result and the odd rows' in the other) -- no trip through the LDS crossbar.
+// Every level joins the same two parts as lane ^ 1, ^ 2, ^ 4, ... would.  All lanes have to be active.
+template <int N, typename F>
+__device__ __forceinline__ float lanes_all(float v, F&& op) {
+  if constexpr (N >= 2) v = op(v, lane_row<0xB1>(v));
+  if constexpr (N >= 4) v = op(v, lane_row<0x4E>(v));
+  if constexpr (N >= 8) v = op(v, lane_row<0x141>(v));
+  if constexpr (N >= 16) v = op(v, lane_row<0x140>(v));
+  if constexpr (N >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
+  if constexpr (N >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
+  return v;
+}
+template <int N>
+__device__ __forceinline__ float lanes_sum(float v) {
+  return lanes_all<N>(v, [](float a, float b) { return a + b; });
+}
+
 // Host: calls f(T{}) with the element type of a KGAT_F32 / BF16 / F16 code; an unknown code is KGAT_ERR_INVALID.
 template <typename F>
 inline int with_dtype(int32_t dtype, F&& f) {

@@ -63,9 +63,7 @@ __device__ __forceinline__ void load_columns(const NormVec& w, int lane, int G, 
 template <int G, int THREADS, int K>
 __device__ __forceinline__ void group_sum(float (&v)[K], float* lds, int& turn) {
 #pragma unroll
-  for (int o = (G < 64 ? G : 64) / 2; o > 0; o >>= 1)
-#pragma unroll
-    for (int i = 0; i < K; ++i) v[i] += __shfl_xor(v[i], o);
+  for (int i = 0; i < K; ++i) v[i] = lanes_sum<(G < 64 ? G : 64)>(v[i]);
   if constexpr (G > 64) {
     constexpr int kWaves = THREADS / 64;
     const int wave = threadIdx.x >> 6;

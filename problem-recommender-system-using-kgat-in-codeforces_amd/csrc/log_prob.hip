@@ -53,15 +53,10 @@ __device__ __forceinline__ Stat rebase(Stat a, float to, float c) {
 // Joins the parts of N lanes (a power of two): the largest maximum first, one rescaling each, then plain sums.
 template <int N>
 __device__ __forceinline__ Stat join_lanes(Stat a, float c) {
-  float m = a.m;
-#pragma unroll
-  for (int o = 1; o < N; o <<= 1) m = max_nan(m, __shfl_xor(m, o));
+  const float m = lanes_all<N>(a.m, max_nan);
   a = rebase(a, m, c);
-#pragma unroll
-  for (int o = 1; o < N; o <<= 1) {
-    a.s += __shfl_xor(a.s, o);
-    a.w += __shfl_xor(a.w, o);
-  }
+  a.s = lanes_sum<N>(a.s);
+  a.w = lanes_sum<N>(a.w);
   return a;
 }
 
@@ -96,9 +91,25 @@ struct Row {
   }
 };
 
+// A given item of the row and its score, loaded long before they are needed.
+struct Given {
+  int64_t item;
+  float score;
+};
+
 template <typename T>
-__device__ __forceinline__ void finish_row(const LogProb& a, int row, Stat r, const Row& w, float c) {
-  const T* s = static_cast<const T*>(a.s) + static_cast<int64_t>(row) * a.ld;
+__device__ __forceinline__ Given load_given(const LogProb& a, int row, int i) {
+  Given g{-1, 0.f};
+  if (i < a.t) {
+    g.item = a.items[static_cast<int64_t>(row) * a.t + i];
+    if (g.item >= 0 && g.item < a.cols) g.score = static_cast<float>((static_cast<const T*>(a.s) + static_cast<int64_t>(row) * a.ld)[g.item]);
+  }
+  return g;
+}
+
+// `g`: load_given of the thread's first item.
+template <typename T>
+__device__ __forceinline__ void finish_row(const LogProb& a, int row, Stat r, const Row& w, float c, Given g) {
   const int64_t rows = a.rows;
   if (threadIdx.x == 0) {
     a.stats[row] = w.bad ? NAN : r.m;
@@ -107,8 +118,8 @@ __device__ __forceinline__ void finish_row(const LogProb& a, int row, Stat r, co
     a.stats[3 * rows + row] = w.bad ? NAN : w.none ? -INFINITY : w.ref.far ? r.m * a.scale + w.l2 * kLn2 : (w.ref.rho + w.l2) * kLn2;
   }
   for (int i = threadIdx.x; i < a.t; i += blockDim.x) {
-    const int64_t at = static_cast<int64_t>(row) * a.t + i, j = a.items[at];
-    a.logp[at] = j < 0 ? 0.f : j >= a.cols ? NAN : w.logp(static_cast<float>(s[j]), c, a.scale);
+    if (i != static_cast<int>(threadIdx.x)) g = load_given<T>(a, row, i);
+    a.logp[static_cast<int64_t>(row) * a.t + i] = g.item < 0 ? 0.f : g.item >= a.cols ? NAN : w.logp(g.score, c, a.scale);
   }
 }
 
@@ -139,7 +150,7 @@ struct Pool {
   float group_floor[4];
   int count, first_lost, now;
   uint64_t floor_key;  // the k-th key, once k were kept (0: none)
-  float floor;         // no smaller score enters
+  float floor;         // no smaller score enters: behind the columns of the keys kept, an equal one ranks after them
 };
 
 template <int NT>
@@ -177,7 +188,7 @@ __device__ __forceinline__ void pool_keep(Pool<NT>& p, int n, int k) {
     p.first_lost = 0x7FFFFFFF;
     if (n >= k) {
       p.floor_key = to[k - 1];
-      p.floor = key_score(to[k - 1]);
+      p.floor = nextafterf(key_score(to[k - 1]), INFINITY);
     }
   }
   __syncthreads();
@@ -214,9 +225,7 @@ __device__ __forceinline__ void pool_floor(Pool<NT>& p, float top, int k) {
     int reach = 0;
 #pragma unroll 8
     for (int j = 0; j < groups; ++j) reach += p.group[j] >= mine ? 1 : 0;
-    float v = reach >= k ? mine : -INFINITY;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v = fmaxf(v, __shfl_xor(v, o));
+    const float v = lanes_all<64>(reach >= k ? mine : -INFINITY, [](float x, float y) { return fmaxf(x, y); });
     if ((threadIdx.x & 63) == 0) p.group_floor[threadIdx.x >> 6] = v;
   }
   __syncthreads();
@@ -239,6 +248,8 @@ __global__ __launch_bounds__(NT, 4) void log_prob_kernel(LogProb a) {
   const int64_t c1 = c0 + a.per < a.cols ? c0 + a.per : a.cols;
   const float c = a.scale * kLog2e;
   if constexpr (TOP) pool_start(pool);
+  Given given{-1, 0.f};
+  if (a.splits == 1) given = load_given<T>(a, row, threadIdx.x);
 
   Stat r{-INFINITY, 0.f, 0.f};
   Vec<T> t[U];
@@ -251,16 +262,19 @@ __global__ __launch_bounds__(NT, 4) void log_prob_kernel(LogProb a) {
     if constexpr (TOP) fetch(base);
     float f[M];
     const bool whole = base + NT * M <= c1;  // uniform
-    float top = -INFINITY;
+    float top = -INFINITY, tops[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      tops[u] = -INFINITY;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         float x = static_cast<float>(t[u].e[j]);
         if (!whole && base + (u * NT + threadIdx.x) * V + j >= c1) x = -INFINITY;
         f[u * V + j] = x;
-        top = max_nan(top, x);
+        tops[u] = max_nan(tops[u], x);
       }
+      top = max_nan(top, tops[u]);
+    }
     if constexpr (!TOP) {  // the next columns are on their way meanwhile (with the candidates' registers: other blocks)
       if (base + NT * M < c1) fetch(base + NT * M);
     }
@@ -290,37 +304,41 @@ __global__ __launch_bounds__(NT, 4) void log_prob_kernel(LogProb a) {
     }
     if constexpr (TOP) {
       if (base == c0) pool_floor(pool, top, a.k);
-      // Candidates: a wave reserves room for all of its own at once.
+      // Candidates: a wave reserves room for all of its own at once.  Few vectors hold one, and few of their elements
+      // reach it, so the loops are a comparison and a scalar branch an element.
       const float floor = pool.floor;
-      const uint64_t floor_key = pool.floor_key;
+      const bool bounded = whole || floor > -INFINITY;  // uniform; else the filled-up columns would enter
       auto item = [&](int i) { return static_cast<uint32_t>(base) + (i / V * NT + threadIdx.x) * V + i % V; };
+      auto enters = [&](int i) { return f[i] >= floor && (bounded || item(i) < static_cast<uint32_t>(c1)); };
       bool lost = false;
       if (__any(top >= floor)) {
-        uint32_t enters = 0;
         int mine = 0;
 #pragma unroll
-        for (int i = 0; i < M; ++i) {
-          bool in = f[i] >= floor;
-          if (!whole) in = in && item(i) < static_cast<uint32_t>(c1);
-          if (floor_key != 0) in = in && item_key(f[i], item(i)) > floor_key;
-          enters |= in ? 1u << i : 0u;
-          mine += __popcll(__ballot(in));
-        }
+        for (int u = 0; u < U; ++u)
+          if (__any(tops[u] >= floor))
+#pragma unroll
+            for (int j = 0; j < V; ++j) mine += __popcll(__ballot(enters(u * V + j)));
         int at = 0;
         if (lane == 0 && mine > 0) at = atomicAdd(&pool.count, mine);
         at = __shfl(at, 0);
         lost = mine > 0 && at + mine > Pool<NT>::kSize;
         if (lost) {
           if (lane == 0) atomicMin(&pool.first_lost, at);
-        } else if (mine > 0) {
+        } else {
           uint64_t* key = pool.key[pool.now];
 #pragma unroll
-          for (int i = 0; i < M; ++i) {
-            const bool in = (enters >> i & 1u) != 0;
-            const uint64_t who = __ballot(in);
-            if (in) key[at + __popcll(who & ((1ull << lane) - 1))] = item_key(f[i], item(i));
-            at += __popcll(who);
-          }
+          for (int u = 0; u < U; ++u)
+            if (__any(tops[u] >= floor))
+#pragma unroll
+              for (int j = 0; j < V; ++j) {
+                const int i = u * V + j;
+                const bool in = enters(i);
+                const uint64_t who = __ballot(in);
+                if (who != 0) {
+                  if (in) key[at + __popcll(who & ((1ull << lane) - 1))] = item_key(f[i], item(i));
+                  at += __popcll(who);
+                }
+              }
         }
       }
       __syncthreads();
@@ -336,8 +354,8 @@ __global__ __launch_bounds__(NT, 4) void log_prob_kernel(LogProb a) {
           pool_step(pool, in, item_key(f[i], item(i)), a.k);
         }
         __syncthreads();
-      } else if (n > Pool<NT>::kSize / 2 && base + NT * M < c1) {
-        pool_keep(pool, n, a.k);
+      } else if (n > a.k + 32 && base + NT * M < c1) {
+        pool_keep(pool, n, a.k);  // raises the floor for the columns to come
       }
     }
   }
@@ -347,7 +365,7 @@ __global__ __launch_bounds__(NT, 4) void log_prob_kernel(LogProb a) {
   r = join_lanes<kWaves>(part[lane % kWaves], c);
   if (a.splits == 1) {
     const Row w(r, c);
-    finish_row<T>(a, row, r, w, c);
+    finish_row<T>(a, row, r, w, c, given);
     if constexpr (TOP) {
       const int64_t o = static_cast<int64_t>(row) * a.k;
       if (w.bad) {
@@ -386,6 +404,7 @@ __global__ __launch_bounds__(1024) void log_prob_join_kernel(LogProb a) {
   const int lane = threadIdx.x & 63, row = blockIdx.x;
   const float c = a.scale * kLog2e;
   const float* part = a.part + static_cast<int64_t>(row) * a.splits * 4;
+  const Given given = load_given<T>(a, row, threadIdx.x);
   Stat r{-INFINITY, 0.f, 0.f};
   for (int p = lane; p < a.splits; p += 64) {
     const Stat b{part[4 * p], part[4 * p + 1], part[4 * p + 2]};
@@ -395,7 +414,7 @@ __global__ __launch_bounds__(1024) void log_prob_join_kernel(LogProb a) {
   }
   r = join_lanes<64>(r, c);
   const Row w(r, c);
-  finish_row<T>(a, row, r, w, c);
+  finish_row<T>(a, row, r, w, c, given);
   if constexpr (TOP) {
     const int64_t o = static_cast<int64_t>(row) * a.k;
     if (w.bad) {  // uniform
@@ -427,9 +446,10 @@ __global__ __launch_bounds__(1024) void log_prob_join_kernel(LogProb a) {
       __syncthreads();
     }
     const int64_t n = static_cast<int64_t>(a.splits) * a.k;
+    const float floor = pool.floor;
     for (int64_t base = 0; base < n; base += NT) {
       const uint64_t key = base + threadIdx.x < n ? lists[base + threadIdx.x] : 0;
-      pool_step(pool, key != 0 && key_score(key) >= pool.floor, key, a.k);
+      pool_step(pool, key != 0 && key_score(key) >= floor, key, a.k);
     }
     __syncthreads();
     pool_rank(pool, pool.count, a.k, [&](int rank, uint64_t key) {
