@@ -110,6 +110,7 @@ __global__ __launch_bounds__(256) void act8_unpack_kernel(Unpack a) {
 // v_mfma_f32_32x32x16_bf16.  Column 4 c + j of the tile lies at LDS row (B / 4) j + c: the threads of a row write
 // neighbouring LDS rows at a pitch of 36 dwords, which spreads 16 of them over all 64 banks.
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 
 constexpr int kDepth = 64;                  // rows a step
@@ -121,7 +122,7 @@ struct Wgrad {
   const int8_t* q;
   const uint8_t* e;
   float* out;      // [splits][o][d]
-  float* bias;     // [splits][tiles_d][o] (nullable): the column sums of the rows that a block counts
+  float* bias;     // [splits][o] (nullable): the column sums of dy
   int64_t n, per;  // rows, rows of a split (a multiple of kDepth; every split has one at least)
   int32_t o, d, nb;
   int32_t tiles_o, tiles_d, splits;
@@ -191,7 +192,12 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
   const T* dy = static_cast<const T*>(a.dy) + (r0 + kg * 8) * a.lddy + first_of(o0 + cg * 4, a.o);
   const int32_t ic = first_of(i0 + cg * 4, ldq);
   const int8_t* qp = a.q + (r0 + kg * 8) * ldq + ic;
-  const uint8_t* ep = a.e + (r0 + kg * 8) * a.nb + ic / kBlock;
+  // The scales of 8 rows and the tile's blocks are one byte for each of the B / 4 threads of a row group: a thread loads
+  // one, and takes its 8 rows' by lane exchange (a load for each was a sixth of the kernel's time).
+  constexpr int kTileBlocks = B / kBlock;
+  const int32_t eb = i0 / kBlock + cg % kTileBlocks < a.nb ? i0 / kBlock + cg % kTileBlocks : a.nb - 1;
+  const uint8_t* ep = a.e + (r0 + kg * 8 + cg / kTileBlocks) * a.nb + eb;
+  const int code_lane = (lane - cg % 64 + cg / (kBlock / 4)) * 4;  // of the group's first row, for ds_bpermute
 
   floatx16 acc[FM][FN];
 #pragma unroll
@@ -203,20 +209,9 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
   const int wm = (wave / kWavesN) * FM * 32, wn = (wave % kWavesN) * FN * 32;
 
   Quad<T> y[8];
-  uint32_t x[8], code[8];
-  // The column sums of dy: the tiles of a split share its steps out among them.
+  uint32_t x[8], codes;
+  // The column sums of dy: every block forms them, one instruction for two terms, and the first of its strip writes them.
   float bias[4] = {0.f, 0.f, 0.f, 0.f};
-  int turns = i0 / B;  // steps until this block's next one
-  auto add_bias = [&]() {
-    if (turns == 0) {
-      turns = a.tiles_d;
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) bias[j] += static_cast<float>(y[k].e[j]);
-    }
-    --turns;
-  };
   auto row_of = [&](const T* p) {
     if constexpr (NARROW) {
       Quad<T> v;
@@ -227,34 +222,44 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
       return load_quad(p);
     }
   };
-  // The next kDepth rows' operands, `left` of them in the share: behind the last one x repeats it and dy is 0.
-  auto fetch = [&](int64_t left) {
-    if (left >= kDepth) {
+  // The next kDepth rows' operands.
+  auto fetch_all = [&]() __attribute__((always_inline)) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        y[k] = row_of(dy + k * a.lddy);
-        x[k] = *reinterpret_cast<const uint32_t*>(qp + k * static_cast<int64_t>(ldq));
-        code[k] = ep[k * static_cast<int64_t>(a.nb)];
-      }
-    } else {
-      const int32_t last = static_cast<int32_t>(left) - 1 - kg * 8;  // from this thread's first row
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int64_t at = k < last ? k : last;
-        y[k] = row_of(dy + at * a.lddy);
-        x[k] = *reinterpret_cast<const uint32_t*>(qp + at * ldq);
-        code[k] = ep[at * a.nb];
-        if (k > last)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) y[k].e[j] = static_cast<T>(0.f);
-      }
+    for (int k = 0; k < 8; ++k) {
+      y[k] = row_of(dy + k * a.lddy);
+      x[k] = *reinterpret_cast<const uint32_t*>(qp + k * static_cast<int64_t>(ldq));
     }
+    codes = *ep;
     dy += kDepth * a.lddy;
     qp += kDepth * static_cast<int64_t>(ldq);
     ep += kDepth * static_cast<int64_t>(a.nb);
   };
+  // The same where the share ends after `left` < kDepth of them: behind its last row x repeats it and dy is 0.
+  auto fetch_last = [&](int64_t left) __attribute__((always_inline)) {
+    const int32_t last = static_cast<int32_t>(left) - 1 - kg * 8;  // from this thread's first row
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int64_t at = k < last ? k : last;
+      y[k] = row_of(dy + at * a.lddy);
+      x[k] = *reinterpret_cast<const uint32_t*>(qp + at * ldq);
+      if (k > last)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[k].e[j] = static_cast<T>(0.f);
+    }
+    const int64_t beyond = kg * 8 + cg / kTileBlocks - (left - 1);  // rows from the share's last to the one whose byte this is
+    codes = *(beyond > 0 ? ep - beyond * a.nb : ep);
+  };
+  auto scales = [&](float (&s)[8]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      s[k] = scale_of(static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(code_lane + k * kTileBlocks * 4, static_cast<int>(codes))));
+  };
+  auto fetch = [&](int64_t left) __attribute__((always_inline)) {
+    if (left >= kDepth) fetch_all();
+    else fetch_last(left);
+  };
   // Column j of the thread's quads into a buffer.
-  auto store = [&](char* buffer, int j) {
+  auto store = [&](char* buffer, int j, const float (&scale)[8]) __attribute__((always_inline)) {
     char* at = buffer + ((B / 4) * j + cg) * kLdsPitch + kg * 16;
     if constexpr (P == 1) {
       u32x4 w;
@@ -262,13 +267,16 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
       for (int k = 0; k < 4; ++k) {
         const uint32_t lo = reinterpret_cast<const uint32_t*>(y[2 * k].e)[j >> 1];
         const uint32_t hi = reinterpret_cast<const uint32_t*>(y[2 * k + 1].e)[j >> 1];
-        w[k] = __builtin_amdgcn_perm(hi, lo, (j & 1) != 0 ? 0x07060302 : 0x05040100);
+        const uint32_t pair = __builtin_amdgcn_perm(hi, lo, (j & 1) != 0 ? 0x07060302 : 0x05040100);
+        bias[j] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), bf16x2{1, 1}, bias[j], false);
+        w[k] = pair;
       }
       *reinterpret_cast<u32x4*>(at) = w;
     } else {
       float f[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) f[k] = static_cast<float>(y[k].e[j]);
+      bias[j] += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
 #pragma unroll
       for (int p = 0; p < P; ++p) {
         u32x4 w;
@@ -286,7 +294,7 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
       float f[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float s = scale_of(code[2 * k + h]);
+        const float s = scale[2 * k + h];
         const uint32_t u = ((x[2 * k + h] ^ 0x80808080u) >> (8 * j)) & 255u;  // q + 128
         f[h] = __builtin_fmaf(static_cast<float>(u), s, -128.f * s);          // exact; NaN where s is inf
       }
@@ -294,7 +302,7 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
     }
     *reinterpret_cast<u32x4*>(at + P * kPlane) = w;
   };
-  auto multiply = [&](const char* buffer, int s) {
+  auto multiply = [&](const char* buffer, int s) __attribute__((always_inline)) {
     const int off = (lane & 31) * kLdsPitch + s * 32 + (lane >> 5) * 16;
     bf16x8 b[FN];
 #pragma unroll
@@ -311,49 +319,64 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
   };
 
   fetch(r1 - r0);
+  int64_t left = r1 - r0;  // rows not multiplied yet
   if constexpr (kStages<T> == 2) {
-    if (a.bias != nullptr) add_bias();
+    float scale[8];
+    scales(scale);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) store(lds, j);
-    if (r0 + kDepth < r1) fetch(r1 - r0 - kDepth);
+    for (int j = 0; j < 4; ++j) store(lds, j, scale);
+    if (left > kDepth) fetch(left - kDepth);
     __syncthreads();
-    int turn = 0;
-    int64_t r = r0;
-    do {
-      const char* now = lds + turn * kBuffer;
-      turn ^= 1;
+    char* now = lds;
+    char* then = lds + kBuffer;
+    auto turn = [&]() {
+      char* t = now;
+      now = then;
+      then = t;
+    };
+    // While two whole steps follow: no branch between the products of a step, the next one's operands on their way
+    // into the other buffer and the loads of the one behind it.
+    for (; left >= 3 * kDepth; left -= kDepth) {
       multiply(now, 0);
       multiply(now, 1);
-      if (r + kDepth < r1) {
-        if (a.bias != nullptr) add_bias();
-        store(lds + turn * kBuffer, 0);
-        store(lds + turn * kBuffer, 1);
-      }
+      scales(scale);
+      store(then, 0, scale);
+      store(then, 1, scale);
       multiply(now, 2);
-      if (r + kDepth < r1) {
-        store(lds + turn * kBuffer, 2);
-        store(lds + turn * kBuffer, 3);
-        if (r + 2 * kDepth < r1) fetch(r1 - r - 2 * kDepth);
-      }
+      store(then, 2, scale);
+      store(then, 3, scale);
+      fetch_all();
       multiply(now, 3);
       __syncthreads();
-      r += kDepth;
-    } while (r < r1);
+      turn();
+    }
+    for (; left > 0; left -= kDepth) {  // the last two or three
+#pragma unroll
+      for (int s = 0; s < kDepth / 16; ++s) multiply(now, s);
+      if (left > kDepth) {
+        scales(scale);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) store(then, j, scale);
+      }
+      if (left > 2 * kDepth) fetch(left - 2 * kDepth);
+      __syncthreads();
+      turn();
+    }
   } else {
-    int64_t r = r0;
     do {
-      if (a.bias != nullptr) add_bias();
+      float scale[8];
+      scales(scale);
       __syncthreads();  // the last step's operands are read
 #pragma unroll
-      for (int j = 0; j < 4; ++j) store(lds, j);
-      if (r + kDepth < r1) fetch(r1 - r - kDepth);
+      for (int j = 0; j < 4; ++j) store(lds, j, scale);
+      if (left > kDepth) fetch(left - kDepth);
       __syncthreads();
 #pragma unroll
       for (int s = 0; s < kDepth / 16; ++s) multiply(lds, s);
-      r += kDepth;
-    } while (r < r1);
+      left -= kDepth;
+    } while (left > 0);
   }
-  if (a.bias != nullptr) {  // the 8 row groups' sums, in their order
+  if (a.bias != nullptr && i0 == 0) {  // the 8 row groups' sums, in their order
     float* sums = reinterpret_cast<float*>(lds);
     __syncthreads();
 #pragma unroll
@@ -364,7 +387,7 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
       float v = 0.f;
 #pragma unroll
       for (int k = 0; k < 8; ++k) v += sums[k * B + tid];
-      if (!NARROW || row < a.o) a.bias[(static_cast<int64_t>(split) * a.tiles_d + i0 / B) * a.o + row] = v;
+      if (!NARROW || row < a.o) a.bias[static_cast<int64_t>(split) * a.o + row] = v;
     }
   }
   float* out = a.out + static_cast<int64_t>(split) * a.o * a.d;
@@ -416,7 +439,7 @@ struct Splits {
   int32_t w;     // row shares
   int64_t per;   // rows of a share
   int64_t floats(int32_t o, int32_t d) const {  // workspace: the shares' tiles, and their column sums
-    return static_cast<int64_t>(w) * o * d + static_cast<int64_t>(w) * tiles_d * o;
+    return static_cast<int64_t>(w) * o * (static_cast<int64_t>(d) + 1);
   }
 };
 
@@ -502,7 +525,7 @@ extern "C" int kgat_act8_wgrad(int32_t dtype, const void* dy, int64_t lddy, cons
     const Splits s = wgrad_splits<T>(n, o, d);
     const int64_t size = static_cast<int64_t>(o) * d;
     float* part_b = workspace + s.w * size;
-    Join j{{workspace, part_b}, {dW, db}, {size, o}, {s.w, s.w * s.tiles_d}, 0};
+    Join j{{workspace, part_b}, {dW, db}, {size, o}, {s.w, s.w}, 0};
     if (n == 0) {  // sums of nothing
       j.parts[0] = j.parts[1] = 0;
     } else {
