@@ -9,6 +9,8 @@
 // The power-of-two scale costs up to one bit against max / 127, and buys exactness: q 2^e has 7 bits of mantissa,
 // so it IS a bf16 number, and the weight gradient dW = dy^T x runs on the bf16 matrix instructions without any
 // further rounding of x.  dy goes in as it is (bf16) or as the exact sum of two (fp16) or three (float) bf16 terms.
+#include <type_traits>
+
 #include "dense.hpp"
 
 namespace kgat {
@@ -144,18 +146,44 @@ __device__ __forceinline__ uint32_t take_term(float& f) {
 }
 
 template <typename T>
-struct Quad {  // 4 columns of one row
-  T e[4];
+struct Quad {  // 4 columns of one row, as they lie in memory
+  uint32_t w[sizeof(T)];
+  __device__ __forceinline__ float at(int j) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[j]);
+    else return static_cast<float>(__builtin_bit_cast(T, static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)))));
+  }
 };
 
-template <typename T>
-__device__ __forceinline__ Quad<T> load_quad(const T* p) {
+typedef u32x2 u32x2_any __attribute__((aligned(2)));
+#define KGAT_GLOBAL __attribute__((address_space(1)))  // of pointers that came through integers
+template <typename P>
+__device__ __forceinline__ const KGAT_GLOBAL P* global_at(uint64_t base, uint64_t offset) {
+  return reinterpret_cast<const KGAT_GLOBAL P*>(reinterpret_cast<const KGAT_GLOBAL char*>(base) + offset);
+}
+
+// NARROW: a row of `width` < 4 columns.
+template <typename T, bool NARROW>
+__device__ __forceinline__ Quad<T> load_quad(uint64_t base, uint64_t offset, int32_t width) {
   Quad<T> v;
-  if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<u32x4*>(v.e) = *reinterpret_cast<const u32x4_any*>(p);
+  if constexpr (NARROW) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = j < width ? j : width - 1;
+      if constexpr (sizeof(T) == 4) {
+        v.w[j] = global_at<uint32_t>(base, offset)[c];
+      } else {
+        const uint32_t e = global_at<uint16_t>(base, offset)[c];
+        v.w[j >> 1] = (j & 1) != 0 ? v.w[j >> 1] | e << 16 : e;
+      }
+    }
+  } else if constexpr (sizeof(T) == 4) {
+    const u32x4 q = *global_at<u32x4_any>(base, offset);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v.w[j] = q[j];
   } else {
-    typedef u32x2 u32x2_any __attribute__((aligned(2)));
-    *reinterpret_cast<u32x2*>(v.e) = *reinterpret_cast<const u32x2_any*>(p);
+    const u32x2 q = *global_at<u32x2_any>(base, offset);
+    v.w[0] = q[0];
+    v.w[1] = q[1];
   }
   return v;
 }
@@ -189,9 +217,15 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
   // A quad that would pass the last column starts earlier: its columns are computed twice, and written twice with the
   // same value.
   auto first_of = [](int32_t c, int32_t width) { return c < width - 4 ? c : width > 4 ? width - 4 : 0; };
-  const T* dy = static_cast<const T*>(a.dy) + (r0 + kg * 8) * a.lddy + first_of(o0 + cg * 4, a.o);
-  const int32_t ic = first_of(i0 + cg * 4, ldq);
-  const int8_t* qp = a.q + (r0 + kg * 8) * ldq + ic;
+  // A wave's rows start at a uniform address (scalar registers, a scalar addition a row); a thread adds its 32-bit
+  // column offset, and where a wave holds several row groups their rows.
+  const int kg0 = __builtin_amdgcn_readfirstlane(kg);
+  const int64_t pitch_y = a.lddy * static_cast<int64_t>(sizeof(T)), pitch_q = ldq;
+  const int32_t oc = first_of(o0 + cg * 4, a.o) * static_cast<int32_t>(sizeof(T)), ic = first_of(i0 + cg * 4, ldq);
+  uint64_t dy = reinterpret_cast<uint64_t>(a.dy) + (r0 + kg0 * 8) * pitch_y;
+  uint64_t qp = reinterpret_cast<uint64_t>(a.q) + (r0 + kg0 * 8) * pitch_q;
+  typedef std::conditional_t<B == 256, uint32_t, int64_t> offset_t;
+  const offset_t off_y = B == 256 ? oc : oc + (kg - kg0) * 8 * pitch_y, off_q = B == 256 ? ic : ic + (kg - kg0) * 8 * pitch_q;
   // The scales of 8 rows and the tile's blocks are one byte for each of the B / 4 threads of a row group: a thread loads
   // one, and takes its 8 rows' by lane exchange (a load for each was a sixth of the kernel's time).
   constexpr int kTileBlocks = B / kBlock;
@@ -212,26 +246,19 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
   uint32_t x[8], codes;
   // The column sums of dy: every block forms them, one instruction for two terms, and the first of its strip writes them.
   float bias[4] = {0.f, 0.f, 0.f, 0.f};
-  auto row_of = [&](const T* p) {
-    if constexpr (NARROW) {
-      Quad<T> v;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v.e[j] = p[j < a.o ? j : a.o - 1];
-      return v;
-    } else {
-      return load_quad(p);
-    }
-  };
   // The next kDepth rows' operands.
   auto fetch_all = [&]() __attribute__((always_inline)) {
+    // The bases are scalars, and new ones every step: left to itself the compiler steps 16 vector addresses instead.
+    uint64_t y0 = dy, q0 = qp;
+    asm("" : "+s"(y0), "+s"(q0));
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      y[k] = row_of(dy + k * a.lddy);
-      x[k] = *reinterpret_cast<const uint32_t*>(qp + k * static_cast<int64_t>(ldq));
+      y[k] = load_quad<T, NARROW>(y0 + k * pitch_y, off_y, a.o);
+      x[k] = *global_at<uint32_t>(q0 + k * pitch_q, off_q);
     }
     codes = *ep;
-    dy += kDepth * a.lddy;
-    qp += kDepth * static_cast<int64_t>(ldq);
+    dy += kDepth * pitch_y;
+    qp += kDepth * pitch_q;
     ep += kDepth * static_cast<int64_t>(a.nb);
   };
   // The same where the share ends after `left` < kDepth of them: behind its last row x repeats it and dy is 0.
@@ -240,11 +267,11 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const int64_t at = k < last ? k : last;
-      y[k] = row_of(dy + at * a.lddy);
-      x[k] = *reinterpret_cast<const uint32_t*>(qp + at * ldq);
+      y[k] = load_quad<T, NARROW>(dy, off_y + at * pitch_y, a.o);
+      x[k] = *global_at<uint32_t>(qp, off_q + at * pitch_q);
       if (k > last)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[k].e[j] = static_cast<T>(0.f);
+        for (int j = 0; j < static_cast<int>(sizeof(T)); ++j) y[k].w[j] = 0;
     }
     const int64_t beyond = kg * 8 + cg / kTileBlocks - (left - 1);  // rows from the share's last to the one whose byte this is
     codes = *(beyond > 0 ? ep - beyond * a.nb : ep);
@@ -265,8 +292,7 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
       u32x4 w;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const uint32_t lo = reinterpret_cast<const uint32_t*>(y[2 * k].e)[j >> 1];
-        const uint32_t hi = reinterpret_cast<const uint32_t*>(y[2 * k + 1].e)[j >> 1];
+        const uint32_t lo = y[2 * k].w[j >> 1], hi = y[2 * k + 1].w[j >> 1];
         const uint32_t pair = __builtin_amdgcn_perm(hi, lo, (j & 1) != 0 ? 0x07060302 : 0x05040100);
         bias[j] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), bf16x2{1, 1}, bias[j], false);
         w[k] = pair;
@@ -275,7 +301,7 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
     } else {
       float f[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = static_cast<float>(y[k].e[j]);
+      for (int k = 0; k < 8; ++k) f[k] = y[k].at(j);
       bias[j] += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
 #pragma unroll
       for (int p = 0; p < P; ++p) {
