@@ -276,14 +276,15 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
     const int64_t beyond = kg * 8 + cg / kTileBlocks - (left - 1);  // rows from the share's last to the one whose byte this is
     codes = *(beyond > 0 ? ep - beyond * a.nb : ep);
   };
-  auto scales = [&](float (&s)[8]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      s[k] = scale_of(static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(code_lane + k * kTileBlocks * 4, static_cast<int>(codes))));
-  };
   auto fetch = [&](int64_t left) __attribute__((always_inline)) {
     if (left >= kDepth) fetch_all();
     else fetch_last(left);
+  };
+  auto scales = [&](float (&s)[8]) __attribute__((always_inline)) {
+    const int mine = static_cast<int>(codes);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      s[k] = scale_of(static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(code_lane + k * kTileBlocks * 4, mine)));
   };
   // Column j of the thread's quads into a buffer.
   auto store = [&](char* buffer, int j, const float (&scale)[8]) __attribute__((always_inline)) {
@@ -319,35 +320,41 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
     for (int k = 0; k < 4; ++k) {
       float f[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float s = scale[2 * k + h];
-        const uint32_t u = ((x[2 * k + h] ^ 0x80808080u) >> (8 * j)) & 255u;  // q + 128
-        f[h] = __builtin_fmaf(static_cast<float>(u), s, -128.f * s);          // exact; NaN where s is inf
-      }
+      for (int h = 0; h < 2; ++h)  // exact; NaN where the scale is inf
+        f[h] = static_cast<float>(static_cast<int8_t>(x[2 * k + h] >> (8 * j))) * scale[2 * k + h];
       w[k] = high_halves(__float_as_uint(f[0]), __float_as_uint(f[1]));
     }
     *reinterpret_cast<u32x4*>(at + P * kPlane) = w;
   };
-  auto multiply = [&](const char* buffer, int s) __attribute__((always_inline)) {
+  // The operands of 16 rows: a wave's columns of x and of each of dy's terms.
+  struct Operands {
+    bf16x8 b[FN], a[P][FM];
+  };
+  auto read = [&](Operands& v, const char* buffer, int s) __attribute__((always_inline)) {
     const int off = (lane & 31) * kLdsPitch + s * 32 + (lane >> 5) * 16;
-    bf16x8 b[FN];
 #pragma unroll
     for (int n = 0; n < FN; ++n)
-      b[n] = *reinterpret_cast<const bf16x8*>(buffer + P * kPlane + (wn + n * 32) * kLdsPitch + off);
+      v.b[n] = *reinterpret_cast<const bf16x8*>(buffer + P * kPlane + (wn + n * 32) * kLdsPitch + off);
 #pragma unroll
     for (int p = 0; p < P; ++p)
 #pragma unroll
-      for (int m = 0; m < FM; ++m) {
-        const bf16x8 v = *reinterpret_cast<const bf16x8*>(buffer + p * kPlane + (wm + m * 32) * kLdsPitch + off);
+      for (int m = 0; m < FM; ++m)
+        v.a[p][m] = *reinterpret_cast<const bf16x8*>(buffer + p * kPlane + (wm + m * 32) * kLdsPitch + off);
+  };
+  auto multiply = [&](const Operands& v) __attribute__((always_inline)) {
 #pragma unroll
-        for (int n = 0; n < FN; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, b[n], acc[m][n], 0, 0, 0);
-      }
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int m = 0; m < FM; ++m)
+#pragma unroll
+        for (int n = 0; n < FN; ++n)
+          acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v.a[p][m], v.b[n], acc[m][n], 0, 0, 0);
   };
 
-  fetch(r1 - r0);
+  float scale[8];
   int64_t left = r1 - r0;  // rows not multiplied yet
+  fetch(left);
   if constexpr (kStages<T> == 2) {
-    float scale[8];
     scales(scale);
 #pragma unroll
     for (int j = 0; j < 4; ++j) store(lds, j, scale);
@@ -360,25 +367,29 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
       now = then;
       then = t;
     };
-    // While two whole steps follow: no branch between the products of a step, the next one's operands on their way
-    // into the other buffer and the loads of the one behind it.
+    Operands v[2];
+    // While two whole steps follow: no branch between the products of a step, the next one's operands on their way into
+    // the other buffer and the loads of the one behind it.  Each phase reads the next 16 rows' operands, decodes a
+    // column and multiplies (groups laid down with sched_group_barrier were 3 % slower than the compiler's own mix).
     for (; left >= 3 * kDepth; left -= kDepth) {
-      multiply(now, 0);
-      multiply(now, 1);
+      read(v[0], now, 0);
       scales(scale);
-      store(then, 0, scale);
-      store(then, 1, scale);
-      multiply(now, 2);
-      store(then, 2, scale);
-      store(then, 3, scale);
-      fetch_all();
-      multiply(now, 3);
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        if (s < 3) read(v[(s + 1) & 1], now, s + 1);
+        store(then, s, scale);
+        if (s == 3) fetch_all();
+        multiply(v[s & 1]);
+      }
       __syncthreads();
       turn();
     }
-    for (; left > 0; left -= kDepth) {  // the last two or three
+    for (; left > 0; left -= kDepth) {  // the last two
 #pragma unroll
-      for (int s = 0; s < kDepth / 16; ++s) multiply(now, s);
+      for (int s = 0; s < 4; ++s) {
+        read(v[0], now, s);
+        multiply(v[0]);
+      }
       if (left > kDepth) {
         scales(scale);
 #pragma unroll
@@ -389,8 +400,8 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
       turn();
     }
   } else {
+    Operands v;
     do {
-      float scale[8];
       scales(scale);
       __syncthreads();  // the last step's operands are read
 #pragma unroll
@@ -398,7 +409,10 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
       if (left > kDepth) fetch(left - kDepth);
       __syncthreads();
 #pragma unroll
-      for (int s = 0; s < kDepth / 16; ++s) multiply(lds, s);
+      for (int s = 0; s < 4; ++s) {
+        read(v, lds, s);
+        multiply(v);
+      }
       left -= kDepth;
     } while (left > 0);
   }
