@@ -485,11 +485,15 @@ struct Splits {
 
 template <typename T>
 Splits wgrad_splits(int64_t n, int32_t o, int32_t d) {
+  // The largest tile reads least and has the fewest blocks: 128 and 256 from where they are not mostly empty, 256 (bf16
+  // only: two buffers of it are LDS's 147 KB) from 32 of them on (o = d = 4096: 504 us against 822 of 128; 2048 x 512, 16
+  // of them: 63 against 50; 1024 x 1024, also 16, equal).
   const int64_t least = o < d ? o : d;
-  const int32_t tile = kPlanes<T> == 1 && least > 128 ? 256 : least > 64 ? 128 : 64;
+  const int64_t large = static_cast<int64_t>((o + 255) / 256) * ((d + 255) / 256);
+  const int32_t tile = kPlanes<T> == 1 && least > 128 && large >= 32 ? 256 : least > 64 ? 128 : 64;
   const int32_t tiles_o = (o + tile - 1) / tile, tiles_d = (d + tile - 1) / tile;
   const int64_t fill = tile == 256 ? kCUs : tile == 128 ? 2 * kCUs : 4 * kCUs;  // blocks the chip holds
-  int64_t w = fill / (static_cast<int64_t>(tiles_o) * tiles_d), most = (n + 511) / 512;
+  int64_t w = fill / (static_cast<int64_t>(tiles_o) * tiles_d), most = (n + 127) / 128;  // two steps a share at least
   if (w > most) w = most;
   if (w < 1) w = 1;
   const int64_t per = n < 1 ? kDepth : ((n + w - 1) / w + kDepth - 1) / kDepth * kDepth;

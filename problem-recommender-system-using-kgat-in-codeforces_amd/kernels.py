@@ -1418,15 +1418,20 @@ ROW_DTYPES = {torch.float32: _lib.KGAT_F32, torch.bfloat16: _lib.KGAT_BF16, torc
 
 
 def _req_rows(t: torch.Tensor, name: str) -> int:
-    """The KGAT_* code of a 2-D row tensor's type (checked as _req does)."""
-    if isinstance(t, torch.Tensor) and t.dtype not in ROW_DTYPES:
-        raise ValueError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
-    _req(t, name, dtype=getattr(t, "dtype", None), dim=2)
-    return ROW_DTYPES[t.dtype]
+    """The KGAT_* code of a 2-D row tensor's type (checked as _req does; the checks that pass are a microsecond)."""
+    code = ROW_DTYPES.get(getattr(t, "dtype", None))
+    if code is None or not t.is_cuda or t.dim() != 2 or t.stride(1) != 1:
+        if isinstance(t, torch.Tensor) and code is None:
+            raise ValueError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
+        _req(t, name, dtype=getattr(t, "dtype", None), dim=2)  # a size-1 last dimension may keep any stride
+    return code
 
 
 def _req_like(t: torch.Tensor, name: str, like: torch.Tensor, shape, dtype) -> None:
-    """A contiguous tensor of this shape and type on ``like``'s device."""
+    """A contiguous tensor of this shape (a tuple) and type on ``like``'s device."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.is_contiguous() and \
+            t.is_cuda and t.get_device() == like.get_device():
+        return
     _req(t, name, dtype=dtype, dim=len(shape))
     if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
         raise ValueError(f"{name}: contiguous {list(shape)} expected, got {list(t.shape)}")
@@ -1434,13 +1439,21 @@ def _req_like(t: torch.Tensor, name: str, like: torch.Tensor, shape, dtype) -> N
         raise ValueError(f"{name}: on {t.device}, the rows are on {like.device}")
 
 
+_ROW_FN: dict = {}  # name -> the bound library function
+
+
 def _row_call(like: torch.Tensor, name: str, *args) -> None:
     """One library call on the current stream of ``like``'s device, which need not be the current device."""
-    if like.device.index == torch.cuda.current_device():
-        _lib.call(name, *args, stream_ptr(like.device))
+    fn = _ROW_FN.get(name)
+    if fn is None:
+        fn = _ROW_FN[name] = getattr(_lib.lib(), name)
+    if like.get_device() == torch.cuda.current_device():
+        status = fn(*args, stream_ptr(like.device))
     else:
         with torch.cuda.device(like.device):
-            _lib.call(name, *args, stream_ptr(like.device))
+            status = fn(*args, stream_ptr(like.device))
+    if status != 0:
+        _lib.check(status, name)
 
 
 def _ptr(t: torch.Tensor | None):
@@ -1450,9 +1463,10 @@ def _ptr(t: torch.Tensor | None):
 def _norm_weight(t: torch.Tensor | None, name: str, x: torch.Tensor) -> None:
     if t is None:
         return
-    if isinstance(t, torch.Tensor) and t.dtype not in (torch.float32, x.dtype):
-        raise ValueError(f"{name}: expected torch.float32 or the rows' {x.dtype}, got {t.dtype}")
-    _req_like(t, name, x, (x.shape[1],), getattr(t, "dtype", None))
+    dtype = getattr(t, "dtype", None)
+    if dtype is not torch.float32 and dtype is not x.dtype:
+        raise ValueError(f"{name}: expected torch.float32 or the rows' {x.dtype}, got {dtype}")
+    _req_like(t, name, x, (x.shape[1],), dtype)
 
 
 def layer_norm_fwd(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
@@ -1470,10 +1484,11 @@ def layer_norm_fwd(x: torch.Tensor, weight: torch.Tensor | None = None, bias: to
     _norm_weight(bias, "bias", x)
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError("weight and bias must have one type")
-    w_code = ROW_DTYPES[next((t.dtype for t in (weight, bias) if t is not None), torch.float32)]
-    y = torch.empty(n, d, dtype=x.dtype, device=x.device)
-    mr = torch.empty(2, n, dtype=torch.float32, device=x.device) if stats else None
-    mean, rstd = mr.unbind(0) if stats else (None, None)
+    w_code = ROW_DTYPES[weight.dtype if weight is not None else torch.float32 if bias is None else bias.dtype]
+    y = x.new_empty((n, d))
+    mean = rstd = None
+    if stats:
+        mean, rstd = x.new_empty(n, dtype=torch.float32), x.new_empty(n, dtype=torch.float32)
     if n:
         _row_call(x, "kgat_layer_norm_fwd", code, x.data_ptr(), x.stride(0), w_code, _ptr(weight), _ptr(bias),
                   y.data_ptr(), d, _ptr(mean), _ptr(rstd), n, d, float(eps))
@@ -1488,7 +1503,7 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: 
     code = _req_rows(x, "x")
     _req_rows(dy, "dy")
     n, d = x.shape
-    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
+    if dy.shape != x.shape or dy.dtype is not x.dtype or dy.get_device() != x.get_device():
         raise ValueError("dy must have x's shape, type and device")
     if not 1 <= d <= _lib.KGAT_NORM_MAX_D:
         raise ValueError(f"x: width must be in [1, {_lib.KGAT_NORM_MAX_D}], got {d}")
@@ -1496,15 +1511,14 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: 
     _req_like(rstd, "rstd", x, (n,), torch.float32)
     _norm_weight(weight, "weight", x)
     w_dtype = torch.float32 if weight is None else weight.dtype
-    dx = torch.empty(n, d, dtype=x.dtype, device=x.device) if need_dx else None
-    dw = torch.empty(d, dtype=w_dtype, device=x.device) if need_dweight else None
-    db = torch.empty(d, dtype=w_dtype, device=x.device) if need_dbias else None
+    dx = x.new_empty((n, d)) if need_dx else None
+    dw = x.new_empty(d, dtype=w_dtype) if need_dweight else None
+    db = x.new_empty(d, dtype=w_dtype) if need_dbias else None
     ws = None
     if need_dweight or need_dbias:
         if n == 0:
             return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
-        ws = torch.empty(max(1, int(_lib.lib().kgat_layer_norm_bwd_workspace(code, n, d))), dtype=torch.float32,
-                         device=x.device)
+        ws = x.new_empty(_lib.lib().kgat_layer_norm_bwd_workspace(code, n, d), dtype=torch.float32)
     if n and (need_dx or ws is not None):
         _row_call(x, "kgat_layer_norm_bwd", code, dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0),
                   mean.data_ptr(), rstd.data_ptr(), ROW_DTYPES[w_dtype], _ptr(weight), _ptr(dx), d, _ptr(dw), _ptr(db),
@@ -1549,8 +1563,8 @@ def act8_pack(x: torch.Tensor) -> Act8:
     if not 1 <= d <= _lib.KGAT_ACT8_MAX_D:
         raise ValueError(f"x: width must be in [1, {_lib.KGAT_ACT8_MAX_D}], got {d}")
     nb = (d + _lib.KGAT_ACT8_BLOCK - 1) // _lib.KGAT_ACT8_BLOCK
-    q = torch.empty(n, nb * _lib.KGAT_ACT8_BLOCK, dtype=torch.int8, device=x.device)
-    e = torch.empty(n, nb, dtype=torch.uint8, device=x.device)
+    q = x.new_empty((n, nb * _lib.KGAT_ACT8_BLOCK), dtype=torch.int8)
+    e = x.new_empty((n, nb), dtype=torch.uint8)
     if n:
         _row_call(x, "kgat_act8_pack", code, x.data_ptr(), x.stride(0), n, d, q.data_ptr(), e.data_ptr())
     return Act8(q, e, (n, d), x.dtype)
@@ -1583,11 +1597,11 @@ def act8_wgrad(dy: torch.Tensor, a: Act8, bias: bool = True):
         raise ValueError(f"dy: {n} rows on {a.device} expected, got {list(dy.shape)} on {dy.device}")
     if not 1 <= o <= _lib.KGAT_ACT8_MAX_D:
         raise ValueError(f"dy: width must be in [1, {_lib.KGAT_ACT8_MAX_D}], got {o}")
-    dW = torch.empty(o, d, dtype=torch.float32, device=dy.device)
-    db = torch.empty(o, dtype=torch.float32, device=dy.device) if bias else None
+    dW = dy.new_empty((o, d), dtype=torch.float32)
+    db = dy.new_empty(o, dtype=torch.float32) if bias else None
     if n == 0:
         return dW.zero_(), None if db is None else db.zero_()
-    ws = torch.empty(max(1, int(_lib.lib().kgat_act8_wgrad_workspace(code, n, o, d))), dtype=torch.float32, device=dy.device)
+    ws = dy.new_empty(_lib.lib().kgat_act8_wgrad_workspace(code, n, o, d), dtype=torch.float32)
     _row_call(dy, "kgat_act8_wgrad", code, dy.data_ptr(), dy.stride(0), a.q.data_ptr(), a.e.data_ptr(), n, o, d,
               dW.data_ptr(), _ptr(db), ws.data_ptr(), ws.numel())
     return dW, db
@@ -1610,7 +1624,7 @@ def _req_scores(scores: torch.Tensor, items: torch.Tensor, scale: float) -> int:
     if not 1 <= c < 2 ** 31 or n >= 2 ** 31:
         raise ValueError(f"scores: 1 to 2^31 - 1 columns and fewer than 2^31 rows expected, got {list(scores.shape)}")
     _req(items, "items", dtype=torch.int64, dim=2)
-    if items.shape[0] != n or not items.is_contiguous() or items.device != scores.device:
+    if items.shape[0] != n or not items.is_contiguous() or items.get_device() != scores.get_device():
         raise ValueError(f"items: contiguous [{n}, t] on {scores.device} expected")
     if items.shape[1] > _lib.KGAT_LOGPROB_MAX_ITEMS:
         raise ValueError(f"items: at most {_lib.KGAT_LOGPROB_MAX_ITEMS} a row, got {items.shape[1]}")
@@ -1629,14 +1643,13 @@ def log_prob_fwd(scores: torch.Tensor, items: torch.Tensor, k: int = 0, scale: f
     (n, c), t = scores.shape, items.shape[1]
     if not 0 <= k <= min(c, _lib.KGAT_LOGPROB_MAX_K):
         raise ValueError(f"k must be in [0, min(columns, {_lib.KGAT_LOGPROB_MAX_K})], got {k}")
-    dev = scores.device
-    logp = torch.empty(n, t, dtype=torch.float32, device=dev)
-    stats = torch.empty(4, n, dtype=torch.float32, device=dev)
-    top = torch.empty(n, k, dtype=torch.int64, device=dev) if k else None
-    top_logp = torch.empty(n, k, dtype=torch.float32, device=dev) if k else None
+    logp = scores.new_empty((n, t), dtype=torch.float32)
+    stats = scores.new_empty((4, n), dtype=torch.float32)
+    top = scores.new_empty((n, k), dtype=torch.int64) if k else None
+    top_logp = scores.new_empty((n, k), dtype=torch.float32) if k else None
     if n:
-        need = int(_lib.lib().kgat_log_prob_workspace(n, c, k))
-        ws = torch.empty(need, dtype=torch.float32, device=dev) if need else None
+        need = _lib.lib().kgat_log_prob_workspace(n, c, k)
+        ws = scores.new_empty(need, dtype=torch.float32) if need else None
         _row_call(scores, "kgat_log_prob_fwd", code, scores.data_ptr(), scores.stride(0), n, c, float(scale),
                   _ptr(items), t, k, _ptr(logp), stats.data_ptr(), _ptr(top), _ptr(top_logp), _ptr(ws), need)
     return LogProbs(logp, stats[2], stats[3], top, top_logp, stats)
@@ -1654,7 +1667,7 @@ def log_prob_bwd(scores: torch.Tensor, items: torch.Tensor, stats: torch.Tensor,
     if dentropy is not None:
         _req_like(dentropy, "dentropy", scores, (n,), torch.float32)
     if out is None:
-        out = torch.empty(n, c, dtype=scores.dtype, device=scores.device)
+        out = scores.new_empty((n, c))
     else:
         _req_rows(out, "out")
         if out.shape != scores.shape or out.dtype != scores.dtype or out.device != scores.device or \
