@@ -9,6 +9,8 @@ Mirrors the reference's ranking code path for path:
   ONCE per evaluation (the reference re-propagates per 256-user batch; the
   scores are identical because PREDICT does not change the model).
 - ``recommend_topk``: the masked ``torch.topk(k=20)`` of main.py:576-605.
+- ``log_likelihood``: the held-out items' log probabilities under the softmax of the same
+  masked scores (not in the reference, which ranks only).
 
 Arithmetic: kgat_score_f32 (fused gather + MFMA GEMM), kgat_mask_rows_f32,
 kgat_topk_f32 (radix select + bitonic sort) and kgat_rank_metrics_f32 -- all
@@ -146,3 +148,51 @@ def recommend_topk(model, user_ids: Sequence[int], item_num: int, exclude: Mappi
         mask_rows(sc, ptr, idx)
         out.append(topk(sc, k).cpu())
     return torch.cat(out)
+
+
+@torch.no_grad()
+def log_likelihood(model, train_interaction_dict: Mapping[int, Sequence[int]],
+                   eval_interaction_dict: Mapping[int, Sequence[int]], item_num: int, scale: float = 1.0,
+                   batch_size: int = TEST_BATCH_SIZE, return_per_user: bool = False):
+    """How likely each user's held-out items are under softmax(scale * scores) over the catalogue, train items masked
+    as ``evaluate`` masks them (main.py:70-130 ranks the same scores).  Returns {"log_likelihood": mean over users of
+    the mean log probability of a user's held-out items, "perplexity": exp of minus that, "entropy": mean over users};
+    users without held-out items count in the entropy only.  With ``return_per_user`` also {"log_likelihood",
+    "entropy"} as ndarray[n_users] in the eval dict's order (nan where a user has no held-out item).
+
+    Arithmetic: kgat_score_f32, kgat_mask_rows_f32 and kgat_log_prob_fwd (one pass over a batch's scores)."""
+    model.eval()
+    tables = model.propagate()
+    dev = tables[0].device
+    users_all = list(eval_interaction_dict.keys())
+    catalogue = torch.arange(item_num, dtype=torch.long, device=dev)
+    likelihood, entropy, known = [], [], []
+    for i in range(0, len(users_all), batch_size):
+        users = users_all[i:i + batch_size]
+        sc = kernels.scores(tables, torch.as_tensor(np.asarray(users, np.int64)).to(dev), catalogue)
+        ptr, idx = _csr([train_interaction_dict[int(u)] for u in users], dev)
+        mask_rows(sc, ptr, idx)
+        held = [np.unique(np.asarray(list(eval_interaction_dict[u]), dtype=np.int64)) for u in users]
+        if any(h.size and (h[0] < 0 or h[-1] >= item_num) for h in held):
+            raise IndexError("held-out item id out of range")
+        width = max(1, max(h.size for h in held))
+        items = np.full((len(users), width), -1, np.int64)
+        for row, h in zip(items, held):
+            row[:h.size] = h
+        total = torch.zeros(len(users), dtype=torch.float64, device=dev)
+        for j in range(0, width, _lib.KGAT_LOGPROB_MAX_ITEMS):
+            part = torch.from_numpy(np.ascontiguousarray(items[:, j:j + _lib.KGAT_LOGPROB_MAX_ITEMS])).to(dev)
+            r = kernels.log_prob_fwd(sc, part, scale=scale)
+            total += r.logp.sum(1, dtype=torch.float64)  # padding adds 0
+        counts = np.array([h.size for h in held], np.float64)
+        known.append(counts > 0)
+        with np.errstate(invalid="ignore", divide="ignore"):
+            likelihood.append(total.cpu().numpy() / counts)  # 0 / 0: nan
+        entropy.append(r.entropy.double().cpu().numpy())
+    likelihood = np.concatenate(likelihood) if likelihood else np.zeros(0)
+    entropy = np.concatenate(entropy) if entropy else np.zeros(0)
+    held_out = likelihood[np.concatenate(known)] if known else likelihood
+    mean = float(held_out.mean()) if held_out.size else float("nan")
+    result = {"log_likelihood": mean, "perplexity": float(np.exp(-mean)),
+              "entropy": float(entropy.mean()) if entropy.size else float("nan")}
+    return (result, {"log_likelihood": likelihood, "entropy": entropy}) if return_per_user else result

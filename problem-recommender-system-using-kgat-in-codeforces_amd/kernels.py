@@ -1526,6 +1526,27 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: 
     return dx, dw, db
 
 
+def gemm_supported(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether kgat_gemm_f32 takes these float32 operands: rows of a multiple of 4, 16-byte aligned."""
+    return all(t.dtype is torch.float32 and t.stride(1) == 1 and t.shape[1] % 4 == 0 and t.stride(0) % 4 == 0 and
+               t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0 and t.numel() > 0 for t in (a, b))
+
+
+def gemm(a: torch.Tensor, b: torch.Tensor, trans_b: bool = False) -> torch.Tensor:
+    """a [n, k] times b [k, m], or b [m, k] transposed, in float32 (kgat_gemm_f32; see gemm_supported)."""
+    _req(a, "a", dim=2)
+    _req(b, "b", dim=2)
+    k, m = (b.shape[1], b.shape[0]) if trans_b else b.shape
+    if a.shape[1] != k or a.device != b.device:
+        raise ValueError(f"gemm: {list(a.shape)} by {list(b.shape)}")
+    if not gemm_supported(a, b):
+        raise ValueError("gemm: rows of a multiple of 4 elements, 16-byte aligned, expected")
+    c = torch.empty(a.shape[0], m, dtype=torch.float32, device=a.device)
+    _row_call(a, "kgat_gemm_f32", 0, int(trans_b), a.shape[0], m, k, a.data_ptr(), a.stride(0), 0, b.data_ptr(),
+              b.stride(0), 0, c.data_ptr(), m, 0, 1, 0)
+    return c
+
+
 class Act8:
     """Activations [n, d] kept in 8 bits (act8_pack): ``q`` int8 [n, 32 * ceil(d / 32)] and ``e`` uint8
     [n, ceil(d / 32)], the power-of-two scale of each 32 columns of a row (value = q * 2^(e - 127); e = 255: NaN).

@@ -920,6 +920,13 @@ def _frontier_forward(graph, users, pos, neg, X0, ws, drops, seeds, early, marks
     return tables, sides, states, (early if L >= 2 else (rows, None, fcount, tok))
 
 
+def _side(sides, l: int) -> torch.Tensor:
+    """Layer l's neighbour sums S_l for its backward, read back from their 8-bit checkpoint where the forward kept one
+    (KGAT.checkpoint_sides)."""
+    s = sides[l]
+    return kernels.act8_unpack(s) if isinstance(s, kernels.Act8) else s
+
+
 def _saved(tables, states, l) -> dict:
     """Layer l's forward output + saved state for the backward (none: it recomputes)."""
     return {} if states[l] is None else {"H": tables[l + 1], "state": states[l]}
@@ -952,7 +959,7 @@ class _CFLoss(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, users, pos, neg, cfg, X0, *ws):
-        graph, drops, seeds, reg, hook, _tu, frontier, marks = cfg
+        graph, drops, seeds, reg, hook, _tu, frontier, marks, pack_sides = cfg
         ctx.marks = marks
         ctx.early = _early_first_hop(graph, users, pos, neg, ws, len(drops), hook, marks)
         fw = _frontier_forward(graph, users, pos, neg, X0, ws, drops, seeds, ctx.early, marks) if frontier else None
@@ -965,7 +972,7 @@ class _CFLoss(torch.autograd.Function):
                 W1, b1, W2, b2 = ws[4 * l: 4 * l + 4]
                 st = kernels.make_state(x.shape[0], W1.shape[1], W1.shape[0], x.device)
                 s, x = kernels.propagate_layer(graph, x, W1, b1, W2, b2, drops[l], seeds[l], state=st)
-                sides.append(s)
+                sides.append(kernels.act8_pack(s) if pack_sides else s)
                 states.append(st)
                 tables.append(x)
         loss, coef = kernels.bpr_fwd(tables, users, pos, neg, reg)
@@ -982,7 +989,7 @@ class _CFLoss(torch.autograd.Function):
         ctx.fast_backward = None
         if ctx.tables is None:
             raise RuntimeError("Trying to backward through the graph a second time")
-        graph, drops, seeds, reg, hook, tu, _frontier, _marks = ctx.cfg
+        graph, drops, seeds, reg, hook, tu, _frontier, _marks, _pack = ctx.cfg
         tables, sides, states, ws = ctx.tables, ctx.sides, ctx.states, ctx.ws
         users, pos, neg = ctx.ids
         gout = gout.reshape(1).to(torch.float32).contiguous()
@@ -1030,7 +1037,7 @@ class _CFLoss(torch.autograd.Function):
         t0 = min(k for k, d in enumerate(dsts) if d is not None)
         kernels.bpr_bwd_multi(tables, t0, users, pos, neg, reg, ctx.coef, gout, dsts, rows, fcount)
         l = L - 1
-        dXdc, dSc, dW1, db1, dW2, db2 = kernels.biinter_bwd(tables[l], sides[l], dHc, *ws[4 * l: 4 * l + 4],
+        dXdc, dSc, dW1, db1, dW2, db2 = kernels.biinter_bwd(tables[l], _side(sides, l), dHc, *ws[4 * l: 4 * l + 4],
                                                             drops[l], seeds[l], rows=rows, **_saved(tables, states, l))
         bits = graph.hop_buffers()[6]
         rank = graph.hop_buffers()[9]  # rank words of the current hop set (frontier_hop / hop_compact)
@@ -1114,19 +1121,20 @@ class _CFLoss(torch.autograd.Function):
                         out_rows, out = cap, (packed[:, din:], packed[:, :din])
                     gfold = fold2 and l == nxt
                     dXdc, dSc, dW1, db1, dW2, db2 = kernels.biinter_bwd_hop(
-                        tables[l], sides[l], dX, W1, W2, drops[l], hrows, hcount, tables[l + 1], states[l], out_rows,
+                        tables[l], _side(sides, l), dX, W1, W2, drops[l], hrows, hcount, tables[l + 1], states[l],
+                        out_rows,
                         dh_compact=compact_dh, out=out, G=dsts[l] if gfold else None,
                         gidx=gidx if gfold else None, gmap=graph.node_map if gfold else None)
                 elif compact_dh:
                     # wide kinds after the first-hop product: dX holds the hop rows compactly
                     hr = hrows[:n_hop]
-                    dXdc, dSc, dW1, db1, dW2, db2 = kernels.biinter_bwd(tables[l], sides[l], dX[:n_hop], W1, b1, W2,
+                    dXdc, dSc, dW1, db1, dW2, db2 = kernels.biinter_bwd(tables[l], _side(sides, l), dX[:n_hop], W1, b1, W2,
                                                                         b2, drops[l], seeds[l], rows=hr,
                                                                         **_saved(tables, states, l))
                     hrows = hr
                 else:
                     # wide kinds: H, dH and the state read through the hop list (X / S gathered once)
-                    dXdc, dSc, dW1, db1, dW2, db2 = kernels.biinter_bwd(tables[l], sides[l], dX, W1, b1, W2, b2,
+                    dXdc, dSc, dW1, db1, dW2, db2 = kernels.biinter_bwd(tables[l], _side(sides, l), dX, W1, b1, W2, b2,
                                                                         drops[l], seeds[l], rows=hrows,
                                                                         dh_full=True, **_saved(tables, states, l))
                 if not (fold2 and l == nxt):
@@ -1151,7 +1159,7 @@ class _CFLoss(torch.autograd.Function):
                                              row_hit=hit if l > 0 else None, src_rank=rank)
                 wgrads[4 * l: 4 * l + 4] = [dW1, db1, dW2, db2]
                 continue
-            dXd, dS, dW1, db1, dW2, db2 = kernels.biinter_bwd(tables[l], sides[l], dX, W1, b1, W2, b2, drops[l],
+            dXd, dS, dW1, db1, dW2, db2 = kernels.biinter_bwd(tables[l], _side(sides, l), dX, W1, b1, W2, b2, drops[l],
                                                               seeds[l], **_saved(tables, states, l))
             kernels.bpr_bwd(tables, l, users, pos, neg, reg, ctx.coef, gout, dXd)
             if l == 0 and hook is not None and hook.replicated:
@@ -1280,6 +1288,10 @@ class KGAT(nn.Module):
         # Opt-in: TRAIN_CF's forward computes each layer on the rows the loss can reach only
         # (_frontier_forward) -- same loss, gradients and updates, bit for bit
         self.frontier_forward = False
+        # Opt-in: TRAIN_CF's full forward keeps each layer's neighbour sums S = A.X for the backward in 8 bits
+        # (kernels.act8_pack: 1.03 bytes an element instead of 4).  The loss is unchanged; the gradients are those of
+        # sums within 2^-7 of the largest of their 32 columns.  frontier_forward keeps few rows and ignores it
+        self.checkpoint_sides = False
         # Opt-in: a plain ``loss.backward()`` of a TRAIN_CF / captured TRAIN_KG loss runs the step's backward
         # without the autograd engine (_StepLoss).  Leave it off under wrappers that hook the leaves' gradient
         # accumulators from C++ (DistributedDataParallel): the direct call cannot see those hooks
@@ -1470,7 +1482,8 @@ class KGAT(nn.Module):
         if marks is None:
             ids = self._ids.check("TRAIN_CF ids", (user_ids, positive_item_ids, negative_item_ids), g.n_nodes,
                                   g.device)
-        cfg = (g, drops, seeds, float(self._regularization_params[0]), hook, self._table_update, frontier, marks)
+        cfg = (g, drops, seeds, float(self._regularization_params[0]), hook, self._table_update, frontier, marks,
+               bool(self.checkpoint_sides) and not frontier and torch.is_grad_enabled())
         loss = _CFLoss.apply(*ids, cfg, self._user_entity_embedding.weight, *self._cf_weights())
         if not self.direct_backward and loss.grad_fn is not None:
             loss.grad_fn.fast_backward = None  # the autograd engine (the default; _StepLoss)
