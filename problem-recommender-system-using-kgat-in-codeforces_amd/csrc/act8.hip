@@ -483,21 +483,46 @@ struct Splits {
   }
 };
 
+// Microseconds of a step of 64 rows with `occ` blocks on a CU, measured (n = 16384, o = d = 1024; 256: also 4096): a
+// step of bf16 dy takes 0.73 / 1.4 us with 1 / 4 blocks of 64, 1.25 / 1.7 with 1 / 2 of 128, 2.25 with one of 256; of
+// fp16 dy 2.3 with 4 (64) and 1.9 / 2.6 (128); of float dy 1.6 / 2.4 (64) and 2.45 / 3.4 (128).
+double step_us(int planes, int32_t tile, int64_t occ) {
+  const double n = static_cast<double>(occ);
+  if (tile == 256) return 2.25;
+  if (tile == 128) return planes == 1 ? 0.8 + 0.45 * n : planes == 2 ? 1.2 + 0.7 * n : 1.5 + 0.95 * n;
+  return planes == 1 ? 0.6 + 0.2 * n : planes == 2 ? 0.9 + 0.35 * n : 1.35 + 0.26 * n;
+}
+
+// The tile and the number of row shares with the least estimated time: the blocks' steps (4, 2 or 1 of them on a CU at
+// once), and the shares' tiles written and read again at 5 TB/s.  One rule for every size: at o = d = 4096 tiles of 256
+// take 504 us and of 128 822 us; at 2048 x 512 (n = 8192) 63 and 50; at o = d = 64 (n = 2048) one share takes 53 us, 16 of
+// them 18.
 template <typename T>
 Splits wgrad_splits(int64_t n, int32_t o, int32_t d) {
-  // The largest tile reads least and has the fewest blocks: 128 and 256 from where they are not mostly empty, 256 (bf16
-  // only: two buffers of it are LDS's 147 KB) from 32 of them on (o = d = 4096: 504 us against 822 of 128; 2048 x 512, 16
-  // of them: 63 against 50; 1024 x 1024, also 16, equal).
-  const int64_t least = o < d ? o : d;
-  const int64_t large = static_cast<int64_t>((o + 255) / 256) * ((d + 255) / 256);
-  const int32_t tile = kPlanes<T> == 1 && least > 128 && large >= 32 ? 256 : least > 64 ? 128 : 64;
-  const int32_t tiles_o = (o + tile - 1) / tile, tiles_d = (d + tile - 1) / tile;
-  const int64_t fill = tile == 256 ? kCUs : tile == 128 ? 2 * kCUs : 4 * kCUs;  // blocks the chip holds
-  int64_t w = fill / (static_cast<int64_t>(tiles_o) * tiles_d), most = (n + 127) / 128;  // two steps a share at least
-  if (w > most) w = most;
-  if (w < 1) w = 1;
-  const int64_t per = n < 1 ? kDepth : ((n + w - 1) / w + kDepth - 1) / kDepth * kDepth;
-  return {tile, tiles_o, tiles_d, static_cast<int32_t>(n < 1 ? 1 : (n + per - 1) / per), per};
+  Splits best{};
+  double least = 1e300;
+  for (int32_t tile = 64; tile <= (kPlanes<T> == 1 ? 256 : 128); tile *= 2) {
+    const int32_t tiles_o = (o + tile - 1) / tile, tiles_d = (d + tile - 1) / tile;
+    const int64_t tiles = static_cast<int64_t>(tiles_o) * tiles_d, occ = tile == 256 ? 1 : tile == 128 ? 2 : 4;
+    // Shares: 1, 2, 3, 4, 6, 8, 12, ... and as many as fill the chip once.
+    const int64_t once = kCUs * occ / tiles;
+    for (int step = 0; step < 24; ++step) {
+      int64_t w = step == 23 ? once : step < 2 ? step + 1 : (int64_t{2} + (step & 1)) << (step / 2 - 1);
+      if (w < 1 || (w > 1 && w * 128 > n)) continue;
+      const int64_t per = n < 1 ? kDepth : ((n + w - 1) / w + kDepth - 1) / kDepth * kDepth;
+      const int64_t shares = n < 1 ? 1 : (n + per - 1) / per, blocks = tiles * shares;
+      const int64_t full = blocks / (kCUs * occ), rest = blocks % (kCUs * occ);
+      const double steps = static_cast<double>(per / kDepth) + 3;  // 3: a block's start and end
+      double us = full * steps * step_us(kPlanes<T>, tile, occ);
+      if (rest > 0) us += steps * step_us(kPlanes<T>, tile, (rest + kCUs - 1) / kCUs);
+      if (shares > 1) us += 3 + 8e-6 / 5 * static_cast<double>(shares) * o * d;
+      if (us < least) {
+        least = us;
+        best = {tile, tiles_o, tiles_d, static_cast<int32_t>(shares), per};
+      }
+    }
+  }
+  return best;
 }
 
 bool act8_shape_ok(int64_t n, int32_t d) { return n >= 0 && d >= 1 && d <= KGAT_ACT8_MAX_D; }
@@ -552,7 +577,10 @@ extern "C" int kgat_act8_unpack(int32_t dtype, const int8_t* q, const uint8_t* e
 extern "C" int64_t kgat_act8_wgrad_workspace(int32_t dtype, int64_t n, int32_t o, int32_t d) {
   using namespace kgat;
   if (!act8_shape_ok(n, d) || o < 1 || o > KGAT_ACT8_MAX_D || dtype < KGAT_F32 || dtype > KGAT_F16) return -1;
-  return (dtype == KGAT_BF16 ? wgrad_splits<__bf16>(n, o, d) : wgrad_splits<float>(n, o, d)).floats(o, d);
+  return (dtype == KGAT_BF16  ? wgrad_splits<__bf16>(n, o, d)
+          : dtype == KGAT_F16 ? wgrad_splits<_Float16>(n, o, d)
+                              : wgrad_splits<float>(n, o, d))
+      .floats(o, d);
 }
 
 extern "C" int kgat_act8_wgrad(int32_t dtype, const void* dy, int64_t lddy, const int8_t* q, const uint8_t* e,
