@@ -981,7 +981,8 @@ int kgat_act8_unpack(int32_t dtype, const int8_t *q, const uint8_t *e, int64_t n
                      void *stream);
 /* A linear layer's weight gradient from its checkpointed input: dW [o][d] = dy^T x, db [o] (nullable) = the column
  * sums of dy [n, o].  The products are exact (bf16 matrix instructions, dy as one to three bf16 terms) and summed in
- * 32 bits.  A row of dy with an infinity or a NaN gives NaN.  n = 0 writes zeros. */
+ * 32 bits.  An infinity or a NaN in dy reaches its row of dW as infinities or NaN (fp16 and float: NaN) and its db.
+ * n = 0 writes zeros. */
 int64_t kgat_act8_wgrad_workspace(int32_t dtype, int64_t n, int32_t o, int32_t d);
 int kgat_act8_wgrad(int32_t dtype, const void *dy, int64_t lddy, const int8_t *q, const uint8_t *e, int64_t n,
                     int32_t o, int32_t d, float *dW, float *db, float *workspace, int64_t workspace_floats,

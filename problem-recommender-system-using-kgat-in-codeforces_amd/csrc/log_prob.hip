@@ -145,8 +145,8 @@ __device__ __forceinline__ int32_t key_item(uint64_t k) {
 template <int NT>
 struct Pool {
   static constexpr int kSize = NT + 256;  // what is kept (at most 128) and one key of every thread always fit
-  uint64_t key[2][kSize];
-  float group[256];
+  alignas(16) uint64_t key[2][kSize];
+  alignas(16) float group[256];
   float group_floor[4];
   int count, first_lost, now;
   uint64_t floor_key;  // the k-th key, once k were kept (0: none)
@@ -171,7 +171,11 @@ __device__ __forceinline__ void pool_rank(const Pool<NT>& p, int n, int k, F&& f
     const uint64_t mine = key[i];
     int rank = 0;
 #pragma unroll 4
-    for (int j = 0; j < n; ++j) rank += key[j] > mine ? 1 : 0;
+    for (int j = 0; j < n / 2; ++j) {  // two keys a read, the same ones in all lanes
+      const ulonglong2 two = reinterpret_cast<const ulonglong2*>(key)[j];
+      rank += (two.x > mine ? 1 : 0) + (two.y > mine ? 1 : 0);
+    }
+    if ((n & 1) != 0) rank += key[n - 1] > mine ? 1 : 0;
     if (rank < k) f(rank, mine);
   }
 }
@@ -223,8 +227,11 @@ __device__ __forceinline__ void pool_floor(Pool<NT>& p, float top, int k) {
   if (threadIdx.x < groups) {
     const float mine = p.group[threadIdx.x];
     int reach = 0;
-#pragma unroll 8
-    for (int j = 0; j < groups; ++j) reach += p.group[j] >= mine ? 1 : 0;
+#pragma unroll 4
+    for (int j = 0; j < groups / 4; ++j) {
+      const float4 g = reinterpret_cast<const float4*>(p.group)[j];
+      reach += (g.x >= mine ? 1 : 0) + (g.y >= mine ? 1 : 0) + (g.z >= mine ? 1 : 0) + (g.w >= mine ? 1 : 0);
+    }
     const float v = lanes_all<64>(reach >= k ? mine : -INFINITY, [](float x, float y) { return fmaxf(x, y); });
     if ((threadIdx.x & 63) == 0) p.group_floor[threadIdx.x >> 6] = v;
   }
@@ -487,7 +494,8 @@ __global__ __launch_bounds__(256) void log_prob_bwd_kernel(LogProbBwd a) {
   const int64_t c1 = c0 + a.per < a.cols ? c0 + a.per : a.cols;
   const T* s = static_cast<const T*>(a.s) + static_cast<int64_t>(row) * a.ld;
   T* ds = static_cast<T*>(a.ds) + static_cast<int64_t>(row) * a.ldds;
-  const float m = a.stats[row], l2 = a.stats[a.rows + row], h = a.stats[2 * static_cast<int64_t>(a.rows) + row];
+  const int64_t rows = a.rows;
+  const float m = a.stats[row], l2 = a.stats[rows + row], h = a.stats[2 * rows + row];
   const float gh = a.dentropy != nullptr ? a.dentropy[row] : 0.f;
   const float c = a.scale * kLog2e;
   const bool none = m == -INFINITY;

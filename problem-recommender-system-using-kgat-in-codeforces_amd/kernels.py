@@ -1456,6 +1456,13 @@ def _row_call(like: torch.Tensor, name: str, *args) -> None:
         _lib.check(status, name)
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the memory spans of two 2-D row tensors meet."""
+    def end(t):
+        return t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
+    return a.numel() > 0 and b.numel() > 0 and a.data_ptr() < end(b) and b.data_ptr() < end(a)
+
+
 def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
@@ -1694,6 +1701,8 @@ def log_prob_bwd(scores: torch.Tensor, items: torch.Tensor, stats: torch.Tensor,
         if out.shape != scores.shape or out.dtype != scores.dtype or out.device != scores.device or \
                 (n > 1 and out.stride(0) < c):
             raise ValueError("out must have the scores' shape, type and device, and rows that do not overlap")
+        if _overlap(out, scores) and not (out.data_ptr() == scores.data_ptr() and (n < 2 or out.stride(0) == scores.stride(0))):
+            raise ValueError("out must be the scores themselves or lie apart from them")
     if n:
         _row_call(scores, "kgat_log_prob_bwd", code, scores.data_ptr(), scores.stride(0), n, c, float(scale),
                   _ptr(items), items.shape[1], stats.data_ptr(), _ptr(dlogp), _ptr(dentropy), out.data_ptr(),

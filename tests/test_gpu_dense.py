@@ -552,6 +552,7 @@ def test_refusals(K):
     a = K.act8_pack(x)
     r = K.log_prob_fwd(x, items)
     g = torch.zeros(4, 2, device=DEV)
+    wide = torch.zeros(5, 48, device=DEV)
     bad = [
         lambda: K.layer_norm_fwd(x.double()),
         lambda: K.layer_norm_fwd(x.cpu()),
@@ -596,6 +597,8 @@ def test_refusals(K):
         lambda: K.log_prob_bwd(x, items, r.stats, g, torch.zeros(3, device=DEV)),
         lambda: K.log_prob_bwd(x, items, r.stats, g, out=torch.zeros(4, 41, device=DEV)),
         lambda: K.log_prob_bwd(x, items, r.stats, g, out=x.half()),
+        lambda: K.log_prob_bwd(wide[:4, :40], items, r.stats, g, out=wide[:4, 1:41]),
+        lambda: K.log_prob_bwd(wide[:4, :40], items, r.stats, g, out=wide[1:5, :40]),
         lambda: K.log_prob_bwd(x, items, r.stats, g, out=torch.zeros(1, 40, device=DEV).expand(4, 40)),
     ]
     for i, f in enumerate(bad):
