@@ -126,15 +126,17 @@ __device__ __forceinline__ void finish_row(const LogProb& a, int row, Stat r, co
 // ------------------------------------------------------------------------------------------------- best items
 // A key orders by score, then by lower item: the upper half is the score's ordered bits (never 0), the lower half the
 // item's complement.  0: no item.
-__device__ __forceinline__ uint64_t item_key(float s, uint32_t item) {
+__device__ __forceinline__ uint32_t ordered(float s) {
   const uint32_t b = __float_as_uint(s + 0.f);  // -0 and +0 are one score
-  const uint32_t o = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-  return (static_cast<uint64_t>(o) << 32) | (0xFFFFFFFFu - item);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
-__device__ __forceinline__ float key_score(uint64_t k) {
-  const uint32_t o = static_cast<uint32_t>(k >> 32);
+__device__ __forceinline__ float unordered(uint32_t o) {
   return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);
 }
+__device__ __forceinline__ uint64_t item_key(float s, uint32_t item) {
+  return (static_cast<uint64_t>(ordered(s)) << 32) | (0xFFFFFFFFu - item);
+}
+__device__ __forceinline__ float key_score(uint64_t k) { return unordered(static_cast<uint32_t>(k >> 32)); }
 __device__ __forceinline__ int32_t key_item(uint64_t k) {
   return static_cast<int32_t>(0xFFFFFFFFu - static_cast<uint32_t>(k));
 }
@@ -146,7 +148,7 @@ template <int NT>
 struct Pool {
   static constexpr int kSize = NT + 256;  // what is kept (at most 128) and one key of every thread always fit
   alignas(16) uint64_t key[2][kSize];
-  alignas(16) float group[256];
+  alignas(16) uint32_t group[256];  // ordered bits of the groups' maxima, 0: empty
   float group_floor[4];
   int count, first_lost, now;
   uint64_t floor_key;  // the k-th key, once k were kept (0: none)
@@ -215,24 +217,29 @@ __device__ __forceinline__ void pool_step(Pool<NT>& p, bool in, uint64_t key, in
   }
 }
 
-// The floor from the threads' own maxima: with the k-th largest of G (64 or 256 > k) groups' maxima as the floor, k
-// scores at least reach it, and of unordered scores hardly more: -G log(1 - k / G) on average.
-template <int NT>
-__device__ __forceinline__ void pool_floor(Pool<NT>& p, float top, int k) {
-  const int groups = k <= 48 ? 64 : 256, lanes = NT / groups;
-  for (int o = 1; o < lanes; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
-  if (threadIdx.x % lanes == 0) p.group[threadIdx.x / lanes] = top;
+// The floor from the maxima of G = 64 or 256 > k groups of the columns: with the k-th largest of them as the floor, k
+// scores at least reach it, and of unordered scores hardly more: -G log(1 - k / G) on average.  `add(i, x)` puts a score
+// into the group i mod G; k groups at least must have one, or all scores are candidates (4013 rows of 271, k = 20:
+// 42 us so, 16 us with a floor).
+__device__ __forceinline__ int pool_groups(int k) { return k <= 48 ? 64 : 256; }
+
+template <int NT, typename F>
+__device__ __forceinline__ void pool_floor(Pool<NT>& p, int k, F&& fill) {
+  const int groups = pool_groups(k);
+  if (threadIdx.x < 256) p.group[threadIdx.x] = 0;
   if (threadIdx.x < 4) p.group_floor[threadIdx.x] = -INFINITY;
   __syncthreads();
+  fill([&](uint32_t i, float x) { atomicMax(&p.group[i & (groups - 1)], ordered(x)); });
+  __syncthreads();
   if (threadIdx.x < groups) {
-    const float mine = p.group[threadIdx.x];
+    const uint32_t mine = p.group[threadIdx.x];
     int reach = 0;
 #pragma unroll 4
     for (int j = 0; j < groups / 4; ++j) {
-      const float4 g = reinterpret_cast<const float4*>(p.group)[j];
+      const uint4 g = reinterpret_cast<const uint4*>(p.group)[j];
       reach += (g.x >= mine ? 1 : 0) + (g.y >= mine ? 1 : 0) + (g.z >= mine ? 1 : 0) + (g.w >= mine ? 1 : 0);
     }
-    const float v = lanes_all<64>(reach >= k ? mine : -INFINITY, [](float x, float y) { return fmaxf(x, y); });
+    const float v = lanes_all<64>(reach >= k && mine != 0 ? unordered(mine) : -INFINITY, [](float x, float y) { return fmaxf(x, y); });
     if ((threadIdx.x & 63) == 0) p.group_floor[threadIdx.x >> 6] = v;
   }
   __syncthreads();
@@ -310,7 +317,18 @@ __global__ __launch_bounds__(NT, 4) void log_prob_kernel(LogProb a) {
       }
     }
     if constexpr (TOP) {
-      if (base == c0) pool_floor(pool, top, a.k);
+      if (base == c0)
+        pool_floor(pool, a.k, [&](auto add) {
+          const int have = static_cast<int>(c1 - c0 < NT * V ? c1 - c0 : NT * V);  // scores of first vectors
+          if (have >= pool_groups(a.k) * V) {  // the threads' maxima
+            if (threadIdx.x * V < have) add(threadIdx.x, top);
+          } else {  // all columns lie there: one by one, numbered so that lanes meet in no group
+            const int stride = (have + V - 1) / V;
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+              if (threadIdx.x * V + j < have) add(j * stride + threadIdx.x, f[j]);
+          }
+        });
       // Candidates: a wave reserves room for all of its own at once.  Few vectors hold one, and few of their elements
       // reach it, so the loops are a comparison and a scalar branch an element.
       const float floor = pool.floor;
@@ -436,11 +454,9 @@ __global__ __launch_bounds__(1024) void log_prob_join_kernel(LogProb a) {
     const uint64_t* lists = a.lists + static_cast<int64_t>(row) * a.splits * a.k;
     auto score_at = [&](int64_t i) { return lists[i] != 0 ? key_score(lists[i]) : -INFINITY; };
     if (a.splits >= a.k) {  // the lists' best scores, dealt to the groups in turn
-      const int groups = a.k <= 48 ? 64 : 256, lanes = NT / groups;
-      float top = -INFINITY;
-      for (int p = threadIdx.x / lanes + groups * (threadIdx.x % lanes); p < a.splits; p += NT)
-        top = fmaxf(top, score_at(static_cast<int64_t>(p) * a.k));
-      pool_floor(pool, top, a.k);
+      pool_floor(pool, a.k, [&](auto add) {
+        for (int p = threadIdx.x; p < a.splits; p += NT) add(p, score_at(static_cast<int64_t>(p) * a.k));
+      });
     } else {  // each list's score at place k / splits, rounded up: k scores at least reach the smallest of them
       const int place = (a.k + a.splits - 1) / a.splits - 1;
       if (threadIdx.x < 64) {

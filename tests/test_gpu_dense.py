@@ -505,6 +505,18 @@ def test_log_prob_ties_and_sorted_rows(K, k, dtype):
     assert torch.equal(r.top_items, logp_ref(small, items, k, 1.0)["top_items"])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("c", [1, 2, 63, 65, 255, 257, 1023, 1025, 2047, 2049, 2056, 9000, 16385, 24577, 24600])
+def test_log_prob_best_items_of_few_columns(K, c, dtype):
+    """Columns about as many as the groups that the floor comes from, in a row's only step and in its last share."""
+    for n, k in ((3, 1), (3, 48), (3, 49), (3, 128), (600, 20), (600, 100)):
+        k = min(k, c)
+        s = torch.randn(n, c, device=DEV).to(dtype)
+        r = K.log_prob_fwd(s, torch.zeros(n, 1, dtype=torch.int64, device=DEV), k=k)
+        value, index = torch.sort(s.float(), dim=1, descending=True, stable=True)
+        assert torch.equal(r.top_items, index[:, :k]), (n, k)
+
+
 def test_log_prob_against_differences(K):
     """The gradient against central differences of the kernels' own forward, taken in 64 bits of its definition."""
     s, items, dlogp, dent = logp_inputs(3, 50, 3, torch.float32, 9, masked=0.0, spread=1.0)
