@@ -3,7 +3,7 @@ probabilities over the item catalogue.
 
 Each is one autograd node over the typed wrappers of ``kernels`` (csrc/layer_norm.hip, act8.hip, log_prob.hip); tensors
 live on the GPU, in float32, bfloat16 or float16.  Inputs of more than two dimensions are taken as rows of their last
-one.  A node's backward can run once; gradients of gradients are not available.
+one.  Gradients of gradients are not available.  The types are the tensors' own: autocast changes nothing.
 """
 from __future__ import annotations
 
@@ -69,13 +69,17 @@ def _product(a: torch.Tensor, b: torch.Tensor, trans_b: bool) -> torch.Tensor:
     torch's plain product."""
     if a.dtype is torch.float32 and kernels.gemm_supported(a, b):
         return kernels.gemm(a, b, trans_b=trans_b)
-    return a @ (b.t() if trans_b else b)
+    with torch.autocast(a.device.type, enabled=False):
+        return a @ (b.t() if trans_b else b)
 
 
 class _LinearAct8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
         rows = _rows(x)
+        kernels._req_rows(rows, "x")
+        if weight.device != rows.device or (bias is not None and bias.device != rows.device):
+            raise ValueError(f"weight and bias: on {rows.device} expected")
         if weight.dim() != 2 or weight.shape[1] != rows.shape[1]:
             raise ValueError(f"weight: [out, {rows.shape[1]}] expected, got {list(weight.shape)}")
         if bias is not None and bias.shape != weight.shape[:1]:

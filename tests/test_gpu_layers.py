@@ -314,3 +314,23 @@ def test_log_likelihood(pkg, many):
         pkg.evaluation.log_likelihood(m, train, {3: [n_items]}, n_items)
     empty = pkg.evaluation.log_likelihood(m, {}, {}, n_items)
     assert np.isnan(empty["log_likelihood"]) and np.isnan(empty["entropy"])
+
+
+def test_linear_act8_types_and_refusals(pkg):
+    """Autocast leaves the types alone; the wrong device or type is refused with and without a gradient."""
+    x = torch.randn(6, 7, device="cuda", requires_grad=True)
+    w, b = torch.randn(5, 7, device="cuda", requires_grad=True), torch.randn(5, device="cuda")
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = pkg.layers.linear_act8(x, w, b)
+    assert y.dtype is torch.float32
+    y.sum().backward()
+    # sums of 5 products of O(1) numbers: 5 roundings of at most 2^-24 of the terms' sum each, on both sides
+    want = w.detach().double().sum(0).expand(6, 7)
+    assert ((x.grad.double() - want).abs() <= 10 * 2.0 ** -24 * w.detach().double().abs().sum(0)).all()
+    for grad in (False, True):
+        with torch.set_grad_enabled(grad):
+            for bad in (lambda: pkg.layers.linear_act8(x.cpu(), w, b), lambda: pkg.layers.linear_act8(x, w.cpu(), b),
+                        lambda: pkg.layers.linear_act8(x, w, b.cpu()), lambda: pkg.layers.linear_act8(x.double(), w, b),
+                        lambda: pkg.layers.linear_act8(x, w[:, :6], b), lambda: pkg.layers.linear_act8(x, w, b[:4])):
+                with pytest.raises(ValueError):
+                    bad()
