@@ -447,8 +447,8 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
   }
 }
 
-// Sums of parts, in their order: the first blocks take dW's elements, the others db's.  64 elements a block, its 4
-// waves every fourth part.
+// Sums of parts, in their order: the first blocks take dW's elements, the others db's.  64 elements a block at a time,
+// its 4 waves every fourth part.
 struct Join {
   const float* part[2];
   float* out[2];
@@ -461,16 +461,21 @@ __global__ __launch_bounds__(256) void act8_join_kernel(Join a) {
   __shared__ float lds[4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int which = blockIdx.x < a.blocks ? 0 : 1;
-  const int64_t i = static_cast<int64_t>(blockIdx.x - (which != 0 ? a.blocks : 0)) * 64 + lane, size = a.size[which];
+  const uint32_t first = which != 0 ? a.blocks : 0, count = which != 0 ? gridDim.x - a.blocks : a.blocks;
+  const int64_t size = a.size[which];
   const float* part = a.part[which];
   const int parts = a.parts[which];
-  float s = 0.f;
-  if (i < size)
+  for (int64_t base = static_cast<int64_t>(blockIdx.x - first) * 64; base < size; base += static_cast<int64_t>(count) * 64) {
+    const int64_t i = base + lane;
+    float s = 0.f;
+    if (i < size)
 #pragma unroll 8
-    for (int p = wave; p < parts; p += 4) s += part[p * size + i];
-  lds[wave][lane] = s;
-  __syncthreads();
-  if (wave == 0 && i < size) a.out[which][i] = (lds[0][lane] + lds[1][lane]) + (lds[2][lane] + lds[3][lane]);
+      for (int p = wave; p < parts; p += 4) s += part[p * size + i];
+    lds[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && i < size) a.out[which][i] = (lds[0][lane] + lds[1][lane]) + (lds[2][lane] + lds[3][lane]);
+    __syncthreads();
+  }
 }
 
 struct Splits {
@@ -527,11 +532,19 @@ Splits wgrad_splits(int64_t n, int32_t o, int32_t d) {
 
 bool act8_shape_ok(int64_t n, int32_t d) { return n >= 0 && d >= 1 && d <= KGAT_ACT8_MAX_D; }
 
-// Blocks of 256 threads for n rows of per_row vectors; -1: more than a launch holds.
-int64_t flat_blocks(int64_t n, int64_t per_row) {
-  if (n > (int64_t{1} << 52) / per_row) return -1;
-  const int64_t b = (n * per_row + 255) / 256;
-  return b > 0x7FFFFFFF ? -1 : b;
+// A grid holds fewer than 2^32 threads along x.
+constexpr int64_t kLaunchThreads = int64_t{1} << 31;
+
+// f(first row, rows, blocks of 256 threads) for n rows of per_row vectors, a thread each, in as many launches as it takes.
+template <typename F>
+int launch_rows(int64_t n, int64_t per_row, F&& f) {
+  const int64_t most = kLaunchThreads / per_row;
+  for (int64_t row = 0; row < n; row += most) {
+    const int64_t rows = n - row < most ? n - row : most;
+    f(row, rows, dim3(static_cast<uint32_t>((rows * per_row + 255) / 256)));
+    KGAT_LAUNCH_CHECK();
+  }
+  return KGAT_OK;
 }
 
 }  // namespace
@@ -543,16 +556,13 @@ extern "C" int kgat_act8_pack(int32_t dtype, const void* x, int64_t ldx, int64_t
   using namespace kgat;
   if (!x || !q || !e || !act8_shape_ok(n, d) || ldx < 0 || (reinterpret_cast<uintptr_t>(q) & 15))
     return KGAT_ERR_INVALID;
-  const Pack a{x, ldx, q, e, n, d};
-  return with_dtype(dtype, [&](auto t) -> int {
+  return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    const int64_t blocks = flat_blocks(n, static_cast<int64_t>((d + kBlock - 1) / kBlock) * (kBlock / Vec<T>::N));
-    if (blocks < 0) return KGAT_ERR_INVALID;
-    if (n == 0) return KGAT_OK;
-    hipLaunchKernelGGL(act8_pack_kernel<T>, dim3(static_cast<uint32_t>(blocks)), dim3(256), 0,
-                       reinterpret_cast<hipStream_t>(stream), a);
-    KGAT_LAUNCH_CHECK();
-    return KGAT_OK;
+    const int64_t nb = (d + kBlock - 1) / kBlock;
+    return launch_rows(n, nb * (kBlock / Vec<T>::N), [&](int64_t row, int64_t rows, dim3 grid) {
+      const Pack a{static_cast<const T*>(x) + row * ldx, ldx, q + row * nb * kBlock, e + row * nb, rows, d};
+      hipLaunchKernelGGL(act8_pack_kernel<T>, grid, dim3(256), 0, reinterpret_cast<hipStream_t>(stream), a);
+    });
   });
 }
 
@@ -561,16 +571,13 @@ extern "C" int kgat_act8_unpack(int32_t dtype, const int8_t* q, const uint8_t* e
   using namespace kgat;
   if (!x || !q || !e || !act8_shape_ok(n, d) || ldx < d || (reinterpret_cast<uintptr_t>(q) & 15))
     return KGAT_ERR_INVALID;
-  const Unpack a{q, e, x, ldx, n, d};
-  return with_dtype(dtype, [&](auto t) -> int {
+  return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    const int64_t blocks = flat_blocks(n, (d + Vec<T>::N - 1) / Vec<T>::N);
-    if (blocks < 0) return KGAT_ERR_INVALID;
-    if (n == 0) return KGAT_OK;
-    hipLaunchKernelGGL(act8_unpack_kernel<T>, dim3(static_cast<uint32_t>(blocks)), dim3(256), 0,
-                       reinterpret_cast<hipStream_t>(stream), a);
-    KGAT_LAUNCH_CHECK();
-    return KGAT_OK;
+    const int64_t nb = (d + kBlock - 1) / kBlock;
+    return launch_rows(n, (d + Vec<T>::N - 1) / Vec<T>::N, [&](int64_t row, int64_t rows, dim3 grid) {
+      const Unpack a{q + row * nb * kBlock, e + row * nb, static_cast<T*>(x) + row * ldx, ldx, rows, d};
+      hipLaunchKernelGGL(act8_unpack_kernel<T>, grid, dim3(256), 0, reinterpret_cast<hipStream_t>(stream), a);
+    });
   });
 }
 
@@ -604,7 +611,7 @@ extern "C" int kgat_act8_wgrad(int32_t dtype, const void* dy, int64_t lddy, cons
       const Wgrad a{dy, lddy, q, e, s.w == 1 ? dW : workspace, db == nullptr ? nullptr : j.parts[1] == 1 ? db : part_b,
                     n, s.per, o, d, (d + kBlock - 1) / kBlock, s.tiles_o, s.tiles_d, s.w};
       const int64_t blocks = static_cast<int64_t>(s.tiles_o) * s.tiles_d * s.w;
-      if (blocks > 0x7FFFFFFF) return KGAT_ERR_INVALID;
+      if (blocks > kLaunchThreads / 512) return KGAT_ERR_INVALID;  // a dW of 2^38 bytes
       const dim3 grid(static_cast<uint32_t>(blocks));
       if (o < 4) hipLaunchKernelGGL((act8_wgrad_kernel<T, 64, true>), grid, dim3(128), 0, st, a);
       else if (s.tile == 64) hipLaunchKernelGGL((act8_wgrad_kernel<T, 64, false>), grid, dim3(128), 0, st, a);
@@ -612,9 +619,8 @@ extern "C" int kgat_act8_wgrad(int32_t dtype, const void* dy, int64_t lddy, cons
       else if constexpr (kPlanes<T> == 1) hipLaunchKernelGGL((act8_wgrad_kernel<T, 256, false>), grid, dim3(512), 0, st, a);
       KGAT_LAUNCH_CHECK();
     }
-    const int64_t blocks_w = j.parts[0] == 1 ? 0 : (size + 63) / 64;
+    const int64_t blocks_w = j.parts[0] == 1 ? 0 : blocks_for(size, 64, 1 << 22);
     const int64_t blocks_b = db == nullptr || j.parts[1] == 1 ? 0 : (o + 63) / 64;
-    if (blocks_w + blocks_b > 0x7FFFFFFF) return KGAT_ERR_INVALID;
     if (blocks_w + blocks_b > 0) {
       j.blocks = static_cast<uint32_t>(blocks_w);
       hipLaunchKernelGGL(act8_join_kernel, dim3(static_cast<uint32_t>(blocks_w + blocks_b)), dim3(256), 0, st, j);

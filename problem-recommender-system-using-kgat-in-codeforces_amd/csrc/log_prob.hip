@@ -75,6 +75,7 @@ struct LogProb {
   int32_t per;           // columns of a split
   float* part;           // [rows][splits][4]: m, S, W
   uint64_t* lists;       // [rows][splits][k], best first, 0 behind the last
+  int32_t row0;          // of this launch
 };
 
 // What a whole row's sums say.
@@ -256,7 +257,7 @@ __global__ __launch_bounds__(NT, 4) void log_prob_kernel(LogProb a) {
   __shared__ Stat part[kWaves];
   __shared__ Pool<TOP ? NT : 0> pool;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int row = blockIdx.x, split = blockIdx.y;
+  const int row = a.row0 + static_cast<int>(blockIdx.x), split = blockIdx.y;
   const T* s = static_cast<const T*>(a.s) + static_cast<int64_t>(row) * a.ld;
   const int64_t c0 = static_cast<int64_t>(split) * a.per;
   const int64_t c1 = c0 + a.per < a.cols ? c0 + a.per : a.cols;
@@ -494,7 +495,8 @@ struct LogProbBwd {
   const float* dentropy;  // [rows] (nullable)
   void* ds;
   int64_t ldds;
-  int32_t per;  // columns of a block
+  int32_t per;   // columns of a block
+  int32_t row0;  // of this launch
 };
 
 // A block per row and share of its columns.  The given items' columns are computed first, from the scores and the
@@ -505,7 +507,7 @@ __global__ __launch_bounds__(256) void log_prob_bwd_kernel(LogProbBwd a) {
   __shared__ int64_t item[KGAT_LOGPROB_MAX_ITEMS];
   __shared__ float grad[KGAT_LOGPROB_MAX_ITEMS];
   __shared__ float sums[4];
-  const int row = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int row = a.row0 + static_cast<int>(blockIdx.x), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t c0 = static_cast<int64_t>(blockIdx.y) * a.per;
   const int64_t c1 = c0 + a.per < a.cols ? c0 + a.per : a.cols;
   const T* s = static_cast<const T*>(a.s) + static_cast<int64_t>(row) * a.ld;
@@ -571,6 +573,9 @@ struct Plan {
   int32_t splits, per;
 };
 
+// Rows of a launch, a block of 256 threads each: a grid holds fewer than 2^32 threads along x.
+constexpr int32_t kLaunchRows = 1 << 23;
+
 constexpr int32_t kTileCols = 8192;   // a 256-thread block's, 32 a thread
 constexpr int32_t kWideCols = 16384;  // a 1024-thread block's, 16 a thread
 
@@ -592,15 +597,18 @@ int64_t work_floats(int32_t rows, int32_t cols, int32_t k) {
 }
 
 template <typename T, bool TOP>
-int log_prob(const LogProb& a, hipStream_t st) {
-  const dim3 grid(a.rows, a.splits);
-  if (a.cols <= 2048)
-    hipLaunchKernelGGL((log_prob_kernel<T, TOP, 256, 8>), grid, dim3(256), 0, st, a);
-  else if (a.cols <= kWideCols && a.rows <= 2 * kCUs)  // few rows: each in one step of a whole CU's threads
-    hipLaunchKernelGGL((log_prob_kernel<T, TOP, 1024, 16>), grid, dim3(1024), 0, st, a);
-  else
-    hipLaunchKernelGGL((log_prob_kernel<T, TOP, 256, 32>), grid, dim3(256), 0, st, a);
-  KGAT_LAUNCH_CHECK();
+int log_prob(LogProb a, hipStream_t st) {
+  for (int64_t row0 = 0; row0 < a.rows; row0 += kLaunchRows) {
+    a.row0 = static_cast<int32_t>(row0);
+    const dim3 grid(a.rows - a.row0 < kLaunchRows ? a.rows - a.row0 : kLaunchRows, a.splits);
+    if (a.cols <= 2048)
+      hipLaunchKernelGGL((log_prob_kernel<T, TOP, 256, 8>), grid, dim3(256), 0, st, a);
+    else if (a.cols <= kWideCols && a.rows <= 2 * kCUs)  // few rows: each in one step of a whole CU's threads
+      hipLaunchKernelGGL((log_prob_kernel<T, TOP, 1024, 16>), grid, dim3(1024), 0, st, a);
+    else
+      hipLaunchKernelGGL((log_prob_kernel<T, TOP, 256, 32>), grid, dim3(256), 0, st, a);
+    KGAT_LAUNCH_CHECK();
+  }
   if (a.splits > 1) {
     hipLaunchKernelGGL((log_prob_join_kernel<T, TOP>), dim3(a.rows), dim3(1024), 0, st, a);
     KGAT_LAUNCH_CHECK();
@@ -635,7 +643,7 @@ extern "C" int kgat_log_prob_fwd(int32_t dtype, const void* scores, int64_t ld, 
     return KGAT_ERR_WORKSPACE;
   const Plan p = plan_rows(rows, cols);
   LogProb a{scores, ld, rows, cols, scale, items, t, k, logp, stats, top_item, top_logp, p.splits, p.per, workspace,
-            reinterpret_cast<uint64_t*>(workspace + (p.splits == 1 ? 0 : static_cast<int64_t>(rows) * p.splits * 4))};
+            reinterpret_cast<uint64_t*>(workspace + (p.splits == 1 ? 0 : static_cast<int64_t>(rows) * p.splits * 4)), 0};
   return with_dtype(dtype, [&](auto e) -> int {
     using T = decltype(e);
     if (rows == 0) return KGAT_OK;
@@ -651,16 +659,18 @@ extern "C" int kgat_log_prob_bwd(int32_t dtype, const void* scores, int64_t ld, 
   if (!scores_ok(scores, ld, rows, cols, items, t, scale) || !stats || (t > 0 && !dlogp) || !dscores ||
       ld_dscores < cols)
     return KGAT_ERR_INVALID;
-  constexpr int32_t per = 16384;
-  LogProbBwd a{scores, ld, rows, cols, scale, items, t, stats, dlogp, dentropy, dscores, ld_dscores, per};
-  const int64_t shares = (static_cast<int64_t>(cols) + per - 1) / per;
-  if (shares > 65535) return KGAT_ERR_INVALID;
+  int32_t per = 16384;
+  while ((static_cast<int64_t>(cols) + per - 1) / per > 65535) per *= 2;  // a grid's limit along y
+  const uint32_t shares = static_cast<uint32_t>((static_cast<int64_t>(cols) + per - 1) / per);
+  LogProbBwd a{scores, ld, rows, cols, scale, items, t, stats, dlogp, dentropy, dscores, ld_dscores, per, 0};
   return with_dtype(dtype, [&](auto e) -> int {
     using T = decltype(e);
-    if (rows == 0) return KGAT_OK;
-    hipLaunchKernelGGL(log_prob_bwd_kernel<T>, dim3(rows, static_cast<uint32_t>(shares)), dim3(256), 0,
-                       reinterpret_cast<hipStream_t>(stream), a);
-    KGAT_LAUNCH_CHECK();
+    for (int64_t row0 = 0; row0 < rows; row0 += kLaunchRows) {
+      a.row0 = static_cast<int32_t>(row0);
+      const dim3 grid(rows - a.row0 < kLaunchRows ? rows - a.row0 : kLaunchRows, shares);
+      hipLaunchKernelGGL(log_prob_bwd_kernel<T>, grid, dim3(256), 0, reinterpret_cast<hipStream_t>(stream), a);
+      KGAT_LAUNCH_CHECK();
+    }
     return KGAT_OK;
   });
 }

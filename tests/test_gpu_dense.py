@@ -679,3 +679,53 @@ def test_outputs_stay_in_their_bounds(K):
     K.log_prob_bwd(s, items, r.stats, dlogp, dent, out=big[:, 3:1002])
     assert (big[:, :3] == 7).all() and (big[:, 1002:] == 7).all()
     assert torch.equal(big[:, 3:1002], K.log_prob_bwd(s, items, r.stats, dlogp, dent))
+
+
+def test_more_rows_than_a_launch(K):
+    """Rows of several launches: the last ones and the borders' are those of a call on them alone."""
+    n = (1 << 23) + 5
+    s = torch.randn(n, 3, device=DEV).to(torch.bfloat16)
+    items = torch.arange(n, device=DEV).remainder(4).sub(1)[:, None].contiguous()
+    g, h = torch.randn(n, 1, device=DEV), torch.randn(n, device=DEV)
+    r = K.log_prob_fwd(s, items, k=2)
+    ds = K.log_prob_bwd(s, items, r.stats, g, h)
+    for part in (slice(0, 9), slice((1 << 23) - 4, n)):
+        w = K.log_prob_fwd(s[part], items[part], k=2)
+        for name in ("logp", "entropy", "lse", "top_items", "top_logp"):
+            assert torch.equal(getattr(r, name)[part], getattr(w, name)), name
+        assert torch.equal(ds[part], K.log_prob_bwd(s[part], items[part], w.stats, g[part], h[part]))
+    n = (1 << 28) + 5
+    x = torch.randn(n, 1, device=DEV)
+    a = K.act8_pack(x)
+    back = K.act8_unpack(a)
+    for part in (slice(0, 9), slice((1 << 28) - 4, n)):
+        w = K.act8_pack(x[part])
+        assert torch.equal(a.q[part], w.q) and torch.equal(a.e[part], w.e)
+        assert torch.equal(back[part], K.act8_unpack(w))
+
+
+def test_a_row_of_2_to_30_scores(K):
+    """Offsets of more than 32 bits, and shares of more columns.  The scores are 0 but for one of log 2^30 = 20.79 (in
+    bf16 20.75): p = e^20.75 / (e^20.75 + c - 1)."""
+    c = (1 << 30) + 77
+    s = torch.zeros(1, c, dtype=torch.bfloat16, device=DEV)
+    best = c - 2
+    s[0, best] = 20.75
+    items = torch.tensor([[best, 5, -1]], device=DEV)
+    top = math.exp(20.75)
+    lse = math.log(top + c - 1)
+    want = torch.tensor([[20.75 - lse, -lse, 0.0]], dtype=torch.float64)
+    r = K.log_prob_fwd(s, items, k=3)
+    # S: a chain of at most 4200 additions (a share's 2^20 columns over 256 threads, and the joins), each off by 2^-24 of
+    # the sum; a term's power off by 2^-22; lse about 21.5, off by some roundings of its size
+    tol = 4200 * 2.0 ** -24 + 24 * 2.0 ** -22
+    assert (r.logp.double().cpu() - want).abs().max() <= tol
+    assert abs(r.lse.item() - lse) <= tol
+    assert r.top_items.tolist() == [[best, 0, 1]]
+    g = torch.tensor([[1.0, 0.0, 3.0]], device=DEV)
+    ds = K.log_prob_bwd(s, items, r.stats, g)
+    p, q = top / (top + c - 1), 1 / (top + c - 1)
+    # exp of a logp off by tol, and bf16's rounding
+    assert abs(ds[0, best].item() - (1 - p)) <= p * 2 * tol + (1 - p) * 2.0 ** -8
+    others = ds[0, [0, 4, 5, 6, 16383, 16384, 1 << 29, c - 3, c - 1]].double().cpu()
+    assert (others + q).abs().max() <= q * (2 * tol + 2.0 ** -8)
