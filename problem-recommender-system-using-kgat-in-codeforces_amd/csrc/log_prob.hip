@@ -13,6 +13,8 @@
 // Masked scores (-inf) have p = 0 and count nowhere.  A row of nothing else has no distribution: logp and lse -inf,
 // H 0, gradient 0.  A row with a NaN or a +inf: everything NaN, best items -1, gradient NaN.
 // A negative item is padding (logp 0, no gradient); one beyond the catalogue makes its logp and the row's gradient NaN.
+#include <type_traits>
+
 #include "dense.hpp"
 
 namespace kgat {
@@ -134,6 +136,12 @@ __device__ __forceinline__ uint32_t ordered(float s) {
 __device__ __forceinline__ float unordered(uint32_t o) {
   return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);
 }
+__device__ __forceinline__ uint32_t lanes_max_bits(uint32_t v) {
+  return __float_as_uint(lanes_all<64>(__uint_as_float(v), [](float x, float y) {
+    const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+    return __uint_as_float(a > b ? a : b);
+  }));
+}
 __device__ __forceinline__ uint64_t item_key(float s, uint32_t item) {
   return (static_cast<uint64_t>(ordered(s)) << 32) | (0xFFFFFFFFu - item);
 }
@@ -150,7 +158,6 @@ struct Pool {
   static constexpr int kSize = NT + 256;  // what is kept (at most 128) and one key of every thread always fit
   alignas(16) uint64_t key[2][kSize];
   alignas(16) uint32_t group[256];  // ordered bits of the groups' maxima, 0: empty
-  float group_floor[4];
   int count, first_lost, now;
   uint64_t floor_key;  // the k-th key, once k were kept (0: none)
   float floor;         // no smaller score enters: behind the columns of the keys kept, an equal one ranks after them
@@ -221,31 +228,50 @@ __device__ __forceinline__ void pool_step(Pool<NT>& p, bool in, uint64_t key, in
 // The floor from the maxima of G = 64 or 256 > k groups of the columns: with the k-th largest of them as the floor, k
 // scores at least reach it, and of unordered scores hardly more: -G log(1 - k / G) on average.  `add(i, x)` puts a score
 // into the group i mod G; k groups at least must have one, or all scores are candidates (4013 rows of 271, k = 20:
-// 42 us so, 16 us with a floor).
-__device__ __forceinline__ int pool_groups(int k) { return k <= 48 ? 64 : 256; }
+// 42 us so, 16 us with a floor).  One wave finds it: 64 groups by counting each one's rank; 256 bit by bit, from the
+// first in which the maxima differ, until k to 9/8 k of them are left (6155 rows of 3781, k = 100: 61 us, 77 by ranks;
+// 8192 rows of 1000, k = 20: 31 us by ranks, 33 by bits).
+__device__ __forceinline__ uint32_t pool_groups(int k) { return k <= 48 ? 64 : 256; }
 
-template <int NT, typename F>
+template <typename T, int NT, typename F>
 __device__ __forceinline__ void pool_floor(Pool<NT>& p, int k, F&& fill) {
-  const int groups = pool_groups(k);
   if (threadIdx.x < 256) p.group[threadIdx.x] = 0;
-  if (threadIdx.x < 4) p.group_floor[threadIdx.x] = -INFINITY;
   __syncthreads();
-  fill([&](uint32_t i, float x) { atomicMax(&p.group[i & (groups - 1)], ordered(x)); });
+  const uint32_t last = pool_groups(k) - 1;
+  fill([&](uint32_t i, float x) { atomicMax(&p.group[i & last], ordered(x)); });
   __syncthreads();
-  if (threadIdx.x < groups) {
-    const uint32_t mine = p.group[threadIdx.x];
-    int reach = 0;
-#pragma unroll 4
-    for (int j = 0; j < groups / 4; ++j) {
-      const uint4 g = reinterpret_cast<const uint4*>(p.group)[j];
-      reach += (g.x >= mine ? 1 : 0) + (g.y >= mine ? 1 : 0) + (g.z >= mine ? 1 : 0) + (g.w >= mine ? 1 : 0);
+  if (threadIdx.x < 64) {
+    uint32_t floor;
+    if (last < 64) {
+      const uint32_t mine = p.group[threadIdx.x];
+      int reach = 0;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const uint4 g = reinterpret_cast<const uint4*>(p.group)[j];
+        reach += (g.x >= mine ? 1 : 0) + (g.y >= mine ? 1 : 0) + (g.z >= mine ? 1 : 0) + (g.w >= mine ? 1 : 0);
+      }
+      floor = lanes_max_bits(reach >= k ? mine : 0);
+    } else {
+      const uint4 g = reinterpret_cast<const uint4*>(p.group)[threadIdx.x];
+      const uint32_t one = __builtin_amdgcn_readfirstlane(g.x);
+      uint32_t differ = (g.x ^ one) | (g.y ^ one) | (g.z ^ one) | (g.w ^ one);
+      differ = __builtin_amdgcn_readfirstlane(lanes_max_bits(differ));  // its first bit is that of all together
+      constexpr int kLow = std::is_same_v<T, float> ? 0 : std::is_same_v<T, __bf16> ? 16 : 13;  // the type's last bit
+      const int most = k + k / 8;
+      int bit = 31 - __builtin_clz(differ | 1);
+      floor = one >> bit >> 1 << bit << 1;  // the bits that all share
+      for (int count = 256; bit >= kLow && count > most; --bit) {
+        const uint32_t v = floor | 1u << bit;
+        const int more = __popcll(__ballot(g.x >= v)) + __popcll(__ballot(g.y >= v)) + __popcll(__ballot(g.z >= v)) +
+                         __popcll(__ballot(g.w >= v));
+        if (more >= k) {
+          floor = v;
+          count = more;
+        }
+      }
     }
-    const float v = lanes_all<64>(reach >= k && mine != 0 ? unordered(mine) : -INFINITY, [](float x, float y) { return fmaxf(x, y); });
-    if ((threadIdx.x & 63) == 0) p.group_floor[threadIdx.x >> 6] = v;
+    if (threadIdx.x == 0) p.floor = floor > ordered(-INFINITY) ? unordered(floor) : -INFINITY;
   }
-  __syncthreads();
-  if (threadIdx.x == 0)
-    p.floor = fmaxf(fmaxf(p.group_floor[0], p.group_floor[1]), fmaxf(p.group_floor[2], p.group_floor[3]));
   __syncthreads();
 }
 
@@ -319,9 +345,9 @@ __global__ __launch_bounds__(NT, 4) void log_prob_kernel(LogProb a) {
     }
     if constexpr (TOP) {
       if (base == c0)
-        pool_floor(pool, a.k, [&](auto add) {
+        pool_floor<T>(pool, a.k, [&](auto add) {
           const int have = static_cast<int>(c1 - c0 < NT * V ? c1 - c0 : NT * V);  // scores of first vectors
-          if (have >= pool_groups(a.k) * V) {  // the threads' maxima
+          if (have >= static_cast<int>(pool_groups(a.k)) * V) {  // the threads' maxima
             if (threadIdx.x * V < have) add(threadIdx.x, top);
           } else {  // all columns lie there: one by one, numbered so that lanes meet in no group
             const int stride = (have + V - 1) / V;
@@ -380,7 +406,7 @@ __global__ __launch_bounds__(NT, 4) void log_prob_kernel(LogProb a) {
           pool_step(pool, in, item_key(f[i], item(i)), a.k);
         }
         __syncthreads();
-      } else if (n > a.k + 32 && base + NT * M < c1) {
+      } else if (n > a.k + a.k / 2 + 24 && base + NT * M < c1) {
         pool_keep(pool, n, a.k);  // raises the floor for the columns to come
       }
     }
@@ -454,26 +480,32 @@ __global__ __launch_bounds__(1024) void log_prob_join_kernel(LogProb a) {
     __syncthreads();
     const uint64_t* lists = a.lists + static_cast<int64_t>(row) * a.splits * a.k;
     auto score_at = [&](int64_t i) { return lists[i] != 0 ? key_score(lists[i]) : -INFINITY; };
-    if (a.splits >= a.k) {  // the lists' best scores, dealt to the groups in turn
-      pool_floor(pool, a.k, [&](auto add) {
-        for (int p = threadIdx.x; p < a.splits; p += NT) add(p, score_at(static_cast<int64_t>(p) * a.k));
-      });
-    } else {  // each list's score at place k / splits, rounded up: k scores at least reach the smallest of them
-      const int place = (a.k + a.splits - 1) / a.splits - 1;
-      if (threadIdx.x < 64) {
-        float low = INFINITY;
-        for (int p = threadIdx.x; p < a.splits; p += 64) low = fminf(low, score_at(static_cast<int64_t>(p) * a.k + place));
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) low = fminf(low, __shfl_xor(low, o));
-        if (lane == 0) pool.floor = low;
-      }
-      __syncthreads();
-    }
     const int64_t n = static_cast<int64_t>(a.splits) * a.k;
+    const int stride = a.splits >= a.k ? a.k : 1;  // enough lists: their best scores give the floor, else all do
+    pool_floor<T>(pool, a.k, [&](auto add) {
+      for (int64_t i = threadIdx.x * static_cast<int64_t>(stride), p = threadIdx.x; i < n; i += NT * static_cast<int64_t>(stride), p += NT)
+        add(static_cast<uint32_t>(p), score_at(i));
+    });
     const float floor = pool.floor;
     for (int64_t base = 0; base < n; base += NT) {
       const uint64_t key = base + threadIdx.x < n ? lists[base + threadIdx.x] : 0;
-      pool_step(pool, key != 0 && key_score(key) >= floor, key, a.k);
+      const bool in = key != 0 && key_score(key) >= floor;
+      const uint64_t who = __ballot(in);
+      if (who != 0) {
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&pool.count, __popcll(who));
+        at = __shfl(at, 0) + __popcll(who & ((1ull << lane) - 1));
+        if (in && at < Pool<NT>::kSize) pool.key[0][at] = key;
+      }
+    }
+    __syncthreads();
+    if (pool.count > Pool<NT>::kSize) {  // many equal scores: again, cut to the k best whenever the pool fills up
+      __syncthreads();
+      if (threadIdx.x == 0) pool.count = 0;
+      for (int64_t base = 0; base < n; base += NT) {
+        const uint64_t key = base + threadIdx.x < n ? lists[base + threadIdx.x] : 0;
+        pool_step(pool, key != 0 && key_score(key) >= floor, key, a.k);
+      }
     }
     __syncthreads();
     pool_rank(pool, pool.count, a.k, [&](int rank, uint64_t key) {
