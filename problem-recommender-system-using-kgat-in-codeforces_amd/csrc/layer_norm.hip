@@ -224,11 +224,14 @@ struct NormBwd {
 
 // The backward in one pass over x and dy: G threads hold a row as NV vectors, keep the weights of their columns and
 // the columns' sums of dy xhat and dy over all the rows they take, and write dx.  At the end the block joins its row
-// groups' sums in their order (by lane exchange within a wave, then through LDS) into its part.
-template <typename T, int G, int NV, int THREADS>
+// groups' sums in their order (by lane exchange within a wave, then through LDS) into its part.  With LDS_SUMS (16
+// columns a thread, one row group) the columns' sums lie in LDS instead, four of a thread together; 128 of its 160 KB.
+template <typename T, int G, int NV, int THREADS, bool LDS_SUMS>
 __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(NormBwd a) {
-  constexpr int V = Vec<T>::N, kGroups = THREADS / (G < 64 ? 64 : G);
+  constexpr int V = Vec<T>::N, kGroups = THREADS / (G < 64 ? 64 : G), kSums = LDS_SUMS ? NV * V / 4 : 0;
+  static_assert(!LDS_SUMS || kGroups == 1, "one row group");
   __shared__ float lds[4 * (THREADS / 64)];
+  __shared__ float4 sums[LDS_SUMS ? 2 * kSums * THREADS : 1];
   __shared__ float cols[kGroups > 1 ? G * NV * V : 1];
   int turn = 0;
   const int lane = threadIdx.x % G;
@@ -237,10 +240,15 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(NormBwd a) {
   const float d = static_cast<float>(a.d);
   float w[NV][V], dw[NV][V], db[NV][V];
   load_columns<T>(a.w, lane, G, a.d, 1.f, w);
+  if constexpr (LDS_SUMS) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+    for (int k = 0; k < 2 * kSums; ++k) sums[k * THREADS + threadIdx.x] = float4{0.f, 0.f, 0.f, 0.f};
+  } else {
 #pragma unroll
-    for (int j = 0; j < V; ++j) dw[i][j] = db[i][j] = 0.f;
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) dw[i][j] = db[i][j] = 0.f;
+  }
   Vec<T> nx[NV], ng[NV];
   float nmean = 0.f, nrstd = 0.f;
   auto fetch = [&](int64_t row) {
@@ -269,8 +277,35 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(NormBwd a) {
       for (int j = 0; j < V; ++j) {
         xh[i][j] = (static_cast<float>(nx[i].e[j]) - mean) * rstd;
         g[i][j] = static_cast<float>(ng[i].e[j]);
-        db[i][j] += g[i][j];
-        dw[i][j] += g[i][j] * xh[i][j];
+        if constexpr (!LDS_SUMS) {
+          db[i][j] += g[i][j];
+          dw[i][j] += g[i][j] * xh[i][j];
+        }
+      }
+    if constexpr (LDS_SUMS) {
+      if (a.part != nullptr)
+#pragma unroll
+        for (int k = 0; k < kSums; ++k) {
+          const float *gk = &g[k * 4 / V][k * 4 % V], *xk = &xh[k * 4 / V][k * 4 % V];
+          float4* at = sums + k * THREADS + threadIdx.x;
+          float4 t = at[0];
+          t.x += gk[0] * xk[0];
+          t.y += gk[1] * xk[1];
+          t.z += gk[2] * xk[2];
+          t.w += gk[3] * xk[3];
+          at[0] = t;
+          t = at[kSums * THREADS];
+          t.x += gk[0];
+          t.y += gk[1];
+          t.z += gk[2];
+          t.w += gk[3];
+          at[kSums * THREADS] = t;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
         g[i][j] *= w[i][j];
         s[0] += g[i][j];
         s[1] += g[i][j] * xh[i][j];
@@ -292,6 +327,15 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(NormBwd a) {
     }
   }
   if (a.part == nullptr) return;
+  if constexpr (LDS_SUMS) {
+#pragma unroll
+    for (int k = 0; k < kSums; ++k) {
+      const float4 p = sums[k * THREADS + threadIdx.x], q = sums[(kSums + k) * THREADS + threadIdx.x];
+      float *pk = &dw[k * 4 / V][k * 4 % V], *qk = &db[k * 4 / V][k * 4 % V];
+      pk[0] = p.x; pk[1] = p.y; pk[2] = p.z; pk[3] = p.w;
+      qk[0] = q.x; qk[1] = q.y; qk[2] = q.z; qk[3] = q.w;
+    }
+  }
   auto join = [&](float (&v)[NV][V], int which) {
     if constexpr (G < 64)
 #pragma unroll
@@ -317,12 +361,16 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(NormBwd a) {
     }
     if (group == 0 && (threadIdx.x & 63) < G) {
       float* to = a.part + (static_cast<int64_t>(blockIdx.x) * 2 + which) * a.d;
+      const NormVec& only = which == 0 ? a.dw : a.db;  // a single part is the result: one launch for the smallest calls
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const int c = (i * G + lane) * V + j;
-          if (c < a.d) to[c] = kGroups > 1 ? v[i][j] + cols[(i * V + j) * G + lane] : v[i][j];
+          const float sum = kGroups > 1 ? v[i][j] + cols[(i * V + j) * G + lane] : v[i][j];
+          if (c >= a.d) continue;
+          if (a.parts > 1) to[c] = sum;
+          else if (only.p != nullptr) only.put(c, sum);
         }
     }
   };
@@ -330,7 +378,28 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(NormBwd a) {
   join(db, 1);
 }
 
-// dx, a block per row (rows of any width).
+// A vector's weights (1 without).
+template <typename T>
+__device__ __forceinline__ void load_weights(const NormVec& w, int64_t c, int32_t d, float (&out)[Vec<T>::N]) {
+  constexpr int V = Vec<T>::N;
+  if (w.p == nullptr) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) out[j] = 1.f;
+  } else if (sizeof(T) == 4 || w.dtype == KGAT_F32) {
+#pragma unroll
+    for (int j = 0; j < V; j += 4) {
+      const Vec<float> v = load_row(static_cast<const float*>(w.p), c + j, d);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) out[j + k] = v.e[k];
+    }
+  } else {
+    const Vec<T> v = load_row(static_cast<const T*>(w.p), c, d);
+#pragma unroll
+    for (int j = 0; j < V; ++j) out[j] = static_cast<float>(v.e[j]);
+  }
+}
+
+// dx of rows wider than a block's registers: a block per row, which it reads twice.
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_dx_kernel(NormBwd a) {
   constexpr int V = Vec<T>::N;
@@ -342,55 +411,64 @@ __global__ __launch_bounds__(THREADS) void norm_dx_kernel(NormBwd a) {
     const T* dy = static_cast<const T*>(a.dy) + row * a.lddy;
     T* dx = static_cast<T*>(a.dx) + row * a.lddx;
     const float mean = a.mean[row], rstd = a.rstd[row];
-    float s[2] = {0.f, 0.f};
+    float s[2] = {0.f, 0.f}, w[V];
     for (int64_t c = threadIdx.x * V; c < a.d; c += THREADS * V) {
       const Vec<T> tx = load_row(x, c, a.d), tg = load_row(dy, c, a.d);
+      load_weights<T>(a.w, c, a.d, w);
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (c + j < a.d) {
-          float g = static_cast<float>(tg.e[j]);
-          if (a.w.p != nullptr) g *= a.w.template at<T>(c + j);
-          s[0] += g;
-          s[1] += g * ((static_cast<float>(tx.e[j]) - mean) * rstd);
-        }
+      for (int j = 0; j < V; ++j) {  // behind the row's end dy is 0
+        const float g = static_cast<float>(tg.e[j]) * w[j];
+        s[0] += g;
+        s[1] += g * ((static_cast<float>(tx.e[j]) - mean) * rstd);
+      }
     }
     group_sum<THREADS, THREADS>(s, lds, turn);
     const float mg = s[0] / d, mgx = s[1] / d;
     for (int64_t c = threadIdx.x * V; c < a.d; c += THREADS * V) {
       const Vec<T> tx = load_row(x, c, a.d), tg = load_row(dy, c, a.d);
+      load_weights<T>(a.w, c, a.d, w);
       Vec<T> t;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float g = static_cast<float>(tg.e[j]);
-        if (a.w.p != nullptr && c + j < a.d) g *= a.w.template at<T>(c + j);
-        t.e[j] = static_cast<T>(rstd * (g - mg - (static_cast<float>(tx.e[j]) - mean) * rstd * mgx));
-      }
+      for (int j = 0; j < V; ++j)
+        t.e[j] = static_cast<T>(rstd * (static_cast<float>(tg.e[j]) * w[j] - mg - (static_cast<float>(tx.e[j]) - mean) * rstd * mgx));
       store_row(dx, c, a.d, t);
     }
   }
 }
 
-// The rows' sums by column: a block takes 64 columns and a share of the rows, its 4 waves every fourth row.
+// The rows' sums by column, of rows wider than a block's registers: a block takes 64 vectors of columns and a share of
+// the rows, its 4 waves every fourth row.
 template <typename T>
 __global__ __launch_bounds__(256) void norm_cols_kernel(NormBwd a) {
-  __shared__ float lds[2][4][64];
+  constexpr int V = Vec<T>::N;
+  __shared__ float lds[2][4][64 * V];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+  const int64_t c0 = static_cast<int64_t>(blockIdx.x) * 64 * V, c = c0 + lane * V;
   const int64_t per = (a.n + a.parts - 1) / a.parts, r0 = blockIdx.y * per, r1 = r0 + per < a.n ? r0 + per : a.n;
-  float sw = 0.f, sb = 0.f;
-  if (c < a.d)
-    for (int64_t row = r0 + wave; row < r1; row += 4) {
-      const float g = static_cast<float>(static_cast<const T*>(a.dy)[row * a.lddy + c]);
-      const float x = static_cast<float>(static_cast<const T*>(a.x)[row * a.ldx + c]);
-      sw += g * ((x - a.mean[row]) * a.rstd[row]);
-      sb += g;
+  float sw[V], sb[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) sw[j] = sb[j] = 0.f;
+  for (int64_t row = r0 + wave; row < r1; row += 4) {
+    const Vec<T> x = load_row(static_cast<const T*>(a.x) + row * a.ldx, c, a.d);
+    const Vec<T> g = load_row(static_cast<const T*>(a.dy) + row * a.lddy, c, a.d);
+    const float mean = a.mean[row], rstd = a.rstd[row];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      sw[j] += static_cast<float>(g.e[j]) * ((static_cast<float>(x.e[j]) - mean) * rstd);
+      sb[j] += static_cast<float>(g.e[j]);
     }
-  lds[0][wave][lane] = sw;
-  lds[1][wave][lane] = sb;
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    lds[0][wave][j * 64 + lane] = sw[j];
+    lds[1][wave][j * 64 + lane] = sb[j];
+  }
   __syncthreads();
-  if (wave < 2 && c < a.d) {
-    const float s = (lds[wave][0][lane] + lds[wave][1][lane]) + (lds[wave][2][lane] + lds[wave][3][lane]);
-    a.part[(static_cast<int64_t>(blockIdx.y) * 2 + wave) * a.d + c] = s;
+  for (int i = threadIdx.x; i < 2 * 64 * V; i += 256) {
+    const int which = i / (64 * V), at = i % (64 * V);  // column c0 + (at % 64) V + at / 64
+    const int64_t to = c0 + at % 64 * V + at / 64;
+    const float s = (lds[which][0][at] + lds[which][1][at]) + (lds[which][2][at] + lds[which][3][at]);
+    if (to < a.d) a.part[(static_cast<int64_t>(blockIdx.y) * 2 + which) * a.d + to] = s;
   }
 }
 
@@ -437,8 +515,8 @@ bool with_shape(int32_t d, F&& f) {
 }
 
 // Elements of a thread: the forward keeps two weights beside each, the backward also two sums, which leaves 8 in the
-// 128 registers of a 1024-thread block (16 spilled 34 to 63 of them).
-constexpr int kFwdElems = 16, kBwdElems = 8;
+// 128 registers of a 1024-thread block (16 spilled 34 to 63 of them); with the sums in LDS it is 16.
+constexpr int kFwdElems = 16, kBwdElems = 8, kBwdLdsElems = 16;
 constexpr int kBwdThreads = 1024;
 
 template <typename T>
@@ -459,7 +537,8 @@ template <typename T>
 int norm_parts(int64_t n, int32_t d) {
   int parts = 0;
   if (with_shape<T, kBwdElems>(d, [&](auto g, auto) { parts = blocks_for(n, kBwdThreads / decltype(g)::value, kCUs); })) return parts;
-  const int64_t cols = (static_cast<int64_t>(d) + 63) / 64;
+  if (d <= kBwdThreads * kBwdLdsElems) return blocks_for(n, 1, kCUs);
+  const int64_t cols = (static_cast<int64_t>(d) + 64 * Vec<T>::N - 1) / (64 * Vec<T>::N);
   int64_t p = (1024 + cols - 1) / cols;  // wide rows: about 1024 blocks in all, 16 rows at least in each
   if (p > (n + 15) / 16) p = (n + 15) / 16;
   return p < 1 ? 1 : static_cast<int>(p);
@@ -470,18 +549,24 @@ int norm_bwd(NormBwd a, hipStream_t st) {
   const bool cols = a.dw.p != nullptr || a.db.p != nullptr;
   a.parts = norm_parts<T>(a.n, a.d);
   if (!cols) a.part = nullptr;
-  const bool done = with_shape<T, kBwdElems>(a.d, [&](auto g, auto nv) {
+  bool done = with_shape<T, kBwdElems>(a.d, [&](auto g, auto nv) {
     constexpr int G = decltype(g)::value, NV = decltype(nv)::value;
-    hipLaunchKernelGGL((norm_bwd_kernel<T, G, NV, kBwdThreads>), dim3(a.parts), dim3(kBwdThreads), 0, st, a);
+    hipLaunchKernelGGL((norm_bwd_kernel<T, G, NV, kBwdThreads, false>), dim3(a.parts), dim3(kBwdThreads), 0, st, a);
   });
+  if (!done && a.d <= kBwdThreads * kBwdLdsElems) {
+    constexpr int NV = kBwdLdsElems / Vec<T>::N;
+    hipLaunchKernelGGL((norm_bwd_kernel<T, kBwdThreads, NV, kBwdThreads, true>), dim3(a.parts), dim3(kBwdThreads), 0, st, a);
+    done = true;
+  }
   KGAT_LAUNCH_CHECK();
   if (!done && a.dx != nullptr && a.n > 0) {
-    hipLaunchKernelGGL((norm_dx_kernel<T, 256>), dim3(blocks_for(a.n, 1, 1 << 20)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((norm_dx_kernel<T, 1024>), dim3(blocks_for(a.n, 1, 1 << 20)), dim3(1024), 0, st, a);
     KGAT_LAUNCH_CHECK();
   }
-  if (!cols) return KGAT_OK;
+  if (!cols || (done && a.parts == 1)) return KGAT_OK;
   if (!done) {
-    hipLaunchKernelGGL(norm_cols_kernel<T>, dim3((a.d + 63) / 64, a.parts), dim3(256), 0, st, a);
+    const int width = 64 * Vec<T>::N;
+    hipLaunchKernelGGL(norm_cols_kernel<T>, dim3((a.d + width - 1) / width, a.parts), dim3(256), 0, st, a);
     KGAT_LAUNCH_CHECK();
   }
   hipLaunchKernelGGL(norm_cols_join_kernel, dim3((2 * a.d + 63) / 64), dim3(1024), 0, st, a);

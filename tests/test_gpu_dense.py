@@ -94,7 +94,9 @@ def norm_inputs(n, d, dtype, w_dtype, seed):
 
 NORM_SHAPES = [(1, 1), (1, 64), (3, 2), (5, 7), (17, 33), (2, 64), (129, 63), (300, 65), (1000, 128), (37, 255),
                (64, 257), (33, 511), (9, 1021), (20, 1024), (7, 2047), (6, 2049), (5, 4096), (3, 4100), (3, 8191),
-               (2, 8193), (2, 16384), (3, 16399), (2, 32769), (2, 70001), (4099, 16), (20011, 8)]
+               (2, 8193), (2, 16384), (3, 16399), (2, 32769), (2, 70001), (4099, 16), (20011, 8),
+               # several rows a block with the sums in LDS, and wider rows in shares
+               (600, 9001), (515, 16384), (70, 16399), (37, 20000)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -503,6 +505,18 @@ def test_log_prob_ties_and_sorted_rows(K, k, dtype):
     small = s[:, :9000].contiguous()
     r = K.log_prob_fwd(small, items, k=k)
     assert torch.equal(r.top_items, logp_ref(small, items, k, 1.0)["top_items"])
+
+
+@pytest.mark.parametrize("k", [20, 40, 128])
+def test_log_prob_ties_over_many_shares(K, k):
+    """More equal scores than the pool that joins the shares holds."""
+    s = torch.zeros(4, 300007, device=DEV)
+    s[1] = torch.randint(0, 2, (300007,), device=DEV, generator=gen(k)).float()
+    s[2, ::2] = -float("inf")
+    s[3, 150000:] = torch.arange(150007, device=DEV).float().div(64).floor()
+    items = torch.zeros(4, 1, dtype=torch.int64, device=DEV)
+    r = K.log_prob_fwd(s, items, k=k)
+    assert torch.equal(r.top_items, logp_ref(s, items, k, 1.0)["top_items"])
 
 
 @pytest.mark.parametrize("dtype", TYPES)
