@@ -57,7 +57,7 @@ __device__ __forceinline__ void load_columns(const NormVec& w, int lane, int G, 
   }
 }
 
-// Sums of K values over the G threads of a row (G a power of two; G > 64: whole waves, through LDS).  Every thread of
+// Sums of K values over the G threads of a row (a power of two up to 64, or whole waves, through LDS).  Every thread of
 // the block calls it.  `turn` alternates between two LDS halves, so one barrier a sum is enough: who writes a half
 // again has passed the barrier of the sum between, and with it every reader of the half.
 template <int G, int THREADS, int K>
@@ -102,6 +102,7 @@ struct NormFwd {
 template <typename T, int G, int NV, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_fwd_kernel(NormFwd a) {
   constexpr int V = Vec<T>::N;
+  static_assert(THREADS % G == 0, "whole rows");
   __shared__ float lds[2 * (THREADS / 64)];
   int turn = 0;
   const int lane = threadIdx.x % G;
@@ -229,6 +230,7 @@ struct NormBwd {
 template <typename T, int G, int NV, int THREADS, bool LDS_SUMS>
 __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(NormBwd a) {
   constexpr int V = Vec<T>::N, kGroups = THREADS / (G < 64 ? 64 : G), kSums = LDS_SUMS ? NV * V / 4 : 0;
+  static_assert(THREADS % G == 0, "whole rows");
   static_assert(!LDS_SUMS || kGroups == 1, "one row group");
   __shared__ float lds[4 * (THREADS / 64)];
   __shared__ float4 sums[LDS_SUMS ? 2 * kSums * THREADS : 1];
@@ -479,6 +481,7 @@ __global__ __launch_bounds__(1024) void norm_cols_join_kernel(NormBwd a) {
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + lane, width = 2 * static_cast<int64_t>(a.d);
   float s = 0.f;
   if (c < width)
+#pragma unroll 8
     for (int p = wave; p < a.parts; p += 16) s += a.part[p * width + c];
   lds[wave][lane] = s;
   __syncthreads();
@@ -491,38 +494,46 @@ __global__ __launch_bounds__(1024) void norm_cols_join_kernel(NormBwd a) {
 }
 
 // The rows' shape: G threads a row, NV vectors a thread, E elements of a thread at most; a narrow row shares its wave
-// with others.  f(G, NV) as integral constants; false: wider than 1024 E columns.
+// with others, a wide one takes 1, 2, 3, 4, 6, 8, 12 or 16 waves (a wave without a column costs as
+// much as any: 16384 x 1032 bf16 backward 39 us with 4 waves a row, 35 with 3).  f(G, NV) as integral constants; false: wider than
+// 1024 E columns.
 template <typename T, int E, typename F>
 bool with_shape(int32_t d, F&& f) {
   constexpr int NV = E / Vec<T>::N;
-  const auto use = [&](auto g, auto nv) {
-    f(g, nv);
-    return true;
-  };
-  const std::integral_constant<int, 1> one{};
-  const std::integral_constant<int, NV> all{};
   const int nvec = (d + Vec<T>::N - 1) / Vec<T>::N;
-  if (nvec <= 8) return use(std::integral_constant<int, 8>{}, one);
-  if (nvec <= 16) return use(std::integral_constant<int, 16>{}, one);
-  if (nvec <= 32) return use(std::integral_constant<int, 32>{}, one);
-  if (nvec <= 64) return use(std::integral_constant<int, 64>{}, one);
-  if (nvec <= 64 * NV) return use(std::integral_constant<int, 64>{}, all);
-  if (nvec <= 128 * NV) return use(std::integral_constant<int, 128>{}, all);
-  if (nvec <= 256 * NV) return use(std::integral_constant<int, 256>{}, all);
-  if (nvec <= 512 * NV) return use(std::integral_constant<int, 512>{}, all);
-  if (nvec <= 1024 * NV) return use(std::integral_constant<int, 1024>{}, all);
-  return false;
+  bool done = false;
+  const auto offer = [&](auto g, auto nv) {
+    if (done || nvec > decltype(g)::value * decltype(nv)::value) return;
+    f(g, nv);
+    done = true;
+  };
+  const auto one = [&](auto g) { offer(g, std::integral_constant<int, 1>{}); };
+  const auto all = [&](auto g) { offer(g, std::integral_constant<int, NV>{}); };
+  one(std::integral_constant<int, 8>{});
+  one(std::integral_constant<int, 16>{});
+  one(std::integral_constant<int, 32>{});
+  one(std::integral_constant<int, 64>{});
+  if constexpr (NV > 1) all(std::integral_constant<int, 64>{});
+  all(std::integral_constant<int, 128>{});
+  all(std::integral_constant<int, 192>{});
+  all(std::integral_constant<int, 256>{});
+  all(std::integral_constant<int, 384>{});
+  all(std::integral_constant<int, 512>{});
+  all(std::integral_constant<int, 768>{});
+  all(std::integral_constant<int, 1024>{});
+  return done;
 }
 
 // Elements of a thread: the forward keeps two weights beside each, the backward also two sums, which leaves 8 in the
 // 128 registers of a 1024-thread block (16 spilled 34 to 63 of them); with the sums in LDS it is 16.
 constexpr int kFwdElems = 16, kBwdElems = 8, kBwdLdsElems = 16;
 constexpr int kBwdThreads = 1024;
+constexpr int bwd_threads(int G) { return kBwdThreads / G * G; }  // whole rows
 
 template <typename T>
 int norm_fwd(const NormFwd& a, hipStream_t st) {
   const bool done = with_shape<T, kFwdElems>(a.d, [&](auto g, auto nv) {
-    constexpr int G = decltype(g)::value, NV = decltype(nv)::value, kThreads = G > 256 ? G : 256;
+    constexpr int G = decltype(g)::value, NV = decltype(nv)::value, kThreads = G > 256 ? G : 256 / G * G;
     const int grid = blocks_for(a.n, kThreads / G, kCUs * (kThreads > 512 ? 1 : 1024 / kThreads));  // 16 waves a CU
     hipLaunchKernelGGL((norm_fwd_kernel<T, G, NV, kThreads>), dim3(grid), dim3(kThreads), 0, st, a);
   });
@@ -551,7 +562,7 @@ int norm_bwd(NormBwd a, hipStream_t st) {
   if (!cols) a.part = nullptr;
   bool done = with_shape<T, kBwdElems>(a.d, [&](auto g, auto nv) {
     constexpr int G = decltype(g)::value, NV = decltype(nv)::value;
-    hipLaunchKernelGGL((norm_bwd_kernel<T, G, NV, kBwdThreads, false>), dim3(a.parts), dim3(kBwdThreads), 0, st, a);
+    hipLaunchKernelGGL((norm_bwd_kernel<T, G, NV, bwd_threads(G), false>), dim3(a.parts), dim3(bwd_threads(G)), 0, st, a);
   });
   if (!done && a.d <= kBwdThreads * kBwdLdsElems) {
     constexpr int NV = kBwdLdsElems / Vec<T>::N;
