@@ -488,25 +488,25 @@ struct Splits {
   }
 };
 
-// Microseconds of a step of 64 rows with `occ` blocks on a CU, measured (n = 16384, o = d = 1024; 256: also 4096): a
+// Microseconds of a step of 64 rows with `occ` blocks on a CU, measured (n = 16384, o = d = 1024 and 4096): a
 // step of bf16 dy takes 0.73 / 1.4 us with 1 / 4 blocks of 64, 1.25 / 1.7 with 1 / 2 of 128, 2.25 with one of 256; of
-// fp16 dy 2.3 with 4 (64) and 1.9 / 2.6 (128); of float dy 1.6 / 2.4 (64) and 2.45 / 3.4 (128).
+// fp16 dy 2.3 with 4 (64), 1.9 / 2.4 (128) and 4.1 (256); of float dy 1.6 / 2.4 (64), 2.45 / 2.95 (128) and 5.8 (256).
 double step_us(int planes, int32_t tile, int64_t occ) {
   const double n = static_cast<double>(occ);
-  if (tile == 256) return 2.25;
-  if (tile == 128) return planes == 1 ? 0.8 + 0.45 * n : planes == 2 ? 1.2 + 0.7 * n : 1.5 + 0.95 * n;
+  if (tile == 256) return planes == 1 ? 2.25 : planes == 2 ? 4.1 : 5.8;
+  if (tile == 128) return planes == 1 ? 0.8 + 0.45 * n : planes == 2 ? 1.3 + 0.55 * n : 1.7 + 0.62 * n;
   return planes == 1 ? 0.6 + 0.2 * n : planes == 2 ? 0.9 + 0.35 * n : 1.35 + 0.26 * n;
 }
 
 // The tile and the number of row shares with the least estimated time: the blocks' steps (4, 2 or 1 of them on a CU at
 // once), and the shares' tiles written and read again at 5 TB/s.  One rule for every size: at o = d = 4096 tiles of 256
-// take 504 us and of 128 822 us; at 2048 x 512 (n = 8192) 63 and 50; at o = d = 64 (n = 2048) one share takes 53 us, 16 of
-// them 18.
+// take 504 us and of 128 822 us (fp16 950 and 1140, float 1375 and 1575); at 2048 x 512 (n = 8192) 63 and 50; at
+// o = d = 64 (n = 2048) one share takes 53 us, 16 of them 18.
 template <typename T>
 Splits wgrad_splits(int64_t n, int32_t o, int32_t d) {
   Splits best{};
   double least = 1e300;
-  for (int32_t tile = 64; tile <= (kPlanes<T> == 1 ? 256 : 128); tile *= 2) {
+  for (int32_t tile = 64; tile <= 256; tile *= 2) {
     const int32_t tiles_o = (o + tile - 1) / tile, tiles_d = (d + tile - 1) / tile;
     const int64_t tiles = static_cast<int64_t>(tiles_o) * tiles_d, occ = tile == 256 ? 1 : tile == 128 ? 2 : 4;
     // Shares: 1, 2, 3, 4, 6, 8, 12, ... and as many as fill the chip once.
@@ -616,7 +616,7 @@ extern "C" int kgat_act8_wgrad(int32_t dtype, const void* dy, int64_t lddy, cons
       if (o < 4) hipLaunchKernelGGL((act8_wgrad_kernel<T, 64, true>), grid, dim3(128), 0, st, a);
       else if (s.tile == 64) hipLaunchKernelGGL((act8_wgrad_kernel<T, 64, false>), grid, dim3(128), 0, st, a);
       else if (s.tile == 128) hipLaunchKernelGGL((act8_wgrad_kernel<T, 128, false>), grid, dim3(256), 0, st, a);
-      else if constexpr (kPlanes<T> == 1) hipLaunchKernelGGL((act8_wgrad_kernel<T, 256, false>), grid, dim3(512), 0, st, a);
+      else hipLaunchKernelGGL((act8_wgrad_kernel<T, 256, false>), grid, dim3(512), 0, st, a);
       KGAT_LAUNCH_CHECK();
     }
     const int64_t blocks_w = j.parts[0] == 1 ? 0 : blocks_for(size, 64, 1 << 22);

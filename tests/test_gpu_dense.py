@@ -273,7 +273,9 @@ def test_act8_borders(K):
 
 
 WGRAD_SHAPES = [(1, 1, 1), (1, 64, 64), (2, 3, 5), (63, 17, 33), (64, 128, 128), (65, 129, 127), (513, 64, 257),
-                (1000, 131, 67), (2048, 64, 64), (4099, 200, 96), (30011, 33, 40), (700, 300, 520), (1025, 513, 260)]
+                (1000, 131, 67), (2048, 64, 64), (4099, 200, 96), (30011, 33, 40), (700, 300, 520), (1025, 513, 260),
+                # tiles of 256, whole and in shares
+                (333, 4001, 3999), (20000, 2000, 2041)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
