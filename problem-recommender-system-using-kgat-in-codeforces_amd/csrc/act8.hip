@@ -597,11 +597,11 @@ extern "C" int kgat_act8_wgrad(int32_t dtype, const void* dy, int64_t lddy, cons
   if (!dy || !q || !e || !dW || !act8_shape_ok(n, d) || o < 1 || o > KGAT_ACT8_MAX_D || lddy < 0 ||
       (reinterpret_cast<uintptr_t>(q) & 15) || dtype < KGAT_F32 || dtype > KGAT_F16)
     return KGAT_ERR_INVALID;
-  if (!workspace || workspace_floats < kgat_act8_wgrad_workspace(dtype, n, o, d)) return KGAT_ERR_WORKSPACE;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   return with_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
     const Splits s = wgrad_splits<T>(n, o, d);
+    if (!workspace || workspace_floats < s.floats(o, d)) return KGAT_ERR_WORKSPACE;
     const int64_t size = static_cast<int64_t>(o) * d;
     float* part_b = workspace + s.w * size;
     Join j{{workspace, part_b}, {dW, db}, {size, o}, {s.w, s.w}, 0};

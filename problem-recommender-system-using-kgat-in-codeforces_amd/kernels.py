@@ -14,7 +14,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .graph import DeviceGraph, stream_ptr
+from .graph import DeviceGraph, _raw_stream, stream_ptr
 
 
 def _req(t: torch.Tensor, name: str, dtype=torch.float32, dim: int | None = None) -> None:
@@ -1439,6 +1439,7 @@ def _req_like(t: torch.Tensor, name: str, like: torch.Tensor, shape, dtype) -> N
         raise ValueError(f"{name}: on {t.device}, the rows are on {like.device}")
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _ROW_FN: dict = {}  # name -> the bound library function
 
 
@@ -1447,8 +1448,9 @@ def _row_call(like: torch.Tensor, name: str, *args) -> None:
     fn = _ROW_FN.get(name)
     if fn is None:
         fn = _ROW_FN[name] = getattr(_lib.lib(), name)
-    if like.get_device() == torch.cuda.current_device():
-        status = fn(*args, stream_ptr(like.device))
+    index = like.get_device()
+    if _raw_stream is not None and index == _current_device():  # stream_ptr's query, its checks made before
+        status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(like.device):
             status = fn(*args, stream_ptr(like.device))
@@ -1492,7 +1494,7 @@ def layer_norm_fwd(x: torch.Tensor, weight: torch.Tensor | None = None, bias: to
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError("weight and bias must have one type")
     w_code = ROW_DTYPES[weight.dtype if weight is not None else torch.float32 if bias is None else bias.dtype]
-    y = x.new_empty((n, d))
+    y = torch.empty_like(x) if x.is_contiguous() else x.new_empty((n, d))
     mean = rstd = None
     if stats:
         mean, rstd = x.new_empty(n, dtype=torch.float32), x.new_empty(n, dtype=torch.float32)
@@ -1518,7 +1520,7 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: 
     _req_like(rstd, "rstd", x, (n,), torch.float32)
     _norm_weight(weight, "weight", x)
     w_dtype = torch.float32 if weight is None else weight.dtype
-    dx = x.new_empty((n, d)) if need_dx else None
+    dx = None if not need_dx else torch.empty_like(x) if x.is_contiguous() else x.new_empty((n, d))
     dw = x.new_empty(d, dtype=w_dtype) if need_dweight else None
     db = x.new_empty(d, dtype=w_dtype) if need_dbias else None
     ws = None
