@@ -16,10 +16,6 @@ namespace {
 struct NormVec {
   void* p;
   int32_t dtype;
-  template <typename T>
-  __device__ __forceinline__ float at(int64_t j) const {
-    return dtype == KGAT_F32 ? static_cast<const float*>(p)[j] : static_cast<float>(static_cast<const T*>(p)[j]);
-  }
   __device__ __forceinline__ void put(int64_t j, float v) const {
     if (dtype == KGAT_F32) static_cast<float*>(p)[j] = v;
     else if (dtype == KGAT_BF16) static_cast<__bf16*>(p)[j] = static_cast<__bf16>(v);
@@ -160,6 +156,28 @@ __global__ __launch_bounds__(THREADS) void norm_fwd_kernel(NormFwd a) {
   }
 }
 
+// A vector's weights; `none` where there is no vector of them.
+template <typename T>
+__device__ __forceinline__ void load_weights(const NormVec& w, int64_t c, int32_t d, float none,
+                                             float (&out)[Vec<T>::N]) {
+  constexpr int V = Vec<T>::N;
+  if (w.p == nullptr) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) out[j] = none;
+  } else if (sizeof(T) == 4 || w.dtype == KGAT_F32) {
+#pragma unroll
+    for (int j = 0; j < V; j += 4) {
+      const Vec<float> v = load_row(static_cast<const float*>(w.p), c + j, d);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) out[j + k] = v.e[k];
+    }
+  } else {
+    const Vec<T> v = load_row(static_cast<const T*>(w.p), c, d);
+#pragma unroll
+    for (int j = 0; j < V; ++j) out[j] = static_cast<float>(v.e[j]);
+  }
+}
+
 // Rows wider than a block's registers: the row is read three times (from the cache the second and third time).
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_fwd_wide_kernel(NormFwd a) {
@@ -171,6 +189,7 @@ __global__ __launch_bounds__(THREADS) void norm_fwd_wide_kernel(NormFwd a) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     T* y = static_cast<T*>(a.y) + row * a.ldy;
     float s[1] = {0.f}, q[1] = {0.f};
+#pragma unroll 4
     for (int64_t c = threadIdx.x * V; c < a.d; c += THREADS * V) {
       const Vec<T> t = load_row(x, c, a.d);
 #pragma unroll
@@ -178,6 +197,7 @@ __global__ __launch_bounds__(THREADS) void norm_fwd_wide_kernel(NormFwd a) {
     }
     group_sum<THREADS, THREADS>(s, lds, turn);
     const float mean = s[0] / d;
+#pragma unroll 4
     for (int64_t c = threadIdx.x * V; c < a.d; c += THREADS * V) {
       const Vec<T> t = load_row(x, c, a.d);
 #pragma unroll
@@ -188,16 +208,14 @@ __global__ __launch_bounds__(THREADS) void norm_fwd_wide_kernel(NormFwd a) {
     }
     group_sum<THREADS, THREADS>(q, lds, turn);
     const float rstd = 1.f / sqrtf(q[0] / d + a.eps);
+#pragma unroll 4
     for (int64_t c = threadIdx.x * V; c < a.d; c += THREADS * V) {
       Vec<T> t = load_row(x, c, a.d);
+      float w[V], b[V];
+      load_weights<T>(a.w, c, a.d, 1.f, w);
+      load_weights<T>(a.b, c, a.d, 0.f, b);
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (c + j < a.d) {
-          float r = (static_cast<float>(t.e[j]) - mean) * rstd;
-          if (a.w.p != nullptr) r *= a.w.template at<T>(c + j);
-          if (a.b.p != nullptr) r += a.b.template at<T>(c + j);
-          t.e[j] = static_cast<T>(r);
-        }
+      for (int j = 0; j < V; ++j) t.e[j] = static_cast<T>((static_cast<float>(t.e[j]) - mean) * rstd * w[j] + b[j]);
       store_row(y, c, a.d, t);
     }
     if (threadIdx.x == 0 && a.mean != nullptr) {
@@ -380,27 +398,6 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(NormBwd a) {
   join(db, 1);
 }
 
-// A vector's weights (1 without).
-template <typename T>
-__device__ __forceinline__ void load_weights(const NormVec& w, int64_t c, int32_t d, float (&out)[Vec<T>::N]) {
-  constexpr int V = Vec<T>::N;
-  if (w.p == nullptr) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) out[j] = 1.f;
-  } else if (sizeof(T) == 4 || w.dtype == KGAT_F32) {
-#pragma unroll
-    for (int j = 0; j < V; j += 4) {
-      const Vec<float> v = load_row(static_cast<const float*>(w.p), c + j, d);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) out[j + k] = v.e[k];
-    }
-  } else {
-    const Vec<T> v = load_row(static_cast<const T*>(w.p), c, d);
-#pragma unroll
-    for (int j = 0; j < V; ++j) out[j] = static_cast<float>(v.e[j]);
-  }
-}
-
 // dx of rows wider than a block's registers: a block per row, which it reads twice.
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_dx_kernel(NormBwd a) {
@@ -414,9 +411,10 @@ __global__ __launch_bounds__(THREADS) void norm_dx_kernel(NormBwd a) {
     T* dx = static_cast<T*>(a.dx) + row * a.lddx;
     const float mean = a.mean[row], rstd = a.rstd[row];
     float s[2] = {0.f, 0.f}, w[V];
+#pragma unroll 4
     for (int64_t c = threadIdx.x * V; c < a.d; c += THREADS * V) {
       const Vec<T> tx = load_row(x, c, a.d), tg = load_row(dy, c, a.d);
-      load_weights<T>(a.w, c, a.d, w);
+      load_weights<T>(a.w, c, a.d, 1.f, w);
 #pragma unroll
       for (int j = 0; j < V; ++j) {  // behind the row's end dy is 0
         const float g = static_cast<float>(tg.e[j]) * w[j];
@@ -426,9 +424,10 @@ __global__ __launch_bounds__(THREADS) void norm_dx_kernel(NormBwd a) {
     }
     group_sum<THREADS, THREADS>(s, lds, turn);
     const float mg = s[0] / d, mgx = s[1] / d;
+#pragma unroll 4
     for (int64_t c = threadIdx.x * V; c < a.d; c += THREADS * V) {
       const Vec<T> tx = load_row(x, c, a.d), tg = load_row(dy, c, a.d);
-      load_weights<T>(a.w, c, a.d, w);
+      load_weights<T>(a.w, c, a.d, 1.f, w);
       Vec<T> t;
 #pragma unroll
       for (int j = 0; j < V; ++j)
