@@ -94,7 +94,10 @@ struct NormFwd {
 
 // G threads hold a row as NV vectors each, and the weights of their columns over all the rows they take (a row's
 // weights are 8 bytes a column: read again for every row they would be up to four times its own bytes, from the
-// cache).  The next row is on its way while one is normalised.
+// cache).  The next row is on its way while one is normalised.  Two passes over the registers, not sums of x and x^2:
+// a row far from 0 keeps its variance.
+// Bound by memory: 1M x 64 float 86 us (512 MB, 6.0 TB/s), 8192 x 4096 bf16 24 us (134 MB, 5.5 TB/s).  At odd widths
+// the 16-byte accesses straddle cache lines: 16484 x 1021 bf16 16.6 us (4.1 TB/s), x 1024 13.4.
 template <typename T, int G, int NV, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_fwd_kernel(NormFwd a) {
   constexpr int V = Vec<T>::N;
@@ -179,6 +182,7 @@ __device__ __forceinline__ void load_weights(const NormVec& w, int64_t c, int32_
 }
 
 // Rows wider than a block's registers: the row is read three times (from the cache the second and third time).
+// 2048 x 32768 bf16 81 us (268 MB, 3.3 TB/s); a weight at a time instead of a vector 279.
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_fwd_wide_kernel(NormFwd a) {
   constexpr int V = Vec<T>::N;
@@ -245,6 +249,10 @@ struct NormBwd {
 // the columns' sums of dy xhat and dy over all the rows they take, and write dx.  At the end the block joins its row
 // groups' sums in their order (by lane exchange within a wave, then through LDS) into its part.  With LDS_SUMS (16
 // columns a thread, one row group) the columns' sums lie in LDS instead, four of a thread together; 128 of its 160 KB.
+// One pass because the sums are free beside it: dx alone takes 8192 x 4096 bf16 34 us, with the sums 42 and their join 4.5
+// (201 MB, 4.8 TB/s), where a second pass would read 134 MB again.  1M x 64 float 155 us (768 MB, 5.0 TB/s: memory);
+// 4096 x 16384 bf16 101 us with the join, by norm_dx_kernel and norm_cols_kernel 446.  Between rows of whole waves the
+// instructions count too (16 waves a CU are all that its registers hold): a second row in flight gained nothing.
 template <typename T, int G, int NV, int THREADS, bool LDS_SUMS>
 __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(NormBwd a) {
   constexpr int V = Vec<T>::N, kGroups = THREADS / (G < 64 ? 64 : G), kSums = LDS_SUMS ? NV * V / 4 : 0;
@@ -398,7 +406,8 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(NormBwd a) {
   join(db, 1);
 }
 
-// dx of rows wider than a block's registers: a block per row, which it reads twice.
+// dx of rows wider than a block's registers: a block per row, which it reads twice (the second time from the cache):
+// 2048 x 32768 bf16 112 us (403 MB, 3.6 TB/s).
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_dx_kernel(NormBwd a) {
   constexpr int V = Vec<T>::N;
@@ -438,7 +447,7 @@ __global__ __launch_bounds__(THREADS) void norm_dx_kernel(NormBwd a) {
 }
 
 // The rows' sums by column, of rows wider than a block's registers: a block takes 64 vectors of columns and a share of
-// the rows, its 4 waves every fourth row.
+// the rows, its 4 waves every fourth row.  2048 x 32768 bf16 50 us with the join (268 MB, 5.4 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void norm_cols_kernel(NormBwd a) {
   constexpr int V = Vec<T>::N;
@@ -473,7 +482,8 @@ __global__ __launch_bounds__(256) void norm_cols_kernel(NormBwd a) {
   }
 }
 
-// dw and db from the parts, in their order: 64 columns of the [2 d] sums a block, 16 waves over the parts.
+// dw and db from the parts, in their order: 64 columns of the [2 d] sums a block, 16 waves over the parts.  Bound by
+// its loads' latency: 256 parts of 2 x 4096 in 4.5 us (8 MB) with 8 loads of a wave on their way, 8 us with one.
 __global__ __launch_bounds__(1024) void norm_cols_join_kernel(NormBwd a) {
   __shared__ float lds[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;

@@ -277,6 +277,11 @@ __device__ __forceinline__ void pool_floor(Pool<NT>& p, int k, F&& fill) {
 
 // A block takes a row (splits = 1) or a share of one, NT M columns at a time, all in registers: maximum, sums, and with
 // TOP the scores that reach the pool's floor.
+// Without TOP bound by memory, and by one v_exp_f32 an element: 4096 x 65537 bf16 124 to 150 us (537 MB, 3.6 to
+// 4.3 TB/s).  With it the candidates' comparisons and ranks come on top: the same with k = 20 213 us, k = 100 301;
+// 6155 x 3781 fp16, k = 100 62 us (24 without best items, 8 the floor, 18 the candidates, 12 their ranks).  Small calls
+// are a block's latency: 1 x 9500 float, k = 20 7.0 us (load, maximum, sums, floor, ranks, one after the other), 256 rows
+// with k = 100 10.8.  3 x 1000003 float, k = 20: 11 us and 5.7 for the join.
 template <typename T, bool TOP, int NT, int M>
 __global__ __launch_bounds__(NT, 4) void log_prob_kernel(LogProb a) {
   constexpr int V = Vec<T>::N, U = M / V, kWaves = NT / 64;
@@ -533,6 +538,7 @@ struct LogProbBwd {
 
 // A block per row and share of its columns.  The given items' columns are computed first, from the scores and the
 // whole list (the first of equal items sums their gradients in list order), and written last: ds may be s itself.
+// Bound by memory: 4096 x 65537 bf16 215 us (1.07 GB, 5.0 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void log_prob_bwd_kernel(LogProbBwd a) {
   constexpr int V = Vec<T>::N, kMine = KGAT_LOGPROB_MAX_ITEMS / 256;
@@ -612,13 +618,14 @@ constexpr int32_t kTileCols = 8192;   // a 256-thread block's, 32 a thread
 constexpr int32_t kWideCols = 16384;  // a 1024-thread block's, 16 a thread
 
 // One block a row where a row fits a block's registers, or there are rows enough; else shares of whole tiles, about 4
-// blocks a CU in all.
+// blocks a CU in all: 16 rows of 627037 float, k = 64 take 33 us in 77 shares and 36 in 39; 103 rows of 457241, k = 100
+// 78 us in 10 shares and 89 in 19, whose lists are joined too.
 Plan plan_rows(int32_t rows, int32_t cols) {
   if (rows < 1 || cols <= kWideCols || rows >= 4 * kCUs) return {1, cols};
   const int64_t tiles = (static_cast<int64_t>(cols) + kTileCols - 1) / kTileCols;
-  int64_t splits = (4 * kCUs + rows - 1) / rows;
-  if (splits > tiles) splits = tiles;
-  const int64_t per = (tiles + splits - 1) / splits * kTileCols;
+  const int64_t want = (4 * kCUs + rows - 1) / rows;
+  const int64_t each = (2 * tiles + want) / (2 * want);  // tiles of a share, to the nearest
+  const int64_t per = (each < 1 ? 1 : each) * kTileCols;
   if (per >= cols) return {1, cols};
   return {static_cast<int32_t>((cols + per - 1) / per), static_cast<int32_t>(per)};
 }
@@ -633,9 +640,12 @@ int log_prob(LogProb a, hipStream_t st) {
   for (int64_t row0 = 0; row0 < a.rows; row0 += kLaunchRows) {
     a.row0 = static_cast<int32_t>(row0);
     const dim3 grid(a.rows - a.row0 < kLaunchRows ? a.rows - a.row0 : kLaunchRows, a.splits);
+    // The smallest block that holds a row in one step: 8192 rows of 1000, k = 20 29 us with 256 x 8 columns and 51 with
+    // 256 x 32.  Few longer rows: a whole CU's threads for each, 256 rows of 9500, k = 100 10.4 us, 256 x 32 15.7; from
+    // 512 rows on the small block is as fast (13.9 and 13.2), at 2048 rows faster (50 and 32).
     if (a.cols <= 2048)
       hipLaunchKernelGGL((log_prob_kernel<T, TOP, 256, 8>), grid, dim3(256), 0, st, a);
-    else if (a.cols <= kWideCols && a.rows <= 2 * kCUs)  // few rows: each in one step of a whole CU's threads
+    else if (a.cols <= kWideCols && a.rows <= 2 * kCUs)
       hipLaunchKernelGGL((log_prob_kernel<T, TOP, 1024, 16>), grid, dim3(1024), 0, st, a);
     else
       hipLaunchKernelGGL((log_prob_kernel<T, TOP, 256, 32>), grid, dim3(256), 0, st, a);
