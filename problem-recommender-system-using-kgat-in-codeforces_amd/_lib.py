@@ -257,8 +257,8 @@ _SIGNATURES = {
                                            c_vp, c_i64, c_i32, c_vp, c_i64, c_vp]),
     "kgat_act8_pack": (ctypes.c_int, [c_i32, c_vp, c_i64, c_i64, c_i32, c_vp, c_vp, c_vp]),
     "kgat_act8_unpack": (ctypes.c_int, [c_i32, c_vp, c_vp, c_i64, c_i32, c_vp, c_i64, c_vp]),
-    "kgat_act8_wgrad_workspace": (c_i64, [c_i32, c_i64, c_i32, c_i32]),
-    "kgat_act8_wgrad": (ctypes.c_int, [c_i32, c_vp, c_i64, c_vp, c_vp, c_i64, c_i32, c_i32, c_vp, c_vp, c_vp, c_i64,
+    "kgat_act8_wgrad_workspace": (c_i64, [c_i32, c_i32, c_i64, c_i32, c_i32]),
+    "kgat_act8_wgrad": (ctypes.c_int, [c_i32, c_vp, c_i64, c_i32, c_vp, c_vp, c_i64, c_i32, c_i32, c_vp, c_vp, c_vp, c_i64,
                                        c_vp]),
     "kgat_log_prob_workspace": (c_i64, [c_i32, c_i32, c_i32]),
     "kgat_log_prob_fwd": (ctypes.c_int, [c_i32, c_vp, c_i64, c_i32, c_i32, c_f32, c_vp, c_i32, c_i32, c_vp, c_vp, c_vp,

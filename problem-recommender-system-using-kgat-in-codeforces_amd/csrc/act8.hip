@@ -9,6 +9,8 @@
 // The power-of-two scale costs up to one bit against max / 127, and buys exactness: q 2^e has 7 bits of mantissa,
 // so it IS a bf16 number, and the weight gradient dW = dy^T x runs on the bf16 matrix instructions without any
 // further rounding of x.  dy goes in as it is (bf16) or as the exact sum of two (fp16) or three (float) bf16 terms.
+// Where x was fp16 its value is an fp16 number too, and fp16 dy goes in as it is: q has 7 bits, |q 2^e| <= 127 * 2^9, and
+// where 2^e lies below fp16's last bit, 2^-24, x 2^-e is an even integer below 128, so that q 2^e is x itself.
 #include <type_traits>
 
 #include "dense.hpp"
@@ -116,11 +118,13 @@ __global__ __launch_bounds__(256) void act8_unpack_kernel(Unpack a) {
 //
 // bf16 dy, n = 16384, o = d = 4096: 505 to 580 us by the card's clock (0.95 to 1.09 PFLOP/s; a library's product of
 // 16-bit operands 565).  The matrix instructions are busy half of the time at 2.0 GHz; without the decoding the kernel
-// takes 402 us, so what is left of it is LDS reads and their waits beside the products.  Narrow outputs are bound by the
-// decoding, which every tile repeats for its own columns: n = 100003, o = 131, d = 257 in fp16 59 us (6 tiles of 128, 45
-// of whose 96 32 x 32 products hold a column of the result).
+// takes 402 us, so what is left of it is LDS reads and their waits beside the products.  fp16 dy and x the same; fp16 dy
+// as two terms 950, float as three 1370.  Narrow outputs are bound by the decoding, which every tile repeats for its own
+// columns: n = 100003, o = 131, d = 257 in fp16 36 us and 4 for the join (15 tiles of 64; two terms 59).
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef __fp16 half2v __attribute__((ext_vector_type(2)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 
 constexpr int kDepth = 64;                  // rows a step
@@ -138,9 +142,16 @@ struct Wgrad {
   int32_t tiles_o, tiles_d, splits;
 };
 
-template <typename T> constexpr int kPlanes = 3;
-template <> constexpr int kPlanes<__bf16> = 1;
-template <> constexpr int kPlanes<_Float16> = 2;
+// How dy goes in: its type, and whether the matrix instructions take fp16 (x was fp16, as dy is).
+template <typename T, bool HALF>
+struct Dy {
+  typedef T type;
+  static constexpr bool kHalf = HALF;
+  static constexpr int kPlanes = sizeof(T) == 4 ? 3 : std::is_same_v<T, __bf16> || HALF ? 1 : 2;  // terms
+  // LDS buffers: two (the next step is written while one is multiplied) where the operands fit twice beside a second
+  // block, one and two barriers a step for dy's two and three terms.
+  static constexpr int kStages = kPlanes == 1 ? 2 : 1;
+};
 
 __device__ __forceinline__ uint32_t high_halves(uint32_t lo, uint32_t hi) {  // [hi's upper 16 : lo's upper 16]
   return __builtin_amdgcn_perm(hi, lo, 0x07060302);
@@ -196,24 +207,23 @@ __device__ __forceinline__ Quad<T> load_quad(uint64_t base, uint64_t offset, int
   return v;
 }
 
-// LDS buffers: two (the next step is written while one is multiplied) where the operands fit twice beside a second
-// block, one and two barriers a step for dy's two and three terms.
-template <typename T> constexpr int kStages = kPlanes<T> == 1 ? 2 : 1;
-
 // NARROW: dy has fewer than 4 columns.
-template <typename T, int B, bool NARROW>
+template <typename D, int B, bool NARROW>
 __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
-  constexpr int P = kPlanes<T>, kPlane = B * kLdsPitch, kBuffer = (P + 1) * kPlane;
+  typedef typename D::type T;
+  constexpr int P = D::kPlanes, kPlane = B * kLdsPitch, kBuffer = (P + 1) * kPlane;
   // Waves along d; 32 x 32 tiles of a wave along o and d.
   constexpr int kWavesN = B == 64 ? 2 : B / 64, FM = B == 64 ? 2 : B / 64, FN = B == 64 ? 1 : 2;
   static_assert(kWavesN * FN * 32 == B && (2 * B / 64) / kWavesN * FM * 32 == B, "the waves cover the tile");
-  __shared__ __align__(16) char lds[kStages<T> * kBuffer];
+  __shared__ __align__(16) char lds[D::kStages * kBuffer];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int cg = tid % (B / 4), kg = tid / (B / 4);
-  // Blocks b, b + 8, ... run on one XCD: give it neighbouring tiles (4 along o at a time), whose operands its L2 shares.
+  // Blocks b, b + 8, ... run on one XCD: give it neighbouring tiles (4 along o at a time), whose operands its L2 shares
+  // (15 tiles of 100003 rows 41 us, with the blocks in their own order 69).
   const int total = a.tiles_o * a.tiles_d * a.splits;
   int id = blockIdx.x;
-  if (total % 8 == 0) id = id % 8 * (total / 8) + id / 8;
+  const int xcd = id % 8, more = total % 8;
+  id = xcd * (total / 8) + (xcd < more ? xcd : more) + id / 8;
   const int split = id / (a.tiles_o * a.tiles_d);
   id -= split * (a.tiles_o * a.tiles_d);
   const int strip = id / (4 * a.tiles_d), rows_here = a.tiles_o - strip * 4 < 4 ? a.tiles_o - strip * 4 : 4;
@@ -303,7 +313,10 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
       for (int k = 0; k < 4; ++k) {
         const uint32_t lo = y[2 * k].w[j >> 1], hi = y[2 * k + 1].w[j >> 1];
         const uint32_t pair = __builtin_amdgcn_perm(hi, lo, (j & 1) != 0 ? 0x07060302 : 0x05040100);
-        bias[j] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), bf16x2{1, 1}, bias[j], false);
+        if constexpr (D::kHalf)
+          bias[j] = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, pair), half2v{1, 1}, bias[j], false);
+        else
+          bias[j] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), bf16x2{1, 1}, bias[j], false);
         w[k] = pair;
       }
       *reinterpret_cast<u32x4*>(at) = w;
@@ -330,24 +343,25 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)  // exact; NaN where the scale is inf
         f[h] = static_cast<float>(static_cast<int8_t>(x[2 * k + h] >> (8 * j))) * scale[2 * k + h];
-      w[k] = high_halves(__float_as_uint(f[0]), __float_as_uint(f[1]));
+      if constexpr (D::kHalf) w[k] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(f[0], f[1]));
+      else w[k] = high_halves(__float_as_uint(f[0]), __float_as_uint(f[1]));
     }
     *reinterpret_cast<u32x4*>(at + P * kPlane) = w;
   };
   // The operands of 16 rows: a wave's columns of x and of each of dy's terms.
   struct Operands {
-    bf16x8 b[FN], a[P][FM];
+    u32x4 b[FN], a[P][FM];
   };
   auto read = [&](Operands& v, const char* buffer, int s) __attribute__((always_inline)) {
     const int off = (lane & 31) * kLdsPitch + s * 32 + (lane >> 5) * 16;
 #pragma unroll
     for (int n = 0; n < FN; ++n)
-      v.b[n] = *reinterpret_cast<const bf16x8*>(buffer + P * kPlane + (wn + n * 32) * kLdsPitch + off);
+      v.b[n] = *reinterpret_cast<const u32x4*>(buffer + P * kPlane + (wn + n * 32) * kLdsPitch + off);
 #pragma unroll
     for (int p = 0; p < P; ++p)
 #pragma unroll
       for (int m = 0; m < FM; ++m)
-        v.a[p][m] = *reinterpret_cast<const bf16x8*>(buffer + p * kPlane + (wm + m * 32) * kLdsPitch + off);
+        v.a[p][m] = *reinterpret_cast<const u32x4*>(buffer + p * kPlane + (wm + m * 32) * kLdsPitch + off);
   };
   auto multiply = [&](const Operands& v) __attribute__((always_inline)) {
 #pragma unroll
@@ -356,13 +370,18 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
       for (int m = 0; m < FM; ++m)
 #pragma unroll
         for (int n = 0; n < FN; ++n)
-          acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v.a[p][m], v.b[n], acc[m][n], 0, 0, 0);
+          if constexpr (D::kHalf)
+            acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, v.a[p][m]),
+                                                               __builtin_bit_cast(half8, v.b[n]), acc[m][n], 0, 0, 0);
+          else
+            acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v.a[p][m]),
+                                                                __builtin_bit_cast(bf16x8, v.b[n]), acc[m][n], 0, 0, 0);
   };
 
   float scale[8];
   int64_t left = r1 - r0;  // rows not multiplied yet
   fetch(left);
-  if constexpr (kStages<T> == 2) {
+  if constexpr (D::kStages == 2) {
     scales(scale);
 #pragma unroll
     for (int j = 0; j < 4; ++j) store(lds, j, scale);
@@ -510,8 +529,7 @@ double step_us(int planes, int32_t tile, int64_t occ) {
 // once), and the shares' tiles written and read again at 5 TB/s.  One rule for every size: at o = d = 4096 tiles of 256
 // take 504 us and of 128 822 us (fp16 950 and 1140, float 1375 and 1575); at 2048 x 512 (n = 8192) 63 and 50; at
 // o = d = 64 (n = 2048) one share takes 53 us, 16 of them 18.
-template <typename T>
-Splits wgrad_splits(int64_t n, int32_t o, int32_t d) {
+Splits wgrad_splits(int planes, int64_t n, int32_t o, int32_t d) {
   Splits best{};
   double least = 1e300;
   for (int32_t tile = 64; tile <= 256; tile *= 2) {
@@ -526,8 +544,8 @@ Splits wgrad_splits(int64_t n, int32_t o, int32_t d) {
       const int64_t shares = n < 1 ? 1 : (n + per - 1) / per, blocks = tiles * shares;
       const int64_t full = blocks / (kCUs * occ), rest = blocks % (kCUs * occ);
       const double steps = static_cast<double>(per / kDepth) + 3;  // 3: a block's start and end
-      double us = full * steps * step_us(kPlanes<T>, tile, occ);
-      if (rest > 0) us += steps * step_us(kPlanes<T>, tile, (rest + kCUs - 1) / kCUs);
+      double us = full * steps * step_us(planes, tile, occ);
+      if (rest > 0) us += steps * step_us(planes, tile, (rest + kCUs - 1) / kCUs);
       if (shares > 1) us += 3 + 8e-6 / 5 * static_cast<double>(shares) * o * d;
       if (us < least) {
         least = us;
@@ -546,6 +564,7 @@ constexpr int64_t kLaunchThreads = int64_t{1} << 31;
 // f(first row, rows, blocks of 256 threads) for n rows of per_row vectors, a thread each, in as many launches as it takes.
 template <typename F>
 int launch_rows(int64_t n, int64_t per_row, F&& f) {
+  if (n > (int64_t{1} << 52) / per_row) return KGAT_ERR_INVALID;  // more than any memory holds
   const int64_t most = kLaunchThreads / per_row;
   for (int64_t row = 0; row < n; row += most) {
     const int64_t rows = n - row < most ? n - row : most;
@@ -589,26 +608,42 @@ extern "C" int kgat_act8_unpack(int32_t dtype, const int8_t* q, const uint8_t* e
   });
 }
 
-extern "C" int64_t kgat_act8_wgrad_workspace(int32_t dtype, int64_t n, int32_t o, int32_t d) {
-  using namespace kgat;
-  if (!act8_shape_ok(n, d) || o < 1 || o > KGAT_ACT8_MAX_D || dtype < KGAT_F32 || dtype > KGAT_F16) return -1;
-  return (dtype == KGAT_BF16  ? wgrad_splits<__bf16>(n, o, d)
-          : dtype == KGAT_F16 ? wgrad_splits<_Float16>(n, o, d)
-                              : wgrad_splits<float>(n, o, d))
-      .floats(o, d);
+namespace kgat {
+namespace {
+
+// f(Dy<...>{}) for dy's type and the type that x was packed from; an unknown one is KGAT_ERR_INVALID.
+template <typename F>
+int with_dy(int32_t dtype, int32_t x_dtype, F&& f) {
+  if (x_dtype < KGAT_F32 || x_dtype > KGAT_F16) return KGAT_ERR_INVALID;
+  if (dtype == KGAT_F16 && x_dtype == KGAT_F16) return f(Dy<_Float16, true>{});
+  return with_dtype(dtype, [&](auto t) { return f(Dy<decltype(t), false>{}); });
 }
 
-extern "C" int kgat_act8_wgrad(int32_t dtype, const void* dy, int64_t lddy, const int8_t* q, const uint8_t* e,
-                               int64_t n, int32_t o, int32_t d, float* dW, float* db, float* workspace,
-                               int64_t workspace_floats, void* stream) {
+}  // namespace
+}  // namespace kgat
+
+extern "C" int64_t kgat_act8_wgrad_workspace(int32_t dtype, int32_t x_dtype, int64_t n, int32_t o, int32_t d) {
+  using namespace kgat;
+  if (!act8_shape_ok(n, d) || o < 1 || o > KGAT_ACT8_MAX_D) return -1;
+  int64_t floats = -1;
+  with_dy(dtype, x_dtype, [&](auto t) {
+    floats = wgrad_splits(decltype(t)::kPlanes, n, o, d).floats(o, d);
+    return static_cast<int>(KGAT_OK);
+  });
+  return floats;
+}
+
+extern "C" int kgat_act8_wgrad(int32_t dtype, const void* dy, int64_t lddy, int32_t x_dtype, const int8_t* q,
+                               const uint8_t* e, int64_t n, int32_t o, int32_t d, float* dW, float* db,
+                               float* workspace, int64_t workspace_floats, void* stream) {
   using namespace kgat;
   if (!dy || !q || !e || !dW || !act8_shape_ok(n, d) || o < 1 || o > KGAT_ACT8_MAX_D || lddy < 0 ||
-      (reinterpret_cast<uintptr_t>(q) & 15) || dtype < KGAT_F32 || dtype > KGAT_F16)
+      (reinterpret_cast<uintptr_t>(q) & 15))
     return KGAT_ERR_INVALID;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  return with_dtype(dtype, [&](auto t) -> int {
-    using T = decltype(t);
-    const Splits s = wgrad_splits<T>(n, o, d);
+  return with_dy(dtype, x_dtype, [&](auto t) -> int {
+    using D = decltype(t);
+    const Splits s = wgrad_splits(D::kPlanes, n, o, d);
     if (!workspace || workspace_floats < s.floats(o, d)) return KGAT_ERR_WORKSPACE;
     const int64_t size = static_cast<int64_t>(o) * d;
     float* part_b = workspace + s.w * size;
@@ -621,10 +656,10 @@ extern "C" int kgat_act8_wgrad(int32_t dtype, const void* dy, int64_t lddy, cons
       const int64_t blocks = static_cast<int64_t>(s.tiles_o) * s.tiles_d * s.w;
       if (blocks > kLaunchThreads / 512) return KGAT_ERR_INVALID;  // a dW of 2^38 bytes
       const dim3 grid(static_cast<uint32_t>(blocks));
-      if (o < 4) hipLaunchKernelGGL((act8_wgrad_kernel<T, 64, true>), grid, dim3(128), 0, st, a);
-      else if (s.tile == 64) hipLaunchKernelGGL((act8_wgrad_kernel<T, 64, false>), grid, dim3(128), 0, st, a);
-      else if (s.tile == 128) hipLaunchKernelGGL((act8_wgrad_kernel<T, 128, false>), grid, dim3(256), 0, st, a);
-      else hipLaunchKernelGGL((act8_wgrad_kernel<T, 256, false>), grid, dim3(512), 0, st, a);
+      if (o < 4) hipLaunchKernelGGL((act8_wgrad_kernel<D, 64, true>), grid, dim3(128), 0, st, a);
+      else if (s.tile == 64) hipLaunchKernelGGL((act8_wgrad_kernel<D, 64, false>), grid, dim3(128), 0, st, a);
+      else if (s.tile == 128) hipLaunchKernelGGL((act8_wgrad_kernel<D, 128, false>), grid, dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((act8_wgrad_kernel<D, 256, false>), grid, dim3(512), 0, st, a);
       KGAT_LAUNCH_CHECK();
     }
     const int64_t blocks_w = j.parts[0] == 1 ? 0 : blocks_for(size, 64, 1 << 22);

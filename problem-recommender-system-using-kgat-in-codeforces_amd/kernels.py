@@ -1631,8 +1631,11 @@ def act8_wgrad(dy: torch.Tensor, a: Act8, bias: bool = True):
     db = dy.new_empty(o, dtype=torch.float32) if bias else None
     if n == 0:
         return dW.zero_(), None if db is None else db.zero_()
-    ws = dy.new_empty(_lib.lib().kgat_act8_wgrad_workspace(code, n, o, d), dtype=torch.float32)
-    _row_call(dy, "kgat_act8_wgrad", code, dy.data_ptr(), dy.stride(0), a.q.data_ptr(), a.e.data_ptr(), n, o, d,
+    x_code = ROW_DTYPES.get(a.dtype, -1)
+    if x_code < 0:
+        raise ValueError(f"a: packed from float32, bfloat16 or float16 expected, got {a.dtype}")
+    ws = dy.new_empty(_lib.lib().kgat_act8_wgrad_workspace(code, x_code, n, o, d), dtype=torch.float32)
+    _row_call(dy, "kgat_act8_wgrad", code, dy.data_ptr(), dy.stride(0), x_code, a.q.data_ptr(), a.e.data_ptr(), n, o, d,
               dW.data_ptr(), _ptr(db), ws.data_ptr(), ws.numel())
     return dW, db
 

@@ -58,14 +58,14 @@ def test_act8_entries_refuse():
         ({"q": ODD}, INVALID), ({"n": -1}, INVALID), ({"d": 0}, INVALID), ({"ldx": 7}, INVALID),
         ({"n": 1 << 60}, INVALID), ({"n": 0}, 0)])
     lib = L.lib()
-    need = lib.kgat_act8_wgrad_workspace(2, 1000, 64, 96)
+    need = lib.kgat_act8_wgrad_workspace(2, 2, 1000, 64, 96)
     assert need >= 64
     for n, o, d in ((-1, 4, 4), (1, 0, 4), (1, 4, 0), (1, (1 << 20) + 1, 4)):
-        assert lib.kgat_act8_wgrad_workspace(0, n, o, d) == -1
-    assert lib.kgat_act8_wgrad_workspace(4, 1, 1, 1) == -1
-    grad = dict(dtype=2, dy=P, lddy=64, q=P, e=P, n=1000, o=64, d=96, dW=P, db=P, ws=P, wsn=need, st=None)
+        assert lib.kgat_act8_wgrad_workspace(0, 0, n, o, d) == -1
+    assert lib.kgat_act8_wgrad_workspace(4, 0, 1, 1, 1) == lib.kgat_act8_wgrad_workspace(0, 3, 1, 1, 1) == -1
+    grad = dict(dtype=2, dy=P, lddy=64, xt=2, q=P, e=P, n=1000, o=64, d=96, dW=P, db=P, ws=P, wsn=need, st=None)
     refused("kgat_act8_wgrad", grad, [
-        ({"dtype": 4}, INVALID), ({"dy": None}, INVALID), ({"q": None}, INVALID), ({"e": None}, INVALID),
+        ({"dtype": 4}, INVALID), ({"xt": -1}, INVALID), ({"dy": None}, INVALID), ({"q": None}, INVALID), ({"e": None}, INVALID),
         ({"dW": None}, INVALID), ({"q": ODD}, INVALID), ({"lddy": -1}, INVALID), ({"n": -1}, INVALID), ({"o": 0}, INVALID),
         ({"d": 0}, INVALID), ({"ws": None}, WORKSPACE), ({"wsn": need - 1}, WORKSPACE)])
 

@@ -315,6 +315,40 @@ def test_act8_wgrad_products_are_exact(K, dtype):
     assert torch.equal(db, dy[0].float())
 
 
+@pytest.mark.parametrize("x_type,dy_type", [(a, b) for a in TYPES for b in TYPES if a is not b])
+@pytest.mark.parametrize("n,o,d", [(70, 3, 33), (900, 64, 70), (3000, 257, 130), (200, 1500, 1400)])
+def test_act8_wgrad_mixed_types(K, n, o, d, x_type, dy_type):
+    """x packed from one type and dy of another (tolerance: see test_act8_wgrad)."""
+    g = gen(n + o)
+    x = act8_inputs(n, d, x_type, n)
+    dy = randn(g, n, o).to(dy_type)
+    dW, db = K.act8_wgrad(dy, K.act8_pack(x))
+    val, _ = act8_ref(x)
+    few = min(8 * math.sqrt(3 * n) + 32, 3 * n + 1) * 2.0 ** -24
+    close(dW, dy.to(F64).t() @ val, few * (dy.to(F64).abs().t() @ val.abs()) + 2.0 ** -140, "dW")
+    close(db, dy.to(F64).sum(0), SUM * dy.to(F64).abs().sum(0), "db")
+
+
+def test_act8_of_fp16_is_fp16(K):
+    """Every finite fp16 number as a block's largest, beside smaller ones of every size: the values are fp16 numbers, and
+    products with the smallest of them are not lost."""
+    bits = torch.arange(1, 0x7C00, device=DEV, dtype=torch.int32).to(torch.int16)
+    top = bits.view(torch.float16)
+    scale = torch.exp2(-torch.arange(32, device=DEV, dtype=torch.float32))
+    x = (top.float()[:, None] * scale * (1 - 2 * (torch.arange(32, device=DEV) % 2))).half()
+    a = K.act8_pack(x)
+    v = K.act8_unpack(a, torch.float32)
+    assert torch.equal(v.half().float(), v)
+    assert torch.equal(K.act8_unpack(a).float(), v)
+    # one row at a time: a product's only rounding is to 32 bits; 2^-24 is fp16's smallest number
+    for i in (0, 1, 5, 1022, 1023, 1024, 5000, 20000, 31742):
+        for dy in (torch.tensor([[1.0, 2.0 ** -24, -3 * 2.0 ** -24, 65504.0, 2.0 ** -14]], device=DEV).half(),):
+            dW, db = K.act8_wgrad(dy, K.act8_pack(x[i:i + 1]))
+            want = dy.to(F64).t() @ v[i:i + 1].to(F64)
+            assert torch.equal(dW.to(F64), want), i  # 11 + 7 bits: exact in 32
+            assert torch.equal(db, dy[0].float())
+
+
 def test_act8_wgrad_not_a_number(K):
     """A NaN block of x spoils its 32 columns of dW, a NaN or an infinity in dy its row of dW; no row spoils others."""
     g = gen(2)
