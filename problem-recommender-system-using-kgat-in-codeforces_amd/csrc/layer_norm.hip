@@ -503,9 +503,9 @@ __global__ __launch_bounds__(1024) void norm_cols_join_kernel(NormBwd a) {
 }
 
 // The rows' shape: G threads a row, NV vectors a thread, E elements of a thread at most; a narrow row shares its wave
-// with others (1M x 4 float forward 11 us with 2 threads a row, 31 with 8), a wide one takes 1, 2, 3, 4, 6, 8, 12 or 16 waves (a wave without a column costs as
-// much as any: 16384 x 1032 bf16 backward 39 us with 4 waves a row, 35 with 3).  f(G, NV) as integral constants; false: wider than
-// 1024 E columns.
+// with others (1M x 4 float forward 11 us with 2 threads a row, 31 with 8), a wide one takes 1, 2, 3, 4, 6, 8, 12 or 16
+// waves (a wave without a column costs as much as any: 16384 x 1032 bf16 backward 39 us with 4 waves a row, 35 with 3).
+// f(G, NV) as integral constants; false: wider than 1024 E columns.
 template <typename T, int E, typename F>
 bool with_shape(int32_t d, F&& f) {
   constexpr int NV = E / Vec<T>::N;
