@@ -1605,12 +1605,16 @@ def act8_unpack(a: Act8, dtype: torch.dtype | None = None, out: torch.Tensor | N
     with unit stride in the last dimension)."""
     n, d = _req_act8(a)
     if out is None:
-        out = torch.empty(n, d, dtype=dtype or a.dtype, device=a.device)
-    elif dtype is not None and out.dtype != dtype:
-        raise ValueError(f"out has {out.dtype}, not {dtype}")
-    code = _req_rows(out, "out")
-    if tuple(out.shape) != (n, d) or out.device != a.device or (n > 1 and out.stride(0) < d):
-        raise ValueError(f"out: [{n}, {d}] rows that do not overlap expected, on {a.device}")
+        code = ROW_DTYPES.get(dtype or a.dtype)
+        if code is None:
+            raise ValueError(f"dtype: expected float32, bfloat16 or float16, got {dtype or a.dtype}")
+        out = a.q.new_empty((n, d), dtype=dtype or a.dtype)
+    else:
+        if dtype is not None and out.dtype != dtype:
+            raise ValueError(f"out has {out.dtype}, not {dtype}")
+        code = _req_rows(out, "out")
+        if tuple(out.shape) != (n, d) or out.device != a.device or (n > 1 and out.stride(0) < d):
+            raise ValueError(f"out: [{n}, {d}] rows that do not overlap expected, on {a.device}")
     if n:
         _row_call(out, "kgat_act8_unpack", code, a.q.data_ptr(), a.e.data_ptr(), n, d, out.data_ptr(),
                   max(out.stride(0), d))
@@ -1623,7 +1627,7 @@ def act8_wgrad(dy: torch.Tensor, a: Act8, bias: bool = True):
     n, d = _req_act8(a)
     code = _req_rows(dy, "dy")
     o = dy.shape[1]
-    if dy.shape[0] != n or dy.device != a.device:
+    if dy.shape[0] != n or dy.get_device() != a.q.get_device():
         raise ValueError(f"dy: {n} rows on {a.device} expected, got {list(dy.shape)} on {dy.device}")
     if not 1 <= o <= _lib.KGAT_ACT8_MAX_D:
         raise ValueError(f"dy: width must be in [1, {_lib.KGAT_ACT8_MAX_D}], got {o}")
