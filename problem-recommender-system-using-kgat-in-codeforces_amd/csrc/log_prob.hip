@@ -277,13 +277,15 @@ __device__ __forceinline__ void pool_floor(Pool<NT>& p, int k, F&& fill) {
 
 // A block takes a row (splits = 1) or a share of one, NT M columns at a time, all in registers: maximum, sums, and with
 // TOP the scores that reach the pool's floor.
-// Without TOP bound by memory, and by one v_exp_f32 an element: 4096 x 65537 bf16 124 to 150 us (537 MB, 3.6 to
-// 4.3 TB/s).  With it the candidates' comparisons and ranks come on top: the same with k = 20 213 us, k = 100 301;
-// 6155 x 3781 fp16, k = 100 62 us (24 without best items, 8 the floor, 18 the candidates, 12 their ranks).  Small calls
+// Without TOP bound by memory, and nearly so by its instructions (one v_exp_f32 and seven more an element): 4096 x 65537
+// float 184 us (1.07 GB, 5.8 TB/s), bf16 117 (537 MB, 4.6 TB/s; 128 with every load's and element's end of the row
+// looked at).  With it the candidates' comparisons and ranks come on top: bf16 with k = 20 192 us, k = 100 282;
+// 6155 x 3781 fp16, k = 100 60 us (24 without best items, 8 the floor, 17 the candidates, 12 their ranks).  Small calls
 // are a block's latency: 1 x 9500 float, k = 20 7.0 us (load, maximum, sums, floor, ranks, one after the other), 256 rows
 // with k = 100 10.8.  3 x 1000003 float, k = 20: 11 us and 5.7 for the join.
+// 5 waves a SIMD where 16-bit scores leave the registers for them (600 x 200003 bf16, k = 100 142 us; with 4 173).
 template <typename T, bool TOP, int NT, int M>
-__global__ __launch_bounds__(NT, 4) void log_prob_kernel(LogProb a) {
+__global__ __launch_bounds__(NT, sizeof(T) == 2 && NT == 256 ? 5 : 4) void log_prob_kernel(LogProb a) {
   constexpr int V = Vec<T>::N, U = M / V, kWaves = NT / 64;
   __shared__ Stat part[kWaves];
   __shared__ Pool<TOP ? NT : 0> pool;
@@ -299,9 +301,15 @@ __global__ __launch_bounds__(NT, 4) void log_prob_kernel(LogProb a) {
 
   Stat r{-INFINITY, 0.f, 0.f};
   Vec<T> t[U];
-  auto fetch = [&](int64_t base) {
+  auto fetch = [&](int64_t base) __attribute__((always_inline)) {
+    if (base + NT * M <= c1) {  // uniform; a scalar address and the thread's offset
+      const T* at = s + base;
 #pragma unroll
-    for (int u = 0; u < U; ++u) t[u] = load_row(s, base + (u * NT + threadIdx.x) * V, c1);
+      for (int u = 0; u < U; ++u) t[u].raw = *reinterpret_cast<const u32x4_any*>(at + u * NT * V + threadIdx.x * V);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) t[u] = load_row(s, base + (u * NT + threadIdx.x) * V, c1);
+    }
   };
   if constexpr (!TOP) fetch(c0);
   for (int64_t base = c0; base < c1; base += NT * M) {
@@ -312,14 +320,22 @@ __global__ __launch_bounds__(NT, 4) void log_prob_kernel(LogProb a) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       tops[u] = -INFINITY;
+      if (whole || base + u * NT * V < c1) {  // uniform, as the next one: a row's last columns seldom fill a step
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float x = static_cast<float>(t[u].e[j]);
-        if (!whole && base + (u * NT + threadIdx.x) * V + j >= c1) x = -INFINITY;
-        f[u * V + j] = x;
-        tops[u] = max_nan(tops[u], x);
+        for (int j = 0; j < V; ++j) f[u * V + j] = static_cast<float>(t[u].e[j]);
+        if (!whole && base + (u + 1) * NT * V > c1) {
+          const int64_t left = c1 - base - (u * NT + threadIdx.x) * V;
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (j >= left) f[u * V + j] = -INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) tops[u] = max_nan(tops[u], f[u * V + j]);
+        top = max_nan(top, tops[u]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[u * V + j] = -INFINITY;
       }
-      top = max_nan(top, tops[u]);
     }
     if constexpr (!TOP) {  // the next columns are on their way meanwhile (with the candidates' registers: other blocks)
       if (base + NT * M < c1) fetch(base + NT * M);
@@ -329,7 +345,7 @@ __global__ __launch_bounds__(NT, 4) void log_prob_kernel(LogProb a) {
     const bool far = __any(ref.far && r.m != -INFINITY);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (base + u * NT * V >= c1) break;  // uniform: a row's last columns seldom fill a step
+      if (base + u * NT * V >= c1) break;  // uniform
       if (!far) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
