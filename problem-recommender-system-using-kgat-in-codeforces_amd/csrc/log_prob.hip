@@ -280,7 +280,7 @@ __device__ __forceinline__ void pool_floor(Pool<NT>& p, int k, F&& fill) {
 // Without TOP bound by memory, and nearly so by its instructions (one v_exp_f32 and seven more an element): 4096 x 65537
 // float 184 us (1.07 GB, 5.8 TB/s), bf16 117 (537 MB, 4.6 TB/s; 128 with every load's and element's end of the row
 // looked at).  With it the candidates' comparisons and ranks come on top: bf16 with k = 20 192 us, k = 100 282;
-// 6155 x 3781 fp16, k = 100 60 us (24 without best items, 8 the floor, 17 the candidates, 12 their ranks).  Small calls
+// 6155 x 3781 fp16, k = 100 52 us (24 without best items; candidates 17, ranks 12).  Small calls
 // are a block's latency: 1 x 9500 float, k = 20 7.0 us (load, maximum, sums, floor, ranks, one after the other), 256 rows
 // with k = 100 10.8.  3 x 1000003 float, k = 20: 11 us and 5.7 for the join.
 // 5 waves a SIMD where 16-bit scores leave the registers for them (600 x 200003 bf16, k = 100 142 us; with 4 173).
@@ -658,11 +658,16 @@ int log_prob(LogProb a, hipStream_t st) {
     const dim3 grid(a.rows - a.row0 < kLaunchRows ? a.rows - a.row0 : kLaunchRows, a.splits);
     // The smallest block that holds a row in one step: 8192 rows of 1000, k = 20 29 us with 256 x 8 columns and 51 with
     // 256 x 32.  Few longer rows: a whole CU's threads for each, 256 rows of 9500, k = 100 10.4 us, 256 x 32 15.7; from
-    // 512 rows on the small block is as fast (13.9 and 13.2), at 2048 rows faster (50 and 32).
+    // 512 rows on the small block is as fast (13.9 and 13.2), at 2048 rows faster (50 and 32).  Candidates of float scores
+    // want the registers that more waves need: 611 rows of 113711, k = 64 91 us with 16 columns a thread, 109 with 32;
+    // with more of them the steps count (8192 rows of 9500, k = 100 174 and 148), as in 16 bits (219 rows of 436892 109
+    // and 99); a row of 3781 fp16, which is one step of either, 52 and 59 for 6155.
     if (a.cols <= 2048)
       hipLaunchKernelGGL((log_prob_kernel<T, TOP, 256, 8>), grid, dim3(256), 0, st, a);
     else if (a.cols <= kWideCols && a.rows <= 2 * kCUs)
       hipLaunchKernelGGL((log_prob_kernel<T, TOP, 1024, 16>), grid, dim3(1024), 0, st, a);
+    else if (a.cols <= 4096 || (TOP && sizeof(T) == 4 && a.k <= 64))
+      hipLaunchKernelGGL((log_prob_kernel<T, TOP, 256, 16>), grid, dim3(256), 0, st, a);
     else
       hipLaunchKernelGGL((log_prob_kernel<T, TOP, 256, 32>), grid, dim3(256), 0, st, a);
     KGAT_LAUNCH_CHECK();
