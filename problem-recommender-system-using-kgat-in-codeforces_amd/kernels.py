@@ -1497,7 +1497,8 @@ def layer_norm_fwd(x: torch.Tensor, weight: torch.Tensor | None = None, bias: to
     y = torch.empty_like(x) if x.is_contiguous() else x.new_empty((n, d))
     mean = rstd = None
     if stats:
-        mean, rstd = x.new_empty(n, dtype=torch.float32), x.new_empty(n, dtype=torch.float32)
+        mean = x.new_empty(n, dtype=torch.float32)
+        rstd = torch.empty_like(mean)
     if n:
         _row_call(x, "kgat_layer_norm_fwd", code, x.data_ptr(), x.stride(0), w_code, _ptr(weight), _ptr(bias),
                   y.data_ptr(), d, _ptr(mean), _ptr(rstd), n, d, float(eps))
@@ -1521,8 +1522,8 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: 
     _norm_weight(weight, "weight", x)
     w_dtype = torch.float32 if weight is None else weight.dtype
     dx = None if not need_dx else torch.empty_like(x) if x.is_contiguous() else x.new_empty((n, d))
-    dw = x.new_empty(d, dtype=w_dtype) if need_dweight else None
-    db = x.new_empty(d, dtype=w_dtype) if need_dbias else None
+    dw = None if not need_dweight else x.new_empty(d, dtype=w_dtype) if weight is None else torch.empty_like(weight)
+    db = None if not need_dbias else x.new_empty(d, dtype=w_dtype) if weight is None else torch.empty_like(weight)
     ws = None
     if need_dweight or need_dbias:
         if n == 0:
