@@ -7,8 +7,9 @@
 // m, S and W come from one pass: who meets a larger score rescales what it has,
 //   S <- S f,  W <- f (W + delta S),  delta = (old m - new m) scale,  f = e^delta.
 // Exponents are kept in base 2, x = s c - rho with c = scale log2 e and rho = m c rounded: one fma and one v_exp_f32 an
-// element, and rho's rounding is the same in every x and in lse.  Where m c leaves the floats' middle range (rows of
-// the type's lowest or largest value) x = (s - m) c instead, so that equal scores stay equal.
+// element, and rho's rounding is the same in every x and in lse.  x at the maximum is that rounding, m c - rho: 2^-5 at
+// most while |m c| < 2^20.  Farther from zero (a row of nothing but a mask's -1e10) its power would leave the floats' range, so
+// there x = (s - m) c, which is 0 at the maximum.
 //
 // Masked scores (-inf) have p = 0 and count nowhere.  A row of nothing else has no distribution: logp and lse -inf,
 // H 0, gradient 0.  A row with a NaN or a +inf: everything NaN, best items -1, gradient NaN.
@@ -30,11 +31,12 @@ __device__ __forceinline__ float max_nan(float a, float b) { return __builtin_el
 // A maximum m and the reference rho that stands for it in base 2.
 struct Ref {
   float m, rho;
-  bool far;  // m c is no ordinary float
-  __device__ __forceinline__ Ref(float m_, float c) : m(m_), rho(m_ * c), far(!(fabsf(m_ * c) < 1e37f)) {}
+  bool far;  // rho's rounding is not small, or no number
+  __device__ __forceinline__ Ref(float m_, float c) : m(m_), rho(m_ * c), far(!(fabsf(m_ * c) < 0x1p20f)) {}
   __device__ __forceinline__ float operator()(float s, float c) const {
     return far ? (s - m) * c : __builtin_fmaf(s, c, -rho);
   }
+  __device__ __forceinline__ float at_max(float c) const { return far ? 0.f : __builtin_fmaf(m, c, -rho); }  // x of m
 };
 
 // A part of a row: its maximum, and S and W relative to it.
@@ -46,7 +48,8 @@ struct Stat {
 __device__ __forceinline__ Stat rebase(Stat a, float to, float c) {
 #pragma clang fp contract(off)
   const Ref from(a.m, c), ref(to, c);
-  float delta = from.far || ref.far ? (a.m - to) * c : from.rho - ref.rho;
+  // The new x of a score less its old one.
+  float delta = from.far || ref.far ? (a.m - to) * c + (ref.at_max(c) - from.at_max(c)) : from.rho - ref.rho;
   delta = fmaxf(delta, kLow);  // from -inf, or NaN from two of them
   const float f = exp2_fast(delta);
   return {to, a.s * f, f * (a.w + delta * a.s)};

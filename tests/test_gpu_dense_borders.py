@@ -1,0 +1,85 @@
+"""The dense-head operators where they are easily wrong: rows far from zero, statistics at the edge of the floats' range,
+what inference and partly frozen layers leave out, roundings counted exactly and what a call allocates.  Definitions,
+tolerances and helpers are tests/test_gpu_dense.py's."""
+from __future__ import annotations
+
+import math
+import sys
+import weakref
+
+import numpy as np
+import pytest
+import torch
+
+from tests.conftest import load_pkg
+from tests.test_gpu_dense import (F64, SUM, TYPES, act8_inputs, act8_ref, check_logp, close, gen, half_step, least, logp_inputs,
+                                  logp_ref, norm_ref, randn)
+from tests.test_gpu_layers import small_model
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture(scope="module")
+def pkg():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    return load_pkg()
+
+
+@pytest.fixture(scope="module")
+def K(pkg):
+    return sys.modules[pkg.__name__ + ".kernels"]
+
+
+# ---------------------------------------------------------------------------------------------------- log probabilities
+def check_far(K, s, items, scale, k=0):
+    """Against the definition, with no allowance for where the row lies: the differences z to the row's maximum are exact
+    in 32 bits here, an exponent is off by 2^-22 of |z| (the difference times scale and log2 e), sums by SUM."""
+    n, c = s.shape
+    dlogp, dent = torch.ones(n, items.shape[1], device=DEV), torch.ones(n, device=DEV)
+    r = K.log_prob_fwd(s, items, k=k, scale=scale)
+    ref = logp_ref(s, items, k, scale, dlogp, dent)
+    hmax = ref["entropy"].abs() + math.log(c)
+    low = 2.0 ** -21 * hmax + SUM * (1 + hmax)
+    close(r.logp, ref["logp"], low[:, None] + 2.0 ** -22 * ref["logp"].abs(), "logp")
+    close(r.entropy, ref["entropy"], low, "entropy")
+    close(r.lse, ref["lse"], low + 2.0 ** -22 * ref["lse"].abs(), "lse")
+    if k:
+        assert torch.equal(r.top_items, ref["top_items"])
+        close(r.top_logp, ref["top_logp"], low[:, None] + 2.0 ** -22 * ref["top_logp"].abs(), "top")
+    ds = K.log_prob_bwd(s, items, r.stats, dlogp, dent, scale=scale)
+    close(ds, ref["dscores"], ref["size"] * (4 * low[:, None] + 2.0 ** -20 * (1 + low[:, None])) * 4 +
+          half_step(s.dtype) * ref["dscores"].abs() + least(s.dtype), "dscores")
+
+
+@pytest.mark.parametrize("scale", [1.0, 0.37])
+@pytest.mark.parametrize("c", [40, 3000, 9000, 40001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_log_prob_rows_of_one_mask_value(K, dtype, c, scale):
+    """A row of nothing but a mask's finite value (-1e10, -1e30, ...) is uniform, as one of zeros is."""
+    values = [v * sign for v in (1e5, 7e5, 1e7, 1e9, 1e10, 3e10, 1e12, 1e15, 1e20, 1e30, 1e36, 3e37) for sign in (1, -1)]
+    s = torch.tensor(values, dtype=torch.float64, device=DEV).to(dtype)[:, None].expand(-1, c).contiguous()
+    items = torch.tensor([0, c // 2, c - 1], device=DEV).expand(len(values), 3).contiguous()
+    check_far(K, s, items, scale, k=20)
+
+
+@pytest.mark.parametrize("c", [64, 3000, 9000, 40001])
+def test_log_prob_rows_far_from_zero(K, c):
+    """Scores a few steps apart, far from zero: the running maximum rises along the row, falls, and jumps about, over
+    values at which its product with log2 e passes a power of two."""
+    bases = [0.0, 5e4, 726817.0, -726817.0, 2.0 ** 19, 2.0 ** 20, -(2.0 ** 20), 1453635.0]
+    steps = torch.arange(c, device=DEV).to(torch.float64).mul(64 / c).floor() / 16 - 2
+    rows = []
+    for b in bases:
+        rows += [b + steps, b + steps.flip(0), b + steps[torch.randperm(c, device=DEV, generator=gen(c))]]
+    s = torch.stack(rows).float()
+    items = torch.tensor([0, c // 2, c - 1], device=DEV).expand(len(rows), 3).contiguous()
+    check_far(K, s, items, 1.0)
+
+
+@pytest.mark.parametrize("n,c", [(5, 3000), (300, 1100)])
+def test_log_prob_of_1024_items_a_row(K, n, c):
+    """The most given items a row, many of them more than once (the gradients of equal items are summed)."""
+    s, items, dlogp, dent = logp_inputs(n, c, 1024, torch.float32, n)
+    check_logp(K, s, items, 0, 1.0, dlogp, dent)
