@@ -92,22 +92,36 @@ struct NormFwd {
   float eps;
 };
 
+// The statistics from the sums of D = x - mean and of D^2 (inv = 1 / d), mean being a rounded 32-bit sum over d: D is
+// exact near the mean, so what the mean is off by stands in D's own sum, to a rounding of D's size.  `shift` is to be
+// taken from every D; var = sum D^2 / d - shift^2, which is 0 for a constant row, not a rounding below it, and infinite
+// where the squares are.
+struct RowStat {
+  float shift, mean, rstd;
+  __device__ __forceinline__ RowStat(float mean_, float sum, float sum2, float inv, float eps) : shift(sum * inv), mean(mean_ + shift) {
+    const float q = sum2 * inv, s = shift * shift;
+    const float var = s < q ? q - s : q < INFINITY ? 0.f : q;
+    rstd = 1.f / sqrtf(var + eps);
+  }
+};
+
 // G threads hold a row as NV vectors each, and the weights of their columns over all the rows they take (a row's
 // weights are 8 bytes a column: read again for every row they would be up to four times its own bytes, from the
 // cache).  The next row is on its way while one is normalised.  Two passes over the registers, not sums of x and x^2:
-// a row far from 0 keeps its variance.
+// a row far from 0 keeps its digits (see RowStat).
 // Bound by memory: 1M x 64 float 86 us (512 MB, 6.0 TB/s), 8192 x 4096 bf16 24 us (134 MB, 5.5 TB/s).  At odd widths
-// the 16-byte accesses straddle cache lines: 16484 x 1021 bf16 16.6 us (4.1 TB/s), x 1024 13.4.
+// the 16-byte accesses straddle cache lines: 16484 x 1021 bf16 16.1 us (4.2 TB/s), x 1024 13.6.  The correction by D's own sum
+// costs 16-bit rows of 1024 columns and more 2 to 4 % (8192 x 4096 23.8 us without it), narrower and float ones nothing.
 template <typename T, int G, int NV, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_fwd_kernel(NormFwd a) {
   constexpr int V = Vec<T>::N;
   static_assert(THREADS % G == 0, "whole rows");
-  __shared__ float lds[2 * (THREADS / 64)];
+  __shared__ float lds[4 * (THREADS / 64)];
   int turn = 0;
   const int lane = threadIdx.x % G;
   const int64_t step = static_cast<int64_t>(gridDim.x) * (THREADS / G);
   const int64_t first = static_cast<int64_t>(blockIdx.x) * (THREADS / G);
-  const float d = static_cast<float>(a.d);
+  const float d = static_cast<float>(a.d), inv = 1.f / d;
   float w[NV][V], b[NV][V];
   load_columns<T>(a.w, lane, G, a.d, 1.f, w);
   load_columns<T>(a.b, lane, G, a.d, 0.f, b);
@@ -121,7 +135,7 @@ __global__ __launch_bounds__(THREADS) void norm_fwd_kernel(NormFwd a) {
   for (int64_t base = first; base < a.n; base += step) {
     const int64_t row = base + threadIdx.x / G;
     float v[NV][V];
-    float s[1] = {0.f}, q[1] = {0.f};
+    float s[1] = {0.f}, q[2] = {0.f, 0.f};  // q: sums of D and of D^2, D = x - mean
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -136,11 +150,13 @@ __global__ __launch_bounds__(THREADS) void norm_fwd_kernel(NormFwd a) {
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        v[i][j] -= mean;
-        if ((i * G + lane) * V + j < a.d) q[0] += v[i][j] * v[i][j];
+        v[i][j] = (i * G + lane) * V + j < a.d ? v[i][j] - mean : 0.f;
+        q[0] += v[i][j];
+        q[1] += v[i][j] * v[i][j];
       }
     group_sum<G, THREADS>(q, lds, turn);
-    const float rstd = 1.f / sqrtf(q[0] / d + a.eps);
+    const RowStat r(mean, q[0], q[1], inv, a.eps);
+    const float shift = r.shift * r.rstd;
     if (row < a.n) {
       T* y = static_cast<T*>(a.y) + row * a.ldy;
 #pragma unroll
@@ -148,12 +164,12 @@ __global__ __launch_bounds__(THREADS) void norm_fwd_kernel(NormFwd a) {
         const int c = (i * G + lane) * V;
         Vec<T> t;
 #pragma unroll
-        for (int j = 0; j < V; ++j) t.e[j] = static_cast<T>(v[i][j] * rstd * w[i][j] + b[i][j]);
+        for (int j = 0; j < V; ++j) t.e[j] = static_cast<T>((v[i][j] * r.rstd - shift) * w[i][j] + b[i][j]);
         store_row(y, c, a.d, t);
       }
       if (lane == 0 && a.mean != nullptr) {
-        a.mean[row] = mean;
-        a.rstd[row] = rstd;
+        a.mean[row] = r.mean;
+        a.rstd[row] = r.rstd;
       }
     }
   }
@@ -182,17 +198,17 @@ __device__ __forceinline__ void load_weights(const NormVec& w, int64_t c, int32_
 }
 
 // Rows wider than a block's registers: the row is read three times (from the cache the second and third time).
-// 2048 x 32768 bf16 81 us (268 MB, 3.3 TB/s); a weight at a time instead of a vector 279.
+// 2048 x 32768 bf16 83 us (268 MB, 3.2 TB/s); a weight at a time instead of a vector 279.
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_fwd_wide_kernel(NormFwd a) {
   constexpr int V = Vec<T>::N;
-  __shared__ float lds[2 * (THREADS / 64)];
+  __shared__ float lds[4 * (THREADS / 64)];
   int turn = 0;
-  const float d = static_cast<float>(a.d);
+  const float d = static_cast<float>(a.d), inv = 1.f / d;
   for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     T* y = static_cast<T*>(a.y) + row * a.ldy;
-    float s[1] = {0.f}, q[1] = {0.f};
+    float s[1] = {0.f}, q[2] = {0.f, 0.f};
 #pragma unroll 4
     for (int64_t c = threadIdx.x * V; c < a.d; c += THREADS * V) {
       const Vec<T> t = load_row(x, c, a.d);
@@ -206,12 +222,14 @@ __global__ __launch_bounds__(THREADS) void norm_fwd_wide_kernel(NormFwd a) {
       const Vec<T> t = load_row(x, c, a.d);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float e = static_cast<float>(t.e[j]) - mean;
-        if (c + j < a.d) q[0] += e * e;
+        const float e = c + j < a.d ? static_cast<float>(t.e[j]) - mean : 0.f;
+        q[0] += e;
+        q[1] += e * e;
       }
     }
     group_sum<THREADS, THREADS>(q, lds, turn);
-    const float rstd = 1.f / sqrtf(q[0] / d + a.eps);
+    const RowStat r(mean, q[0], q[1], inv, a.eps);
+    const float shift = r.shift * r.rstd;
 #pragma unroll 4
     for (int64_t c = threadIdx.x * V; c < a.d; c += THREADS * V) {
       Vec<T> t = load_row(x, c, a.d);
@@ -219,12 +237,12 @@ __global__ __launch_bounds__(THREADS) void norm_fwd_wide_kernel(NormFwd a) {
       load_weights<T>(a.w, c, a.d, 1.f, w);
       load_weights<T>(a.b, c, a.d, 0.f, b);
 #pragma unroll
-      for (int j = 0; j < V; ++j) t.e[j] = static_cast<T>((static_cast<float>(t.e[j]) - mean) * rstd * w[j] + b[j]);
+      for (int j = 0; j < V; ++j) t.e[j] = static_cast<T>(((static_cast<float>(t.e[j]) - mean) * r.rstd - shift) * w[j] + b[j]);
       store_row(y, c, a.d, t);
     }
     if (threadIdx.x == 0 && a.mean != nullptr) {
-      a.mean[row] = mean;
-      a.rstd[row] = rstd;
+      a.mean[row] = r.mean;
+      a.rstd[row] = r.rstd;
     }
   }
 }

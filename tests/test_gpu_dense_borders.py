@@ -83,3 +83,53 @@ def test_log_prob_of_1024_items_a_row(K, n, c):
     """The most given items a row, many of them more than once (the gradients of equal items are summed)."""
     s, items, dlogp, dent = logp_inputs(n, c, 1024, torch.float32, n)
     check_logp(K, s, items, 0, 1.0, dlogp, dent)
+
+
+# ---------------------------------------------------------------------------------------------------- layer norm
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,d", [(50, 96), (300, 3), (40, 257), (7, 1021), (5, 5000), (9, 9001), (3, 16399), (2, 70001)])
+def test_layer_norm_rows_far_from_zero(K, n, d, dtype):
+    """Rows of spread about 1 around a far mean.  The deviations from a rounded mean are exact or off by 2^-24 of
+    themselves, and their own mean (off by SUM of the mean deviation) corrects the rest: nothing in y grows with the mean.
+    The saved mean is off by its one rounding, which the backward's xhat sees as 2^-24 |mean| / sd."""
+    at = 4096 if dtype == torch.float32 else 60
+    x = (randn(gen(d), n, d) + at).to(dtype)
+    dy = randn(gen(d + 1), n, d, dtype=dtype)
+    y, mean, rstd = K.layer_norm_fwd(x, stats=True)
+    ry, rmean, rrstd, xhat, g, rdx, rdw, rdb = norm_ref(x, None, None, 1e-5, dy)
+    dev = (x.to(F64) - rmean[:, None]).abs().mean(1)
+    close(mean, rmean, 2.0 ** -24 * rmean.abs() + 2 * SUM * dev, "mean")
+    close(rstd, rrstd, 4 * SUM * rrstd, "rstd")
+    close(y, ry, half_step(dtype) * ry.abs() + 4 * SUM * (1 + xhat.abs()) + least(dtype), "y")
+    dx, dw, db = K.layer_norm_bwd(dy, x, mean, rstd)
+    spread = (2.0 ** -24 * rmean.abs() * rrstd + 4 * SUM)[:, None]  # xhat's error
+    ga, gx = g.abs().mean(1, keepdim=True), (g * xhat).abs().mean(1, keepdim=True)
+    # dx = rstd (g - mean g - xhat mean(g xhat)): xhat's error in both places, the sums' and rstd's
+    off = rrstd[:, None] * (spread * (gx + (xhat.abs() + 1) * ga) + 8 * SUM * (g.abs() + ga + (xhat.abs() + 1) * gx))
+    close(dx, rdx, half_step(dtype) * rdx.abs() + off + least(dtype), "dx")
+    close(dw, rdw, (dy.to(F64).abs() * (spread + SUM * xhat.abs())).sum(0) + 2.0 ** -24 * rdw.abs(), "dweight")
+
+
+@pytest.mark.parametrize("d", [3, 40, 1021, 5000, 16399, 70001])
+def test_layer_norm_constant_rows(K, d):
+    """A constant row is its bias wherever it lies.  With D = x - mean, at most 2^-18 |x|, its correction is within
+    (SUM + 2^-23) of D, and 1 / sqrt(eps) = 317 multiplies what is left."""
+    x = torch.tensor([1000.1, -77.7, 0.3, 12345.6], device=DEV)[:, None].expand(4, d).contiguous()
+    b = randn(gen(d), d)
+    y, mean, rstd = K.layer_norm_fwd(x, None, b, 1e-5, stats=True)
+    left = x[:, :1].to(F64).abs() * 2.0 ** -18 * (SUM + 2.0 ** -23) * 317
+    close(y, b.to(F64).expand(4, d), left + 2.0 ** -24 * b.to(F64).abs(), "y")
+    close(mean, x[:, 0], 2.0 ** -24 * x[:, 0].to(F64).abs(), "mean")
+    # rstd, relative: half of var's error over eps, both of its terms being D^2 to 1.5 SUM; eps, the sum, the root and the
+    # quotient are a rounding of 2^-24 each
+    off = 1.5 * SUM * (x[:, 0].to(F64) * 2.0 ** -18).square() / 1e-5 + 2.0 ** -22
+    close(rstd, torch.full((4,), 1e-5 ** -0.5, dtype=F64, device=DEV), 317 * off, "rstd")
+
+
+def test_layer_norm_rows_of_huge_spread(K):
+    """A row whose squares pass the floats' range has an infinite variance: rstd 0, y the bias, no NaN; its neighbours
+    keep theirs."""
+    x, b = randn(gen(1), 3, 1000), randn(gen(2), 1000)
+    x[1] *= 1e27
+    y, mean, rstd = K.layer_norm_fwd(x, None, b, stats=True)
+    assert torch.equal(y[1], b) and rstd[1] == 0 and (rstd[[0, 2]] > 0).all()
