@@ -133,3 +133,21 @@ def test_layer_norm_rows_of_huge_spread(K):
     x[1] *= 1e27
     y, mean, rstd = K.layer_norm_fwd(x, None, b, stats=True)
     assert torch.equal(y[1], b) and rstd[1] == 0 and (rstd[[0, 2]] > 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [5, 8, 33, 1021, 9001, 16399])
+def test_layer_norm_backward_of_a_large_constant_row(K, d, dtype):
+    """mean times rstd is beyond the floats' range, xhat is 0: dx = rstd (g - mean g), at widths that end inside a vector
+    too.  (2^100: the row's sums are exact.)"""
+    x = torch.full((3, d), 2.0 ** 100, device=DEV, dtype=dtype)
+    x[1] = randn(gen(d), d).to(dtype)
+    dy = randn(gen(d + 1), 3, d, dtype=dtype)
+    _, mean, rstd = K.layer_norm_fwd(x, eps=1e-20, stats=True)
+    dx, dw, db = K.layer_norm_bwd(dy, x, mean, rstd)
+    assert torch.isfinite(dw).all() and torch.isfinite(db).all()
+    g = dy.to(F64)[[0, 2]]
+    want = (g - g.mean(1, keepdim=True)) * 1e10
+    # rstd = 1 / sqrt(1e-20 in 32 bits): a rounding of eps, of the root and of the quotient
+    close(dx[[0, 2]], want, half_step(dtype) * want.abs() + 1e10 * SUM * (g.abs() + g.abs().mean(1, keepdim=True)), "dx")
+    assert torch.isfinite(dx[1]).all()
