@@ -4,6 +4,9 @@ probabilities over the item catalogue.
 Each is one autograd node over the typed wrappers of ``kernels`` (csrc/layer_norm.hip, act8.hip, log_prob.hip); tensors
 live on the GPU, in float32, bfloat16 or float16.  Inputs of more than two dimensions are taken as rows of their last
 one.  Gradients of gradients are not available.  The types are the tensors' own: autocast changes nothing.
+
+``needs_input_grad`` is what the inputs ask for, also under ``torch.no_grad``, and inside ``forward`` the grad mode is
+always off: the nodes that keep something for the backward are told the caller's grad mode (``grad``).
 """
 from __future__ import annotations
 
@@ -11,7 +14,7 @@ import torch
 from torch import nn
 from torch.autograd.function import once_differentiable
 
-from . import kernels
+from . import _lib, kernels
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -24,9 +27,9 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, eps):
+    def forward(ctx, x, weight, bias, eps, grad):
         rows = _rows(x)
-        if not any(ctx.needs_input_grad[:3]):
+        if not (grad and any(ctx.needs_input_grad)):
             return kernels.layer_norm_fwd(rows, weight, bias, eps).view(x.shape)
         y, mean, rstd = kernels.layer_norm_fwd(rows, weight, bias, eps, stats=True)
         ctx.save_for_backward(x, mean, rstd, weight)
@@ -40,13 +43,13 @@ class _LayerNorm(torch.autograd.Function):
         dx, dw, db = kernels.layer_norm_bwd(_rows(dy), _rows(x), mean, rstd, weight, *ctx.needs_input_grad[:3])
         if db is not None:
             db = db.to(ctx.bias_dtype)
-        return None if dx is None else dx.view(x.shape), dw, db, None
+        return None if dx is None else dx.view(x.shape), dw, db, None, None
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
                eps: float = 1e-5) -> torch.Tensor:
     """Layer norm over the last dimension, in x's type; weight / bias in float32 or x's type (kernels.layer_norm_fwd)."""
-    return _LayerNorm.apply(x, weight, bias, eps)
+    return _LayerNorm.apply(x, weight, bias, eps, torch.is_grad_enabled())
 
 
 class LayerNorm(nn.LayerNorm):
@@ -75,7 +78,7 @@ def _product(a: torch.Tensor, b: torch.Tensor, trans_b: bool) -> torch.Tensor:
 
 class _LinearAct8(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias):
+    def forward(ctx, x, weight, bias, grad):
         rows = _rows(x)
         kernels._req_rows(rows, "x")
         if weight.device != rows.device or (bias is not None and bias.device != rows.device):
@@ -84,11 +87,13 @@ class _LinearAct8(torch.autograd.Function):
             raise ValueError(f"weight: [out, {rows.shape[1]}] expected, got {list(weight.shape)}")
         if bias is not None and bias.shape != weight.shape[:1]:
             raise ValueError(f"bias: [{weight.shape[0]}] expected, got {list(bias.shape)}")
+        if ctx.needs_input_grad[1] and not 1 <= rows.shape[1] <= _lib.KGAT_ACT8_MAX_D:
+            raise ValueError(f"x: width must be in [1, {_lib.KGAT_ACT8_MAX_D}], got {rows.shape[1]}")
         w = weight.to(rows.dtype)
         y = _product(rows, w, True)
         if bias is not None:
             y = y + bias.to(rows.dtype)
-        if any(ctx.needs_input_grad):
+        if grad and any(ctx.needs_input_grad):
             a = kernels.act8_pack(rows) if ctx.needs_input_grad[1] else None
             ctx.save_for_backward(weight, *((a.q, a.e) if a is not None else ()))
             ctx.rows = (tuple(rows.shape), rows.dtype)
@@ -110,14 +115,14 @@ class _LinearAct8(torch.autograd.Function):
             dW = dW.to(weight.dtype)
         elif ctx.needs_input_grad[2]:
             db = dy.sum(0, dtype=torch.float32)
-        return dx, dW, None if db is None else db.to(ctx.bias_dtype)
+        return dx, dW, None if db is None else db.to(ctx.bias_dtype), None
 
 
 def linear_act8(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None) -> torch.Tensor:
     """``F.linear`` that keeps its input for the backward in 8 bits (1.03 bytes an element against 4 or 2;
     kernels.act8_pack).  The output and the input's gradient are those of the exact input; the weight's gradient is the
     exact product with the 8-bit values, within 2^-7 of each block's largest (kernels.act8_wgrad)."""
-    return _LinearAct8.apply(x, weight, bias)
+    return _LinearAct8.apply(x, weight, bias, torch.is_grad_enabled())
 
 
 class LinearAct8(nn.Linear):

@@ -151,3 +151,42 @@ def test_layer_norm_backward_of_a_large_constant_row(K, d, dtype):
     # rstd = 1 / sqrt(1e-20 in 32 bits): a rounding of eps, of the root and of the quotient
     close(dx[[0, 2]], want, half_step(dtype) * want.abs() + 1e10 * SUM * (g.abs() + g.abs().mean(1, keepdim=True)), "dx")
     assert torch.isfinite(dx[1]).all()
+
+
+# ---------------------------------------------------------------------------------------------------- layers
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+def test_inference_keeps_nothing_for_a_backward(pkg, K, monkeypatch, mode):
+    """Without gradients a linear layer packs no input and a norm writes no statistics; the outputs are the same bits, and
+    what is refused stays refused."""
+    x = randn(gen(1), 30, 64)
+    norm, lin = pkg.layers.LayerNorm(64).to(DEV), pkg.layers.LinearAct8(64, 32).to(DEV)
+    calls = []
+    pack, fwd = K.act8_pack, K.layer_norm_fwd
+    monkeypatch.setattr(K, "act8_pack", lambda t: calls.append("pack") or pack(t))
+
+    def norm_fwd(*a, stats=False):
+        calls.append("stats" if stats else "norm")
+        return fwd(*a, stats=stats)
+
+    monkeypatch.setattr(K, "layer_norm_fwd", norm_fwd)
+    with_grad = lin(norm(x))
+    assert with_grad.requires_grad and calls == ["stats", "pack"]
+    calls.clear()
+    with mode():
+        got = lin(norm(x))
+        for bad in (lambda: lin(x[:, :60]), lambda: lin(x.double()), lambda: norm(x.double()), lambda: lin(x.cpu()),
+                    lambda: pkg.layers.linear_act8(x, lin.weight, lin.bias[:4]),
+                    lambda: pkg.layers.linear_act8(x[:, :0], torch.nn.Parameter(lin.weight[:, :0]))):
+            with pytest.raises(ValueError):
+                bad()
+    assert not got.requires_grad and torch.equal(got, with_grad.detach())
+    assert "pack" not in calls and "stats" not in calls
+
+
+def test_no_gradient_asked_for_keeps_nothing(pkg, K, monkeypatch):
+    x, w = randn(gen(1), 30, 64), randn(gen(2), 8, 64)
+    monkeypatch.setattr(K, "act8_pack", lambda t: pytest.fail("packed"))
+    assert not pkg.layers.linear_act8(x, w).requires_grad
+    b = randn(gen(3), 8).requires_grad_(True)
+    pkg.layers.linear_act8(x, w, b).sum().backward()  # a bias alone needs no input
+    assert torch.equal(b.grad, torch.full((8,), 30.0, device=DEV))
