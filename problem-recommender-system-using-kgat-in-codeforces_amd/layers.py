@@ -67,13 +67,15 @@ class LayerNorm(nn.LayerNorm):
         return layer_norm(x, self.weight, self.bias, self.eps)
 
 
-def _product(a: torch.Tensor, b: torch.Tensor, trans_b: bool) -> torch.Tensor:
-    """a [n, k] times b [k, m] (or its transpose b [m, k]): the library's fp32 GEMM where it takes the widths, else
-    torch's plain product."""
+def _product(a: torch.Tensor, b: torch.Tensor, trans_b: bool, bias: torch.Tensor | None = None) -> torch.Tensor:
+    """a [n, k] times b [k, m] (or its transpose b [m, k]), plus bias [m]: the library's fp32 GEMM where it takes the
+    widths, else torch's plain product.  A 16-bit result is rounded once: the bias goes into the product's 32-bit sum."""
     if a.dtype is torch.float32 and kernels.gemm_supported(a, b):
-        return kernels.gemm(a, b, trans_b=trans_b)
+        y = kernels.gemm(a, b, trans_b=trans_b)
+        return y if bias is None else y.add_(bias)
+    b = b.t() if trans_b else b
     with torch.autocast(a.device.type, enabled=False):
-        return a @ (b.t() if trans_b else b)
+        return a @ b if bias is None else torch.addmm(bias, a, b)
 
 
 class _LinearAct8(torch.autograd.Function):
@@ -90,9 +92,7 @@ class _LinearAct8(torch.autograd.Function):
         if ctx.needs_input_grad[1] and not 1 <= rows.shape[1] <= _lib.KGAT_ACT8_MAX_D:
             raise ValueError(f"x: width must be in [1, {_lib.KGAT_ACT8_MAX_D}], got {rows.shape[1]}")
         w = weight.to(rows.dtype)
-        y = _product(rows, w, True)
-        if bias is not None:
-            y = y + bias.to(rows.dtype)
+        y = _product(rows, w, True, None if bias is None else bias.to(rows.dtype))
         if grad and any(ctx.needs_input_grad):
             a = kernels.act8_pack(rows) if ctx.needs_input_grad[1] else None
             ctx.save_for_backward(weight, *((a.q, a.e) if a is not None else ()))
@@ -120,8 +120,9 @@ class _LinearAct8(torch.autograd.Function):
 
 def linear_act8(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None) -> torch.Tensor:
     """``F.linear`` that keeps its input for the backward in 8 bits (1.03 bytes an element against 4 or 2;
-    kernels.act8_pack).  The output and the input's gradient are those of the exact input; the weight's gradient is the
-    exact product with the 8-bit values, within 2^-7 of each block's largest (kernels.act8_wgrad)."""
+    kernels.act8_pack).  The output, rounded once, and the input's gradient are those of the exact input (products by
+    kgat_gemm_f32 in float32 where the widths are multiples of 4, else torch's); the weight's gradient is the exact product
+    with the 8-bit values, within 2^-7 of each block's largest (kernels.act8_wgrad)."""
     return _LinearAct8.apply(x, weight, bias, torch.is_grad_enabled())
 
 

@@ -190,3 +190,49 @@ def test_no_gradient_asked_for_keeps_nothing(pkg, K, monkeypatch):
     b = randn(gen(3), 8).requires_grad_(True)
     pkg.layers.linear_act8(x, w, b).sum().backward()  # a bias alone needs no input
     assert torch.equal(b.grad, torch.full((8,), 30.0, device=DEV))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,d,o", [(70, 64, 96), (33, 40, 3), (1, 128, 64), (300, 33, 17)])
+def test_linear_act8_rounds_once(pkg, dtype, n, d, o):
+    """16-bit outputs: the product's 32-bit sum (d terms and the bias, 2^-23 of their size a term at the worst), rounded
+    once; a product that nearly cancels the bias keeps its digits."""
+    g = gen(n + d)
+    x, w = randn(g, n, d, dtype=dtype), (randn(g, o, d) * 0.5).to(dtype)
+    b = (randn(g, o) * 4).to(dtype)
+    want = x.to(F64) @ w.to(F64).t() + b.to(F64)
+    size = x.to(F64).abs() @ w.to(F64).abs().t() + b.to(F64).abs()
+    for grad in (False, True):
+        y = pkg.layers.linear_act8(x, w.clone().requires_grad_(grad), b).detach()
+        close(y, want, half_step(dtype) * want.abs() + (d + 1) * 2.0 ** -23 * size + least(dtype), f"y, grad {grad}")
+    assert pkg.layers.linear_act8(x.view(1, n, d), w, b).shape == (1, n, o)
+    assert pkg.layers.linear_act8(x[0], w, b).shape == (o,)
+    assert pkg.layers.linear_act8(x[:0], w, b).shape == (0, o)
+
+
+def test_linear_act8_16_bit_step_in_a_captured_graph(pkg):
+    """Forward and every gradient of a 16-bit layer, replayed on new inputs with eager work between."""
+    g = gen(8)
+    x, dy = randn(g, 500, 64, dtype=torch.bfloat16).requires_grad_(True), randn(g, 500, 48, dtype=torch.bfloat16)
+    w, b = randn(g, 48, 64).requires_grad_(True), randn(g, 48).requires_grad_(True)
+
+    def step():
+        y = pkg.layers.linear_act8(x, w, b)
+        return [y.detach(), *torch.autograd.grad(y, (x, w, b), dy)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for turn in range(4):
+        with torch.no_grad():
+            x.copy_(randn(g, 500, 64))
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [t.clone() for t in got]
+        assert all(torch.equal(p, q) for p, q in zip(kept, step())), turn
