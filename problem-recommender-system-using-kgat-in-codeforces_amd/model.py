@@ -921,10 +921,16 @@ def _frontier_forward(graph, users, pos, neg, X0, ws, drops, seeds, early, marks
 
 
 def _side(sides, l: int) -> torch.Tensor:
-    """Layer l's neighbour sums S_l for its backward, read back from their 8-bit checkpoint where the forward kept one
-    (KGAT.checkpoint_sides)."""
+    """Layer l's neighbour sums S_l for its backward, which reads them once: read back from their 8-bit checkpoint where
+    the forward kept one (KGAT.checkpoint_sides), and the checkpoint let go, so that no more than one layer's sums are
+    there in full beside the checkpoints of the layers below."""
     s = sides[l]
-    return kernels.act8_unpack(s) if isinstance(s, kernels.Act8) else s
+    if isinstance(s, kernels.Act8):
+        sides[l] = None
+        s = kernels.act8_unpack(s)
+    elif s is None:
+        raise RuntimeError("Trying to backward through the graph a second time")
+    return s
 
 
 def _saved(tables, states, l) -> dict:

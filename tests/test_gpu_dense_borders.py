@@ -236,3 +236,32 @@ def test_linear_act8_16_bit_step_in_a_captured_graph(pkg):
         torch.cuda.synchronize()
         kept = [t.clone() for t in got]
         assert all(torch.equal(p, q) for p, q in zip(kept, step())), turn
+
+
+# ---------------------------------------------------------------------------------------------------- KGAT's checkpoints
+@pytest.mark.parametrize("direct", [False, True])
+@pytest.mark.parametrize("dim,layers", [(64, [64, 32, 16]), (256, [256, 128])])
+def test_checkpoint_sides_are_let_go_once_read(pkg, K, monkeypatch, dim, layers, direct):
+    """The backward holds one layer's sums in full, and no checkpoint of a layer that it is done with."""
+    m, U, E = small_model(pkg, dim, layers)
+    m.train()
+    m.direct_backward, m.checkpoint_sides = direct, True
+    rng = np.random.default_rng(2)
+    ids = [torch.from_numpy(rng.integers(0, hi, 64)).to(DEV) for hi in (U, int(E * 0.1), int(E * 0.1))]
+    kept, alive = [], []
+    pack, unpack = K.act8_pack, K.act8_unpack
+
+    def packed(t):
+        a = pack(t)
+        kept.append(weakref.ref(a.q))
+        return a
+
+    def unpacked(a, *more, **named):
+        alive.append(sum(r() is not None for r in kept))
+        return unpack(a, *more, **named)
+
+    monkeypatch.setattr(K, "act8_pack", packed)
+    monkeypatch.setattr(K, "act8_unpack", unpacked)
+    m(*ids, mode=pkg.KGATMode.TRAIN_CF).backward()
+    assert alive == list(range(len(layers), 0, -1))
+    assert not any(r() is not None for r in kept)
