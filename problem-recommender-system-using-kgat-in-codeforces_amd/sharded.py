@@ -1066,6 +1066,16 @@ class RowShardedKGAT(nn.Module):
             cached = self._row_blocks = _RowBlocks(self.shard, K)
         return cached
 
+    @property
+    def checkpoint_sides(self) -> bool:
+        """KGAT.checkpoint_sides is not available here: a shard's forward keeps its neighbour sums in float32."""
+        return False
+
+    @checkpoint_sides.setter
+    def checkpoint_sides(self, on: bool) -> None:
+        if on:
+            raise ValueError("checkpoint_sides: KGAT only, RowShardedKGAT keeps its neighbour sums in float32")
+
     # ------------------------------------------------------------------ state
     @torch.no_grad()
     def load_full_state(self, state_dict: dict) -> None:

@@ -103,3 +103,14 @@ def test_wrappers_refuse_cpu_tensors():
                                                        torch.zeros(3, 1, dtype=torch.uint8), (3, 8), torch.float32))):
         with pytest.raises(ValueError):
             f()
+
+
+def test_row_sharded_model_refuses_checkpoint_sides():
+    """The flag would have no effect there."""
+    sharded = __import__(pkg.__name__ + ".sharded", fromlist=["sharded"])
+    m = sharded.RowShardedKGAT.__new__(sharded.RowShardedKGAT)
+    torch.nn.Module.__init__(m)
+    m.checkpoint_sides = False
+    assert m.checkpoint_sides is False
+    with pytest.raises(ValueError, match="checkpoint_sides"):
+        m.checkpoint_sides = True
