@@ -510,8 +510,9 @@ struct Splits {
   int32_t tiles_o, tiles_d;
   int32_t w;     // row shares
   int64_t per;   // rows of a share
-  int64_t floats(int32_t o, int32_t d) const {  // workspace: the shares' tiles, and their column sums
-    return static_cast<int64_t>(w) * o * (static_cast<int64_t>(d) + 1);
+  // Workspace: the shares' tiles, and their column sums; one share writes its results.
+  int64_t floats(int32_t o, int32_t d) const {
+    return w == 1 ? 0 : static_cast<int64_t>(w) * o * (static_cast<int64_t>(d) + 1);
   }
 };
 
@@ -644,9 +645,9 @@ extern "C" int kgat_act8_wgrad(int32_t dtype, const void* dy, int64_t lddy, int3
   return with_dy(dtype, x_dtype, [&](auto t) -> int {
     using D = decltype(t);
     const Splits s = wgrad_splits(D::kPlanes, n, o, d);
-    if (!workspace || workspace_floats < s.floats(o, d)) return KGAT_ERR_WORKSPACE;
-    const int64_t size = static_cast<int64_t>(o) * d;
-    float* part_b = workspace + s.w * size;
+    const int64_t need = s.floats(o, d), size = static_cast<int64_t>(o) * d;
+    if (need > 0 && (!workspace || workspace_floats < need)) return KGAT_ERR_WORKSPACE;
+    float* part_b = need > 0 ? workspace + s.w * size : nullptr;
     Join j{{workspace, part_b}, {dW, db}, {size, o}, {s.w, s.w}, 0};
     if (n == 0) {  // sums of nothing
       j.parts[0] = j.parts[1] = 0;

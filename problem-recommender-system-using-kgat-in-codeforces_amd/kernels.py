@@ -1639,9 +1639,10 @@ def act8_wgrad(dy: torch.Tensor, a: Act8, bias: bool = True):
     x_code = ROW_DTYPES.get(a.dtype, -1)
     if x_code < 0:
         raise ValueError(f"a: packed from float32, bfloat16 or float16 expected, got {a.dtype}")
-    ws = dy.new_empty(_lib.lib().kgat_act8_wgrad_workspace(code, x_code, n, o, d), dtype=torch.float32)
+    need = _lib.lib().kgat_act8_wgrad_workspace(code, x_code, n, o, d)
+    ws = dy.new_empty(need, dtype=torch.float32) if need else None
     _row_call(dy, "kgat_act8_wgrad", code, dy.data_ptr(), dy.stride(0), x_code, a.q.data_ptr(), a.e.data_ptr(), n, o, d,
-              dW.data_ptr(), _ptr(db), ws.data_ptr(), ws.numel())
+              dW.data_ptr(), _ptr(db), _ptr(ws), need)
     return dW, db
 
 

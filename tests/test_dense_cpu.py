@@ -70,6 +70,15 @@ def test_act8_entries_refuse():
         ({"d": 0}, INVALID), ({"ws": None}, WORKSPACE), ({"wsn": need - 1}, WORKSPACE)])
 
 
+def test_act8_wgrad_of_one_share_needs_no_workspace():
+    """One row's tile is written where it belongs, and so are the zeros of no rows; shares are joined."""
+    need = L.lib().kgat_act8_wgrad_workspace
+    for dtype in range(3):
+        assert need(dtype, dtype, 1, 64, 96) == need(dtype, dtype, 0, 64, 96) == 0
+        assert need(dtype, dtype, 64, 4096, 4096) == 0
+        assert need(dtype, dtype, 100003, 131, 257) >= 2 * 131 * 258
+
+
 def test_log_prob_entries_refuse():
     lib = L.lib()
     need = lib.kgat_log_prob_workspace(2, 200000, 20)

@@ -265,3 +265,22 @@ def test_checkpoint_sides_are_let_go_once_read(pkg, K, monkeypatch, dim, layers,
     m(*ids, mode=pkg.KGATMode.TRAIN_CF).backward()
     assert alive == list(range(len(layers), 0, -1))
     assert not any(r() is not None for r in kept)
+
+
+# ---------------------------------------------------------------------------------------------------- 8-bit checkpoints
+@pytest.mark.parametrize("dtype", TYPES)
+def test_act8_wgrad_of_one_share_allocates_its_results_alone(K, dtype):
+    """Where the rows are not shared out there are no parts to keep: the call's memory is dW and db."""
+    x, dy = randn(gen(1), 64, 1024, dtype=dtype), randn(gen(2), 64, 1000, dtype=dtype)
+    a = K.act8_pack(x)
+    want = K.act8_wgrad(dy, a)
+    del want
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    dW, db = K.act8_wgrad(dy, a)
+    assert torch.cuda.max_memory_allocated() - before <= 4 * 1000 * 1025 + 2048  # an allocation's rounding, twice
+    val, _ = act8_ref(x)
+    size = dy.to(F64).abs().t() @ val.abs()
+    close(dW, dy.to(F64).t() @ val, (8 * math.sqrt(3 * 64) + 32) * 2.0 ** -24 * size, "dW")
+    close(db, dy.to(F64).sum(0), SUM * dy.to(F64).abs().sum(0), "db")
