@@ -129,6 +129,7 @@ typedef float floatx16 __attribute__((ext_vector_type(16)));
 
 constexpr int kDepth = 64;                  // rows a step
 constexpr int kLdsPitch = kDepth * 2 + 16;  // bytes
+constexpr int32_t kNarrow = 4;              // fewer columns of dy are no quad: the NARROW kernel
 
 struct Wgrad {
   const void* dy;
@@ -529,11 +530,11 @@ double step_us(int planes, int32_t tile, int64_t occ) {
 // The tile and the number of row shares with the least estimated time: the blocks' steps (4, 2 or 1 of them on a CU at
 // once), and the shares' tiles written and read again at 5 TB/s.  One rule for every size: at o = d = 4096 tiles of 256
 // take 504 us and of 128 822 us (fp16 950 and 1140, float 1375 and 1575); at 2048 x 512 (n = 8192) 63 and 50; at
-// o = d = 64 (n = 2048) one share takes 53 us, 16 of them 18.
+// o = d = 64 (n = 2048) one share takes 53 us, 16 of them 18.  Outputs of fewer than 4 columns have a kernel of 64 alone.
 Splits wgrad_splits(int planes, int64_t n, int32_t o, int32_t d) {
   Splits best{};
   double least = 1e300;
-  for (int32_t tile = 64; tile <= 256; tile *= 2) {
+  for (int32_t tile = 64; tile <= (o < kNarrow ? 64 : 256); tile *= 2) {
     const int32_t tiles_o = (o + tile - 1) / tile, tiles_d = (d + tile - 1) / tile;
     const int64_t tiles = static_cast<int64_t>(tiles_o) * tiles_d, occ = tile == 256 ? 1 : tile == 128 ? 2 : 4;
     // Shares: 1, 2, 3, 4, 6, 8, 12, ... and as many as fill the chip once.
@@ -657,7 +658,7 @@ extern "C" int kgat_act8_wgrad(int32_t dtype, const void* dy, int64_t lddy, int3
       const int64_t blocks = static_cast<int64_t>(s.tiles_o) * s.tiles_d * s.w;
       if (blocks > kLaunchThreads / 512) return KGAT_ERR_INVALID;  // a dW of 2^38 bytes
       const dim3 grid(static_cast<uint32_t>(blocks));
-      if (o < 4) hipLaunchKernelGGL((act8_wgrad_kernel<D, 64, true>), grid, dim3(128), 0, st, a);
+      if (o < kNarrow) hipLaunchKernelGGL((act8_wgrad_kernel<D, 64, true>), grid, dim3(128), 0, st, a);
       else if (s.tile == 64) hipLaunchKernelGGL((act8_wgrad_kernel<D, 64, false>), grid, dim3(128), 0, st, a);
       else if (s.tile == 128) hipLaunchKernelGGL((act8_wgrad_kernel<D, 128, false>), grid, dim3(256), 0, st, a);
       else hipLaunchKernelGGL((act8_wgrad_kernel<D, 256, false>), grid, dim3(512), 0, st, a);

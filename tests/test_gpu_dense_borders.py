@@ -284,3 +284,17 @@ def test_act8_wgrad_of_one_share_allocates_its_results_alone(K, dtype):
     size = dy.to(F64).abs().t() @ val.abs()
     close(dW, dy.to(F64).t() @ val, (8 * math.sqrt(3 * 64) + 32) * 2.0 ** -24 * size, "dW")
     close(db, dy.to(F64).sum(0), SUM * dy.to(F64).abs().sum(0), "db")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("o", [1, 2, 3])
+@pytest.mark.parametrize("n,d", [(70, 5000), (3000, 5000), (5, 70001)])
+def test_act8_wgrad_of_narrow_outputs_and_wide_inputs(K, n, d, o, dtype):
+    """Every column of dW is written (tolerance: see test_act8_wgrad)."""
+    x, dy = act8_inputs(n, d, dtype, n), randn(gen(n + o), n, o, dtype=dtype)
+    torch.full((o * d + 64,), float("nan"), device=DEV)  # what an unwritten column would show
+    dW, db = K.act8_wgrad(dy, K.act8_pack(x))
+    val, _ = act8_ref(x)
+    few = min(8 * math.sqrt(3 * n) + 32, 3 * n + 1) * 2.0 ** -24
+    close(dW, dy.to(F64).t() @ val, few * (dy.to(F64).abs().t() @ val.abs()) + 2.0 ** -140, "dW")
+    close(db, dy.to(F64).sum(0), SUM * dy.to(F64).abs().sum(0), "db")
