@@ -2,8 +2,9 @@
 //
 // A row's columns are cut into blocks of 32.  With A the largest |x| of a block,
 //   e = floor(log2 A) - 6  (at least -126),   q = clamp(round_half_even(x 2^-e), -127, 127),   value = q 2^e,
-// so |x - value| <= 2^(e-1) <= 2^-7 A (one step, 2^-6 A, where x 2^-e lies above 127.5).  A block that holds an
-// infinity or a NaN has the exponent code 255 and stands for NaN in all its columns: a diverged step stays visible.
+// so |x - value| <= 2^-7 A: A lies in [64, 128) steps of 2^e, rounding costs half a step of 64 or more, and clipping a
+// steps to 127 costs (a - 127) / a < 1 / 128 (at the least e, 2^-127 in place of it).  A block that holds an infinity or
+// a NaN has the exponent code 255 and stands for NaN in all its columns: a diverged step stays visible.
 // Stored: q as int8 [n, 32 ceil(d/32)] (zeros behind column d), the code e + 127 as one byte a block.
 //
 // The power-of-two scale costs up to one bit against max / 127, and buys exactness: q 2^e has 7 bits of mantissa,

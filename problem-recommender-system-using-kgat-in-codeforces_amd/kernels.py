@@ -1588,7 +1588,7 @@ def _req_act8(a) -> tuple[int, int]:
 
 def act8_pack(x: torch.Tensor) -> Act8:
     """x [n, d] in 8 bits with a power-of-two scale for each 32 columns of a row (kgat_act8_pack): within 2^-7 of each
-    block's largest absolute value (2^-6 in its topmost 1/255).  A block with an infinity or a NaN becomes NaN."""
+    block's largest absolute value (or 2^-127).  A block with an infinity or a NaN becomes NaN."""
     code = _req_rows(x, "x")
     n, d = x.shape
     if not 1 <= d <= _lib.KGAT_ACT8_MAX_D:

@@ -297,3 +297,17 @@ def test_act8_wgrad_of_narrow_outputs_and_wide_inputs(K, n, d, o, dtype):
     few = min(8 * math.sqrt(3 * n) + 32, 3 * n + 1) * 2.0 ** -24
     close(dW, dy.to(F64).t() @ val, few * (dy.to(F64).abs().t() @ val.abs()) + 2.0 ** -140, "dW")
     close(db, dy.to(F64).sum(0), SUM * dy.to(F64).abs().sum(0), "db")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_act8_error_bound(K, dtype):
+    """Within 2^-7 of the block's largest everywhere, clipped values too: a block's largest lies in [64, 128) steps,
+    rounding costs at most half a step of 64, clipping a to 127 costs (a - 127) / a < 1 / 128."""
+    g = gen(3)
+    x = randn(g, 500, 320) * torch.exp2(torch.randint(-8, 8, (500, 1), device=DEV, generator=g).float())
+    x[::2, ::32] = torch.linspace(126.5, 127.999, 250, device=DEV)[:, None]  # the topmost steps of a power of two
+    x[::2, 1::32] = -x[::2, ::32]
+    x = x.to(dtype)
+    val = K.act8_unpack(K.act8_pack(x), torch.float32).to(F64)
+    top = x.to(F64).abs().view(500, -1, 32).amax(2).repeat_interleave(32, 1)
+    assert ((val - x.to(F64)).abs() <= top * 2.0 ** -7 + 2.0 ** -127).all()
