@@ -24,6 +24,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLow = -1e30f;  // a base-2 exponent whose power is 0, and whose products with 0 are 0
+constexpr float kNone = -200.f;  // the same, and whose products with any gradient are finite
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }  // NaN wins
@@ -590,7 +591,7 @@ __global__ __launch_bounds__(256) void log_prob_bwd_kernel(LogProbBwd a) {
 
   auto slope = [&](float x, float own) {
     const float b = ref(x, c) - l2, p = exp2_fast(b);
-    return none ? 0.f : a.scale * (own - p * (g + gh * (fmaxf(b, kLow) * kLn2 + h)));
+    return none ? 0.f : a.scale * (own - p * (g + gh * (fmaxf(b, kNone) * kLn2 + h)));
   };
   float mine[kMine];
   int32_t column[kMine];  // -1: not this thread's to write

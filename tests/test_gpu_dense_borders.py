@@ -85,6 +85,15 @@ def test_log_prob_of_1024_items_a_row(K, n, c):
     check_logp(K, s, items, 0, 1.0, dlogp, dent)
 
 
+def test_log_prob_large_entropy_gradients(K):
+    """A loss scale on the entropy term: masked columns get 0, the others what they get without it, scaled."""
+    s, items, dlogp, dent = logp_inputs(6, 700, 2, torch.float32, 3, masked=0.3)
+    r = K.log_prob_fwd(s, items)
+    big = K.log_prob_bwd(s, items, r.stats, dlogp * 2.0 ** 30, dent * 2.0 ** 30)
+    one = K.log_prob_bwd(s, items, r.stats, dlogp, dent)
+    assert torch.isfinite(one).all() and torch.equal(big, one * 2.0 ** 30)  # powers of two: the same bits
+
+
 # ---------------------------------------------------------------------------------------------------- layer norm
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,d", [(50, 96), (300, 3), (40, 257), (7, 1021), (5, 5000), (9, 9001), (3, 16399), (2, 70001)])
