@@ -3,7 +3,7 @@ probabilities over the item catalogue.
 
 Each is one autograd node over the typed wrappers of ``kernels`` (csrc/layer_norm.hip, act8.hip, log_prob.hip); tensors
 live on the GPU, in float32, bfloat16 or float16.  Inputs of more than two dimensions are taken as rows of their last
-one.  Gradients of gradients are not available.  The types are the tensors' own: autocast changes nothing.
+one (``log_probs`` takes two: its items belong to the rows).  Gradients of gradients are not available.  The types are the tensors' own: autocast changes nothing.
 
 ``needs_input_grad`` is what the inputs ask for, also under ``torch.no_grad``, and inside ``forward`` the grad mode is
 always off: the nodes that keep something for the backward are told the caller's grad mode (``grad``).

@@ -247,6 +247,44 @@ def test_linear_act8_16_bit_step_in_a_captured_graph(pkg):
         assert all(torch.equal(p, q) for p, q in zip(kept, step())), turn
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,o", [(100003, 131), (70001, 8), (257, 4096)])
+def test_bias_alone_in_a_captured_graph(pkg, n, o, dtype):
+    """A trained bias beside a frozen weight: the captured backward, replayed on new gradients with eager work between,
+    gives the eager bits, and those are dy's column sums."""
+    g = gen(n)
+    x, w = randn(g, n, 8, dtype=dtype), randn(g, o, 8, dtype=dtype)
+    b, dy = randn(g, o).requires_grad_(True), randn(g, n, o, dtype=dtype)
+
+    def step():
+        return torch.autograd.grad(pkg.layers.linear_act8(x, w, b), b, dy)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for turn in range(4):
+        dy.copy_(randn(g, n, o))
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = got.clone()
+        assert torch.equal(kept, step()), turn
+        close(kept, dy.to(F64).sum(0), SUM * dy.to(F64).abs().sum(0), f"db, turn {turn}")
+
+
+def test_log_probs_takes_two_dimensions(pkg):
+    """The one layer that does: its items belong to the rows."""
+    for bad in (lambda: pkg.layers.log_probs(torch.zeros(2, 3, 40, device=DEV), torch.zeros(6, 1, dtype=torch.int64, device=DEV)),
+                lambda: pkg.layers.log_probs(torch.zeros(40, device=DEV), torch.zeros(1, 1, dtype=torch.int64, device=DEV))):
+        with pytest.raises(ValueError):
+            bad()
+
+
 # ---------------------------------------------------------------------------------------------------- KGAT's checkpoints
 @pytest.mark.parametrize("direct", [False, True])
 @pytest.mark.parametrize("dim,layers", [(64, [64, 32, 16]), (256, [256, 128])])
