@@ -117,11 +117,12 @@ __global__ __launch_bounds__(256) void act8_unpack_kernel(Unpack a) {
 // v_mfma_f32_32x32x16_bf16.  Column 4 c + j of the tile lies at LDS row (B / 4) j + c: the threads of a row write
 // neighbouring LDS rows at a pitch of 36 dwords, which spreads 16 of them over all 64 banks.
 //
-// bf16 dy, n = 16384, o = d = 4096: 505 to 580 us by the card's clock (0.95 to 1.09 PFLOP/s; a library's product of
-// 16-bit operands 565).  The matrix instructions are busy half of the time at 2.0 GHz; without the decoding the kernel
-// takes 402 us, so what is left of it is LDS reads and their waits beside the products.  fp16 dy and x the same; fp16 dy
-// as two terms 950, float as three 1370.  Narrow outputs are bound by the decoding, which every tile repeats for its own
-// columns: n = 100003, o = 131, d = 257 in fp16 36 us and 4 for the join (15 tiles of 64; two terms 59).
+// bf16 dy, n = 16384, o = d = 4096: 517 us called again and again on the same operands (1.06 PFLOP/s; a library's
+// product of 16-bit operands 565), 580 to 716, mean 631, in a trace of the first 20 calls with their packs.  The matrix
+// instructions are busy half of the time at 2.0 GHz; without the decoding the kernel takes 402 us, so what is left of it is
+// LDS reads and their waits beside the products.  fp16 dy and x 531; fp16 dy as two terms 950, float as three 1374.
+// Narrow outputs are bound by the decoding, which every tile repeats for its own columns: n = 100003, o = 131, d = 257 in
+// fp16 36 us and 4 for the join (15 tiles of 64; two terms 59).
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -477,7 +478,7 @@ __global__ __launch_bounds__(2 * B) void act8_wgrad_kernel(Wgrad a) {
 }
 
 // Sums of parts, in their order: the first blocks take dW's elements, the others db's.  64 elements a block at a time,
-// its 4 waves every fourth part.  83 parts of 131 x 257 in 5 us (11 MB): launch and latency.
+// its 4 waves every fourth part.  68 parts of 131 x 257 in 4.6 us (9 MB): launch and latency.
 struct Join {
   const float* part[2];
   float* out[2];

@@ -267,8 +267,8 @@ struct NormBwd {
 // the columns' sums of dy xhat and dy over all the rows they take, and write dx.  At the end the block joins its row
 // groups' sums in their order (by lane exchange within a wave, then through LDS) into its part.  With LDS_SUMS (16
 // columns a thread, one row group) the columns' sums lie in LDS instead, four of a thread together; 128 of its 160 KB.
-// One pass because the sums are free beside it: dx alone takes 8192 x 4096 bf16 34 us, with the sums 42 and their join 4.5
-// (201 MB, 4.8 TB/s), where a second pass would read 134 MB again.  1M x 64 float 155 us (768 MB, 5.0 TB/s: memory);
+// One pass because the sums are free beside it: dx alone takes 8192 x 4096 bf16 34 us, with the sums 41 and their join 4.5
+// (201 MB, 4.9 TB/s), where a second pass would read 134 MB again.  1M x 64 float 155 us (768 MB, 5.0 TB/s: memory);
 // 4096 x 16384 bf16 101 us with the join, by norm_dx_kernel and norm_cols_kernel 446.  Between rows of whole waves the
 // instructions count too (16 waves a CU are all that its registers hold): a second row in flight gained nothing.
 template <typename T, int G, int NV, int THREADS, bool LDS_SUMS>
