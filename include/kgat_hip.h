@@ -981,9 +981,10 @@ int kgat_act8_unpack(int32_t dtype, const int8_t *q, const uint8_t *e, int64_t n
                      void *stream);
 /* A linear layer's weight gradient from its checkpointed input: dW [o][d] = dy^T x, db [o] (nullable) = the column
  * sums of dy [n, o] of dtype.  x_dtype: the type that x was packed from.  The products are exact (fp16 matrix
- * instructions where both are fp16, else bf16 ones with dy as one to three terms) and summed in 32 bits.  An infinity or a
- * NaN in dy reaches its row of dW as infinities or NaN, and its db.  n = 0 writes zeros.  workspace:
- * kgat_act8_wgrad_workspace floats, 0 (and none) where the rows are not shared out. */
+ * instructions where both are fp16, else bf16 ones with dy as one to three terms; a float dy's digits below bf16's last,
+ * 2^-133, are left out) and summed in 32 bits.  An infinity or a NaN in dy reaches its row of dW as infinities or NaN,
+ * and its db.  n = 0 writes zeros.  workspace: kgat_act8_wgrad_workspace floats, 0 (and none) where the rows are not
+ * shared out. */
 int64_t kgat_act8_wgrad_workspace(int32_t dtype, int32_t x_dtype, int64_t n, int32_t o, int32_t d);
 int kgat_act8_wgrad(int32_t dtype, const void *dy, int64_t lddy, int32_t x_dtype, const int8_t *q, const uint8_t *e,
                     int64_t n, int32_t o, int32_t d, float *dW, float *db, float *workspace, int64_t workspace_floats,

@@ -9,7 +9,8 @@
 //
 // The power-of-two scale costs up to one bit against max / 127, and buys exactness: q 2^e has 7 bits of mantissa,
 // so it IS a bf16 number, and the weight gradient dW = dy^T x runs on the bf16 matrix instructions without any
-// further rounding of x.  dy goes in as it is (bf16) or as the exact sum of two (fp16) or three (float) bf16 terms.
+// further rounding of x.  dy goes in as it is (bf16) or as the exact sum of two (fp16) or three (float) bf16 terms: of a
+// float its digits down to bf16's last, 2^-133, which is all of them from 2^-110 up.
 // Where x was fp16 its value is an fp16 number too, and fp16 dy goes in as it is: q has 7 bits, |q 2^e| <= 127 * 2^9, and
 // where 2^e lies below fp16's last bit, 2^-24, x 2^-e is an even integer below 128, so that q 2^e is x itself.
 #include <type_traits>

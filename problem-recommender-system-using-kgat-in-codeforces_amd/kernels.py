@@ -1624,7 +1624,8 @@ def act8_unpack(a: Act8, dtype: torch.dtype | None = None, out: torch.Tensor | N
 
 def act8_wgrad(dy: torch.Tensor, a: Act8, bias: bool = True):
     """(dW, db) of a linear layer y = x W^T + b from its checkpointed input: dW = dy^T x float32 [o, d] and db = the
-    column sums of dy float32 [o] (None without ``bias``).  Exact products, summed in 32 bits (kgat_act8_wgrad)."""
+    column sums of dy float32 [o] (None without ``bias``).  Exact products, summed in 32 bits (kgat_act8_wgrad); dW takes a
+    float32 dy's digits down to 2^-133."""
     n, d = _req_act8(a)
     code = _req_rows(dy, "dy")
     o = dy.shape[1]

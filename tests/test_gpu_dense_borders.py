@@ -358,3 +358,17 @@ def test_act8_error_bound(K, dtype):
     val = K.act8_unpack(K.act8_pack(x), torch.float32).to(F64)
     top = x.to(F64).abs().view(500, -1, 32).amax(2).repeat_interleave(32, 1)
     assert ((val - x.to(F64)).abs() <= top * 2.0 ** -7 + 2.0 ** -127).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_act8_wgrad_of_tiny_gradients(K, dtype):
+    """dy down to its type's smallest numbers: 16-bit types keep every digit, a float's third bf16 term ends at 2^-133."""
+    x = randn(gen(1), 64, 40) * 2.0 ** 60
+    a = K.act8_pack(x)
+    val, _ = act8_ref(x)
+    for e in (-8, -14, -20, -24) if dtype == torch.float16 else (-60, -109, -118, -126, -130, -133):
+        dy = (torch.randn(64, 48, device=DEV, dtype=F64, generator=gen(-e)) * 2.0 ** e).float().to(dtype)
+        dW, db = K.act8_wgrad(dy, a)
+        lost = 2.0 ** -133 * val.abs().sum(0) if dtype == torch.float32 else 0.0
+        close(dW, dy.to(F64).t() @ val, (8 * math.sqrt(3 * 64) + 32) * 2.0 ** -24 * (dy.to(F64).abs().t() @ val.abs()) + lost, f"dW {e}")
+        close(db, dy.to(F64).sum(0), SUM * dy.to(F64).abs().sum(0), f"db {e}")
